@@ -59,6 +59,12 @@ OP_ARGTYPES = {
     "tensor_sdpa_device_f32": [_P, _P, _P, _P, _F, _I, _P],
     "tensor_sdpa_device_f16": [_P, _P, _P, _P, _F, _I, _P],
     "tensor_linear_q8_0_f16": [_P, _P, _P], "tensor_linear_q4_0_f16": [_P, _P, _P],
+    "tensor_kv_cache_append_f32": [_P, _P, _P, _P], "tensor_kv_cache_append_f16": [_P, _P, _P, _P],
+    "tensor_kv_cache_truncate": [_P, _P],
+    "tensor_kv_cache_read_f32": [_P, _P, _P], "tensor_kv_cache_read_f16": [_P, _P, _P],
+    "tensor_kv_cache_attention_f32": [_P, _P, _P, _F, _I, _P, _P],
+    "tensor_kv_cache_attention_f16": [_P, _P, _P, _F, _I, _P, _P],
+    "tensor_kv_cache_evict": [_P, _P, _Z, _Z, _Z, _P, _P, _P],
     "tensor_device_synchronize": [],
 }
 
@@ -158,6 +164,15 @@ def load_library(path: str = LIB_PATH) -> ctypes.CDLL:
     lib.tensor_dtype_size.restype = _Z
     lib.tensor_dtype_name.argtypes = [_I]
     lib.tensor_dtype_name.restype = ctypes.c_char_p
+    lib.tensor_kv_cache_create.argtypes = [_Z, _Z, _Z, _Z, _Z, ctypes.POINTER(_P), ctypes.c_char_p, _Z]
+    lib.tensor_kv_cache_create.restype = _I
+    lib.tensor_kv_cache_free.argtypes = [_P]
+    lib.tensor_kv_cache_free.restype = None
+    lib.tensor_kv_cache_length.argtypes = [_P, _Z]
+    for name in ("tensor_kv_cache_capacity", "tensor_kv_cache_byte_length"):
+        getattr(lib, name).argtypes = [_P]
+    for name in ("tensor_kv_cache_length", "tensor_kv_cache_capacity", "tensor_kv_cache_byte_length"):
+        getattr(lib, name).restype = _Z
     lib.tensor_quantize_linear_weight_f16.argtypes = [_P, _Z, _Z, _I, ctypes.POINTER(_P),
                                                       ctypes.c_char_p, _Z]
     lib.tensor_quantize_linear_weight_f16.restype = _I
@@ -228,6 +243,42 @@ class Tensor:
             pass
 
 
+class KvCache:
+    """Owns one TensorKvCache: keys and values of one layer held in 8 bits.
+    Passed to Sdk.call like a Tensor; host arrays of counts or lengths are
+    ctypes arrays of c_uint32, one number per sequence."""
+
+    def __init__(self, sdk: "Sdk", batch: int, kv_heads: int, capacity: int, head_dim: int,
+                 value_dim: Optional[int] = None):
+        self.sdk, self.batch = sdk, batch
+        handle = ctypes.c_void_p()
+        err = ctypes.create_string_buffer(512)
+        if not sdk.lib.tensor_kv_cache_create(batch, kv_heads, capacity, head_dim,
+                                              head_dim if value_dim is None else value_dim,
+                                              ctypes.byref(handle), err, 512):
+            raise SdkError(err.value.decode())
+        self.handle = handle.value
+
+    @property
+    def lengths(self) -> list[int]:
+        return [int(self.sdk.lib.tensor_kv_cache_length(self.handle, b)) for b in range(self.batch)]
+
+    @property
+    def nbytes(self) -> int:
+        return int(self.sdk.lib.tensor_kv_cache_byte_length(self.handle))
+
+    def free(self) -> None:
+        if self.handle:
+            self.sdk.lib.tensor_kv_cache_free(self.handle)
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.free()
+        except Exception:
+            pass
+
+
 class Sdk:
     """Library handle with Tensor construction and checked op calls."""
 
@@ -244,6 +295,10 @@ class Sdk:
 
     def tensor(self, dtype: str, shape: Sequence[int], device: bool = True) -> Tensor:
         return Tensor(self, dtype, shape, device)
+
+    def kv_cache(self, batch: int, kv_heads: int, capacity: int, head_dim: int,
+                 value_dim: Optional[int] = None) -> KvCache:
+        return KvCache(self, batch, kv_heads, capacity, head_dim, value_dim)
 
     def from_numpy(self, array: np.ndarray, dtype: Optional[str] = None,
                    device: bool = True) -> Tensor:
@@ -275,7 +330,7 @@ class Sdk:
 
     @staticmethod
     def _arg(a):
-        if isinstance(a, Tensor):
+        if isinstance(a, (Tensor, KvCache)):
             return a.handle
         if isinstance(a, ctypes.Structure):
             return ctypes.addressof(a)
