@@ -7,7 +7,7 @@
  * scale: with a the largest |x| of the block, x being the appended elements
  * rounded to f16,
  *     scale = a / 127,   code = 127 x / a rounded to nearest, ties to even,
- * and stand for code * scale. The tokens of the last, partial block are held
+ * and stand for the f32 product code * scale. The tokens of the last, partial block are held
  * in f16 until the block is full, so what a cache holds does not depend on
  * how its tokens were split over calls.
  *

@@ -42,7 +42,7 @@ typedef float f32x2 __attribute__((ext_vector_type(2)));
 constexpr uint32_t kThreads = 256;
 constexpr uint32_t kWaves = 4;
 constexpr uint32_t kRows = 16;         // packed rows of a wave
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr double kLog2e = 1.4426950408889634;
 constexpr float kUnitRange = 8.0f;     // a value scale further from the unit moves it
 // P of a row whose maximum is M is 2^(s - M + kHeadroom): as far up in f16 as the
 // unit's range and the lazy rescale of the maximum (by more than 2^kLazy) leave
@@ -60,11 +60,13 @@ template <typename S> struct Args {
     f32x2 *part_ml;      // [part][row] running maximum (log2 units) and sum
     f32x2 *row_ml;       // [row] maximum and 1 / sum (0: the row adds no weight), or null
     float *weights;
+    float *scores;       // [row][score_stride] scores in log2 units, or null
     size_t rows;         // of all sequences
+    size_t score_stride;
     size_t weight_stride;
     uint32_t weight_tokens;
     uint32_t first, pairs, group, n, parts, row_group0;
-    float scale2;        // scale * log2 e
+    double scale2;       // scale * log2 e
     int causal;
     Counts count;
 };
@@ -228,8 +230,12 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(Args<S> a) {
 
     // one block: kf(u, s) and vf(j, s) give the A operands
     auto step = [&](uint32_t t, Meta meta, auto kf, auto vf, auto keys_done) {
-        const float factor = meta.k_scale * a.scale2 * q.factor;
-        float p[16];
+        const double factor2 = (double)meta.k_scale * a.scale2;
+        const float factor = (float)factor2 * q.factor;
+        // f32: what rounding takes off the factor and the scores is added back in
+        // the exponent (scores of 10 would be off by 1e-6 of their weight)
+        const float factor_rest = (float)(factor2 - (double)(float)factor2) * q.factor;
+        float p[16], rest[kPair ? 16 : 1];
 #pragma unroll
         for (uint32_t u = 0; u < 4; ++u) {
             f32x4 acc = {0, 0, 0, 0};
@@ -240,7 +246,13 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(Args<S> a) {
                 if constexpr (kPair) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q.lo[s], acc, 0, 0, 0);
             }
 #pragma unroll
-            for (uint32_t e = 0; e < 4; ++e) p[4 * u + e] = acc[e] * factor;
+            for (uint32_t e = 0; e < 4; ++e) {
+                p[4 * u + e] = acc[e] * factor;
+                if constexpr (kPair) {
+                    const float off = __builtin_fmaf(acc[e], factor, -p[4 * u + e]) + acc[e] * factor_rest;
+                    rest[4 * u + e] = fabsf(p[4 * u + e]) < 1e30f ? off : 0.0f;
+                }
+            }
         }
         keys_done();
         if ((int)(t * kTokens + kTokens) > least || meta.marked != 0) {
@@ -250,6 +262,12 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(Args<S> a) {
                 if (mine >> e & 1) p[e] = __builtin_nanf("");
                 if ((int)(t * kTokens + 16 * g + e) >= seen) p[e] = neg_inf;
             }
+        }
+        if (a.scores != nullptr && live) {
+            float *const out = a.scores + row * a.score_stride + t * kTokens + 16 * g;
+#pragma unroll
+            for (uint32_t e = 0; e < 16; e += 4)
+                *reinterpret_cast<f32x4 *>(out + e) = f32x4{p[e], p[e + 1], p[e + 2], p[e + 3]};
         }
         float top = neg_inf;
 #pragma unroll
@@ -277,7 +295,9 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(Args<S> a) {
         float add = 0.0f;
 #pragma unroll
         for (uint32_t e = 0; e < 16; ++e) {
-            const float x = __builtin_amdgcn_exp2f(p[e] - base);
+            float x = p[e] - base;
+            if constexpr (kPair) x += rest[e];
+            x = __builtin_amdgcn_exp2f(x);
             const float y = x * ratio;
             ph[e / 8][e % 8] = (_Float16)y;
             if constexpr (kPair) {
@@ -383,7 +403,10 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(Args<S> a) {
             for (uint32_t k = 0; k < kWaves; ++k) v += lds_o[k][j][lane] * w[k];
             if (writes) store_out(out, c.vdim, 16 * j + 4 * g, finish(v, top, total));
         }
-        if (a.row_ml != nullptr && writes && g == 0 && wave == 0) a.row_ml[row] = weight_terms(top, total);
+        if (writes && g == 0 && wave == 0) {
+            if (a.row_ml != nullptr) a.row_ml[row] = weight_terms(top, total);
+            if (a.scores != nullptr) a.part_ml[row] = f32x2{top, total};
+        }
     } else {
         float *const out = a.part_o + ((size_t)part * a.rows + row) * c.vdim;
 #pragma unroll
@@ -397,30 +420,65 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(Args<S> a) {
     }
 }
 
-// Merges the parts of a row: one workgroup per row, its waves take every fourth
-// part, a lane four output elements.
+// Maximum and sum of a row from its parts', by one wave.
+__device__ inline f32x2 fold_ml(const f32x2 *ml, uint32_t parts, size_t rows, uint32_t lane) {
+    float top = -__builtin_inff(), total = 0.0f;
+    for (uint32_t s = lane; s < parts; s += kWave) top = fmaxf(top, ml[s * rows].x);
+    top = wave_max(top);
+    for (uint32_t s = lane; s < parts; s += kWave) {
+        const f32x2 v = ml[s * rows];
+        total += (top == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(v.x - top)) * v.y;
+    }
+    return f32x2{top, wave_sum(total)};
+}
+
+// Merges the parts of a row, one workgroup per row: its waves take every fourth
+// part, a lane four output elements. The workgroups after `folds` do 256 tokens
+// of one (sequence, head) each: their weights from the stored scores.
 template <typename S>
-__global__ __launch_bounds__(kThreads) void kv_fold_kernel(Args<S> a, uint32_t row0) {
+__global__ __launch_bounds__(kThreads) void kv_fold_kernel(Args<S> a, uint32_t folds, uint32_t token_groups) {
     __shared__ f32x4 lds_o[kWaves][kWave];
-    __shared__ float lds_l[kWaves];
+    __shared__ f32x2 lds_ml[kRows];
     const View &c = a.c;
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x / kWave;
-    const uint32_t in_head = a.group * a.n, of_pairs = row0 + blockIdx.x;
-    const uint32_t b = of_pairs / (in_head * c.heads);
-    if (of_pairs % a.n >= a.count.n[b]) return;
-    const size_t row = (size_t)a.first * c.heads * in_head + of_pairs;
-    float top = -__builtin_inff();
-    for (uint32_t s = 0; s < a.parts; ++s) top = fmaxf(top, a.part_ml[(size_t)s * a.rows + row].x);
+    const uint32_t lane = threadIdx.x & 63, wave = (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const uint32_t in_head = a.group * a.n;
+    if (blockIdx.x >= folds) {
+        const uint32_t tg = (blockIdx.x - folds) % token_groups, pair = (blockIdx.x - folds) / token_groups;
+        const uint32_t b = pair / c.heads, seq = a.first + b, length = min(c.length[seq], a.weight_tokens);
+        const size_t head = (size_t)seq * c.heads + pair % c.heads;
+        if (tg * kThreads >= length) return;
+        for (uint32_t r = wave; r < in_head; r += kWaves) {
+            const size_t row = head * in_head + r;
+            const f32x2 ml = r % a.n < a.count.n[b] ? fold_ml(a.part_ml + row, a.parts, a.rows, lane)
+                                                    : f32x2{-__builtin_inff(), 0.0f};
+            if (lane == 0) lds_ml[r] = weight_terms(ml.x, ml.y);
+        }
+        __syncthreads();
+        const uint32_t t = tg * kThreads + threadIdx.x;
+        if (t >= length) return;
+        float total = 0.0f;
+        for (uint32_t r = 0; r < in_head; ++r) {
+            const f32x2 ml = lds_ml[r];
+            if (ml.y != 0.0f)
+                total += __builtin_amdgcn_exp2f(a.scores[(head * in_head + r) * a.score_stride + t] - ml.x) * ml.y;
+        }
+        a.weights[head * a.weight_stride + t] += total;
+        return;
+    }
+    const uint32_t b = blockIdx.x / (in_head * c.heads);
+    if (blockIdx.x % a.n >= a.count.n[b]) return;
+    const size_t row = (size_t)a.first * c.heads * in_head + blockIdx.x;
+    const f32x2 all = fold_ml(a.part_ml + row, a.parts, a.rows, lane);
     f32x4 v = {0, 0, 0, 0};
-    float total = 0.0f;
     const uint32_t d = 4 * lane;
+    const bool fours = c.vdim % 4 == 0;
+#pragma unroll 4
     for (uint32_t s = wave; s < a.parts; s += kWaves) {
-        const f32x2 ml = a.part_ml[(size_t)s * a.rows + row];
-        const float w = top == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(ml.x - top);
-        total += w * ml.y;
+        const float m = a.part_ml[(size_t)s * a.rows + row].x;
+        const float w = all.x == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - all.x);
         const float *src = a.part_o + ((size_t)s * a.rows + row) * c.vdim;
-        if (c.vdim % 4 == 0) {
-            if (d < c.vdim) v += *reinterpret_cast<const f32x4 *>(src + d) * w;
+        if (fours) {
+            v += *reinterpret_cast<const f32x4 *>(src + (d < c.vdim ? d : 0)) * w;
         } else {
 #pragma unroll
             for (uint32_t e = 0; e < 4; ++e)
@@ -428,15 +486,11 @@ __global__ __launch_bounds__(kThreads) void kv_fold_kernel(Args<S> a, uint32_t r
         }
     }
     lds_o[wave][lane] = v;
-    if (lane == 0) lds_l[wave] = total;
     __syncthreads();
     if (wave != 0) return;
-    for (uint32_t k = 1; k < kWaves; ++k) {
-        v += lds_o[k][lane];
-        total += lds_l[k];
-    }
-    store_out(a.out + row * c.vdim, c.vdim, d, finish(v, top, total));
-    if (a.row_ml != nullptr && lane == 0) a.row_ml[row] = weight_terms(top, total);
+    for (uint32_t k = 1; k < kWaves; ++k) v += lds_o[k][lane];
+    store_out(a.out + row * c.vdim, c.vdim, d, finish(v, all.x, all.y));
+    if (a.row_ml != nullptr && lane == 0) a.row_ml[row] = weight_terms(all.x, all.y);
 }
 
 // Softmax weights of one block's tokens, summed over the rows that see them: the
@@ -486,7 +540,7 @@ __global__ __launch_bounds__(kThreads) void kv_weights_kernel(Args<S> a) {
         Query<S, P> q;
         q.load(a.q + row * c.dim, c.dim, g);
         const f32x2 ml = live ? a.row_ml[row] : f32x2{0.0f, 0.0f};
-        const float factor = k_scale * a.scale2 * q.factor;
+        const float factor = (float)((double)k_scale * a.scale2) * q.factor;
 #pragma unroll
         for (uint32_t u = 0; u < 4; ++u) {
             f32x4 s4 = {0, 0, 0, 0};
@@ -522,7 +576,9 @@ __global__ __launch_bounds__(kThreads) void kv_weights_kernel(Args<S> a) {
 
 struct Plan {
     uint32_t row_groups, parts;
-    size_t rows, o_bytes, ml_bytes, row_bytes;
+    bool scores;   // the weights come from scores that the rows kernel stores
+    size_t rows, score_stride;
+    size_t o_bytes, ml_bytes, row_bytes, score_bytes;
 };
 
 size_t whole256(size_t bytes) { return (bytes + 255) / 256 * 256; }
@@ -540,8 +596,13 @@ Plan plan_of(const View &c, const AttentionShape &a) {
     p.parts = parts < 1 ? 1 : (uint32_t)parts;
     p.rows = (size_t)a.batch * a.q_heads * a.n;
     p.o_bytes = p.parts > 1 ? whole256(p.parts * p.rows * c.vdim * 4) : 0;
-    p.ml_bytes = p.parts > 1 ? whole256(p.parts * p.rows * sizeof(f32x2)) : 0;
-    p.row_bytes = a.weights != nullptr ? whole256(p.rows * sizeof(f32x2)) : 0;
+    // a token's scores, 4 bytes per row written and read again, against its key
+    // again: for up to a tile of rows the scores
+    p.scores = a.weights != nullptr && in_head <= kRows;
+    p.score_stride = (size_t)blocks * kTokens;
+    p.ml_bytes = p.parts > 1 || p.scores ? whole256(p.parts * p.rows * sizeof(f32x2)) : 0;
+    p.row_bytes = a.weights != nullptr && !p.scores ? whole256(p.rows * sizeof(f32x2)) : 0;
+    p.score_bytes = p.scores ? whole256(p.rows * p.score_stride * 4) : 0;
     return p;
 }
 
@@ -557,13 +618,16 @@ hipError_t launch(Args<S> a, const Plan &p, uint32_t batch, uint32_t longest, hi
         const hipError_t status = hipGetLastError();
         if (status != hipSuccess) return status;
     }
-    if (p.parts > 1) {
-        const uint32_t rows = a.pairs * a.group * a.n;   // at most 512 row groups where there are parts
-        kv_fold_kernel<S><<<rows, kThreads, 0, s>>>(a, 0);
+    if (p.parts > 1 || p.scores) {
+        // (at most 512 row groups where there are parts)
+        const uint32_t folds = p.parts > 1 ? a.pairs * a.group * a.n : 0;
+        const uint32_t token_groups = p.scores ? (blocks * kTokens + kThreads - 1) / kThreads : 0;
+        if (folds + a.pairs * token_groups == 0) return hipSuccess;
+        kv_fold_kernel<S><<<folds + a.pairs * token_groups, kThreads, 0, s>>>(a, folds, token_groups);
         const hipError_t status = hipGetLastError();
         if (status != hipSuccess) return status;
     }
-    if (a.weights != nullptr && blocks > 0) {
+    if (a.row_ml != nullptr && blocks > 0) {
         kv_weights_kernel<S, P><<<dim3(blocks, a.c.heads, batch), kThreads, 0, s>>>(a);
         return hipGetLastError();
     }
@@ -582,6 +646,8 @@ hipError_t run(const View &c, const AttentionShape &sh, const void *query, void 
     a.part_o = reinterpret_cast<float *>(ws);
     a.part_ml = reinterpret_cast<f32x2 *>(ws + p.o_bytes);
     a.row_ml = p.row_bytes ? reinterpret_cast<f32x2 *>(ws + p.o_bytes + p.ml_bytes) : nullptr;
+    a.scores = p.scores ? reinterpret_cast<float *>(ws + p.o_bytes + p.ml_bytes + p.row_bytes) : nullptr;
+    a.score_stride = p.score_stride;
     a.weights = sh.weights;
     a.weight_tokens = sh.weight_tokens;
     a.weight_stride = sh.weight_stride;
@@ -589,7 +655,7 @@ hipError_t run(const View &c, const AttentionShape &sh, const void *query, void 
     a.group = sh.q_heads / c.heads;
     a.n = sh.n;
     a.parts = p.parts;
-    a.scale2 = sh.scale * kLog2e;
+    a.scale2 = (double)sh.scale * kLog2e;
     a.causal = sh.causal;
     const uint32_t widest = c.kp > c.vp ? c.kp : c.vp;
     for (uint32_t first = 0; first < sh.batch; first += kBatchPerLaunch) {
@@ -613,7 +679,7 @@ hipError_t run(const View &c, const AttentionShape &sh, const void *query, void 
 
 size_t attention_workspace(const View &c, const AttentionShape &a) {
     const Plan p = plan_of(c, a);
-    return p.o_bytes + p.ml_bytes + p.row_bytes;
+    return p.o_bytes + p.ml_bytes + p.row_bytes + p.score_bytes;
 }
 
 hipError_t attention(bool f32, const View &c, const AttentionShape &a, const void *query, void *output,

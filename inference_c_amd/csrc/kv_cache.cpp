@@ -380,7 +380,8 @@ int tensor_kv_cache_evict(const TensorKvCache *cache, const TensorBuffer *weight
         return fail(error, error_capacity, "cache evict: out of device memory for its workspace");
     const kv::EvictArgs a{static_cast<const float *>(dev(weights)), (uint32_t)tokens, (uint32_t)first, (uint32_t)recent,
                           (uint32_t)keep, static_cast<float *>(dev(target_weights)), static_cast<uint32_t *>(dev(kept)),
-                          (uint32_t)slots, static_cast<uint32_t *>(workspace.get()), (uint32_t)most};
+                          (uint32_t)slots, static_cast<uint32_t *>(workspace.get()), (uint32_t)most,
+                          (uint32_t)longest};
     if (!hip_ok(kv::evict(source->view, target->view, (uint32_t)source->batch, a, sdk_stream()),
                 "cache evict: kernel launch", error, error_capacity))
         return 0;

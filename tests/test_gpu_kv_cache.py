@@ -211,6 +211,21 @@ def test_evict(sdk, case, dims):
     check_read(sdk, target, model, "target cut")
 
 
+@pytest.mark.parametrize("length", [32768, 32769, 70001])
+def test_evict_of_long_sequences(sdk, length):
+    """Around the length up to which the weights stay in registers."""
+    pair = Pair(sdk, 1, 1, length, 4, 4, 30)
+    pair.append(length)
+    w = np.rint(pair.rng.exponential(50, (1, 1, length))).astype(np.float32)     # many equal ones
+    target = sdk.kv_cache(1, 1, 5000, 4, 4)
+    for first, recent, keep in ((4, 100, 5000), (0, 0, 1), (7, 0, 4097)):
+        kept = sdk.tensor("u32", (1, 1, keep))
+        sdk.call("tensor_kv_cache_evict", pair.cache, sdk.from_numpy(w), first, recent, keep, target, None, kept)
+        model, index = pair.model.evict(w, first, recent, keep)
+        assert np.array_equal(kept.download()[0, 0], index[0][0])
+        check_read(sdk, target, model)
+
+
 def test_evict_of_equal_scales_keeps_codes(sdk):
     """Values that lie on the borders of the new codes (all blocks of one scale,
     the largest code gone): exact ties, decided for the even code."""
