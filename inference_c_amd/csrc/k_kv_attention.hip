@@ -26,50 +26,11 @@
 // f32: q and P each are a pair of f16 (q scaled by a power of two to a largest
 // element of 2^13 .. 2^14), 22 significant bits, and codes are exact: two MFMAs
 // in place of one.
-#include "kern_common.hpp"
-#include "kv.hpp"
+#include "kv_attention.hpp"
 
 namespace icsdk {
 namespace kv {
 namespace {
-
-typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
-typedef _Float16 half4 __attribute__((ext_vector_type(4)));
-typedef _Float16 half8 __attribute__((ext_vector_type(8)));
-typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-
-constexpr uint32_t kThreads = 256;
-constexpr uint32_t kWaves = 4;
-constexpr uint32_t kRows = 16;         // packed rows of a wave
-constexpr double kLog2e = 1.4426950408889634;
-constexpr float kUnitRange = 8.0f;     // a value scale further from the unit moves it
-// P of a row whose maximum is M is 2^(s - M + kHeadroom): as far up in f16 as the
-// unit's range and the lazy rescale of the maximum (by more than 2^kLazy) leave
-// room for, 2^15 in all, so that small weights keep their bits: absolute
-// errors of P, relative to the row's largest, are below 2^-26 (f16; P is rounded
-// to 2^-11 anyway) and 2^-34 (f32, whose maximum is never left behind).
-template <typename S> constexpr float kLazy = sizeof(S) == 4 ? 0.0f : 8.0f;
-template <typename S> constexpr float kHeadroom = sizeof(S) == 4 ? 12.0f : 4.0f;
-// Arguments of a launch over sequences first .. (pairs / heads of them).
-template <typename S> struct Args {
-    View c;
-    const S *q;
-    S *out;
-    float *part_o;       // [part][row][vdim], rows of all sequences
-    f32x2 *part_ml;      // [part][row] running maximum (log2 units) and sum
-    f32x2 *row_ml;       // [row] maximum and 1 / sum (0: the row adds no weight), or null
-    float *weights;
-    float *scores;       // [row][score_stride] scores in log2 units, or null
-    size_t rows;         // of all sequences
-    size_t score_stride;
-    size_t weight_stride;
-    uint32_t weight_tokens;
-    uint32_t first, pairs, group, n, parts, row_group0;
-    double scale2;       // scale * log2 e
-    int causal;
-    Counts count;
-};
 
 // Largest and sum over the four lanes that hold one row.
 __device__ inline float groups_max(float v) {
@@ -79,18 +40,6 @@ __device__ inline float groups_max(float v) {
 __device__ inline float groups_sum(float v) {
     v += __shfl_xor(v, 16, kWave);
     return v + __shfl_xor(v, 32, kWave);
-}
-
-// Eight codes (as bytes + 128) as f16, exact.
-__device__ inline half8 codes(uint32_t a, uint32_t b) {
-    const uint32_t one = 0x64646464u;
-    const half2_t bias = {(_Float16)1152.0f, (_Float16)1152.0f};
-    u32x4 r;
-    r[0] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(one, a, 0x04010400u)) - bias);
-    r[1] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(one, a, 0x04030402u)) - bias);
-    r[2] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(one, b, 0x04010400u)) - bias);
-    r[3] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(one, b, 0x04030402u)) - bias);
-    return __builtin_bit_cast(half8, r);
 }
 
 // The dims that a lane's operand of k step s has: 64-dim chunks of 16 per lane
@@ -150,37 +99,6 @@ template <typename S, uint32_t P> struct Query {
         }
     }
 };
-
-// How many keys packed row r sees (0 or fewer: none); padded rows and rows past
-// the head see all.
-__device__ inline int seen_by(uint32_t i, bool live, uint32_t length, uint32_t count, int causal) {
-    return causal && live ? (int)length - (int)count + (int)i + 1 : (int)length;
-}
-
-template <typename S>
-__device__ inline void store_out(S *row, uint32_t vdim, uint32_t d, f32x4 v) {
-    if (vdim % 4 == 0) {
-        if (d < vdim) {
-            if constexpr (sizeof(S) == 4) *reinterpret_cast<f32x4 *>(row + d) = v;
-            else *reinterpret_cast<half4 *>(row + d) = half4{(_Float16)v.x, (_Float16)v.y, (_Float16)v.z, (_Float16)v.w};
-        }
-    } else {
-#pragma unroll
-        for (uint32_t e = 0; e < 4; ++e)
-            if (d + e < vdim) row[d + e] = (S)v[e];
-    }
-}
-
-// Outputs of a row from its maximum, its sum and its sum of weighted values.
-__device__ inline f32x4 finish(f32x4 o, float big, float total) {
-    if (!__builtin_isfinite(big)) return f32x4{0, 0, 0, 0};
-    const float inverse = 1.0f / total;
-    return f32x4{o.x * inverse, o.y * inverse, o.z * inverse, o.w * inverse};
-}
-__device__ inline f32x2 weight_terms(float big, float total) {
-    const bool counts = __builtin_isfinite(big) && __builtin_isfinite(total);
-    return f32x2{counts ? big : 0.0f, counts ? 1.0f / total : 0.0f};
-}
 
 // One workgroup: 16 packed rows of one (sequence, kv head) and one part of its
 // blocks; wave w takes blocks w, w + 4, ... of the part and the waves' results
@@ -493,104 +411,35 @@ __global__ __launch_bounds__(kThreads) void kv_fold_kernel(Args<S> a, uint32_t f
     if (a.row_ml != nullptr && lane == 0) a.row_ml[row] = weight_terms(all.x, all.y);
 }
 
-// Softmax weights of one block's tokens, summed over the rows that see them: the
-// scores again, now with the rows' maxima and sums known. The block's keys stay
-// in registers and each wave walks every fourth group of 16 rows.
-template <typename S, uint32_t P>
-__global__ __launch_bounds__(kThreads) void kv_weights_kernel(Args<S> a) {
-    constexpr bool kPair = sizeof(S) == 4;
-    constexpr uint32_t KS = P / 32;
-    __shared__ float lds_w[kWaves][kTokens];
-    const View &c = a.c;
-    const uint32_t lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
-    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const uint32_t t = blockIdx.x, h = blockIdx.y, b = blockIdx.z, seq = a.first + b;
-    const size_t head = (size_t)seq * c.heads + h;
-    const uint32_t length = c.length[seq], count = a.count.n[b];
-    if (t * kTokens >= length || count == 0) return;
-    const uint32_t in_head = a.group * a.n;
-    const bool open = t == length / kTokens;
-    const Meta meta = c.meta[head * c.blocks + t];
-    const float k_scale = open ? 1.0f : meta.k_scale;
-    const uint32_t key_of = (m / 4) * 16 + m % 4;
-    half8 k[4][KS];
-#pragma unroll
-    for (uint32_t u = 0; u < 4; ++u)
-#pragma unroll
-        for (uint32_t s = 0; s < KS; ++s) {
-            const uint32_t d = step_dim<P>(s, g), at = d < c.kp ? d : 0;
-            if (open) {
-                k[u][s] = *reinterpret_cast<const half8 *>(c.kt + (head * kTokens + key_of + 4 * u) * c.kp + at);
-            } else {
-                const u32x2 w = *reinterpret_cast<const u32x2 *>(
-                    c.k + ((head * c.blocks + t) * kTokens + key_of + 4 * u) * c.kp + at);
-                k[u][s] = codes(w.x, w.y);
-            }
-        }
-    float acc[16];
-#pragma unroll
-    for (int e = 0; e < 16; ++e) acc[e] = 0.0f;
-    const uint32_t marked = (uint32_t)(meta.marked >> (16 * g));
-    for (uint32_t row0 = wave * kRows; row0 < in_head; row0 += kWaves * kRows) {
-        const uint32_t r = row0 + m, i = r % a.n;
-        const bool live = r < in_head && i < count;
-        const int seen = seen_by(i, live, length, count, a.causal);
-        if (!wave_any(live && seen > (int)(t * kTokens))) continue;
-        const size_t row = head * in_head + min(r, in_head - 1);
-        Query<S, P> q;
-        q.load(a.q + row * c.dim, c.dim, g);
-        const f32x2 ml = live ? a.row_ml[row] : f32x2{0.0f, 0.0f};
-        const float factor = (float)((double)k_scale * a.scale2) * q.factor;
-#pragma unroll
-        for (uint32_t u = 0; u < 4; ++u) {
-            f32x4 s4 = {0, 0, 0, 0};
-#pragma unroll
-            for (uint32_t s = 0; s < KS; ++s) {
-                s4 = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[u][s], q.hi[s], s4, 0, 0, 0);
-                if constexpr (kPair) s4 = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[u][s], q.lo[s], s4, 0, 0, 0);
-            }
-#pragma unroll
-            for (uint32_t e = 0; e < 4; ++e) {
-                const uint32_t at = 4 * u + e;
-                const bool counts = ml.y != 0.0f && (int)(t * kTokens + 16 * g + at) < seen && !(marked >> at & 1);
-                acc[at] += counts ? __builtin_amdgcn_exp2f(s4[e] * factor - ml.x) * ml.y : 0.0f;
-            }
-        }
-    }
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-#pragma unroll
-        for (int d = 1; d < 16; d *= 2) acc[e] += __shfl_xor(acc[e], d, kWave);
-        if (m == 0) lds_w[wave][16 * g + e] = acc[e];
-    }
-    __syncthreads();
-    const uint32_t token = t * kTokens + lane;
-    if (wave == 0 && token < min(length, a.weight_tokens)) {
-        float total = 0.0f;
-        for (uint32_t w = 0; w < kWaves; ++w) total += lds_w[w][lane];
-        a.weights[head * a.weight_stride + token] += total;
-    }
-}
-
 // ---- plan and launch ---------------------------------------------------------------
 
 struct Plan {
-    uint32_t row_groups, parts;
+    bool tiles;    // many rows: k_kv_tiles.hip
     bool scores;   // the weights come from scores that the rows kernel stores
+    uint32_t row_groups, parts, row_parts;
     size_t rows, score_stride;
-    size_t o_bytes, ml_bytes, row_bytes, score_bytes;
+    size_t o_bytes, ml_bytes, row_bytes, score_bytes, partial_bytes;
+    size_t bytes() const { return o_bytes + ml_bytes + row_bytes + score_bytes + partial_bytes; }
 };
 
 size_t whole256(size_t bytes) { return (bytes + 255) / 256 * 256; }
+uint32_t widest_of(const View &c) { return c.kp > c.vp ? c.kp : c.vp; }
 
-Plan plan_of(const View &c, const AttentionShape &a) {
-    Plan p;
+constexpr uint32_t kMinTileRows = 64;   // packed rows of a head from which tiles are used
+constexpr uint32_t kWorkgroups = 512;   // two for every CU
+
+Plan plan_of(bool f32, const View &c, const AttentionShape &a) {
+    Plan p{};
     const uint32_t in_head = a.q_heads / c.heads * a.n;
-    p.row_groups = (in_head + kRows - 1) / kRows;
     const uint32_t blocks = (a.longest + kTokens - 1) / kTokens;
-    // parts: workgroups for every CU twice over, a block for each wave at least
-    const uint64_t base = (uint64_t)a.batch * c.heads * p.row_groups;
-    uint64_t parts = base >= 512 ? 1 : 512 / base;
+    const uint64_t pairs = (uint64_t)a.batch * c.heads;
+    p.tiles = in_head >= kMinTileRows && tiles_fit(f32, widest_of(c));
+    const uint32_t rows_each = p.tiles ? kTileRows : kRows;
+    p.row_groups = (in_head + rows_each - 1) / rows_each;
+    // parts: workgroups for every CU twice over, with a block for each wave (tiles:
+    // four blocks) at least
+    const uint64_t base = pairs * p.row_groups;
+    uint64_t parts = base >= kWorkgroups ? 1 : kWorkgroups / base;
     const uint32_t most = (blocks + kWaves - 1) / kWaves;
     parts = parts < most ? parts : most;
     p.parts = parts < 1 ? 1 : (uint32_t)parts;
@@ -603,19 +452,41 @@ Plan plan_of(const View &c, const AttentionShape &a) {
     p.ml_bytes = p.parts > 1 || p.scores ? whole256(p.parts * p.rows * sizeof(f32x2)) : 0;
     p.row_bytes = a.weights != nullptr && !p.scores ? whole256(p.rows * sizeof(f32x2)) : 0;
     p.score_bytes = p.scores ? whole256(p.rows * p.score_stride * 4) : 0;
+    p.row_parts = 1;
+    if (p.row_bytes != 0 && blocks != 0) {
+        // weights: workgroups for every CU twice over, with 32 rows for each wave at least
+        const uint64_t groups = pairs * blocks, fit = (in_head + kTileRows - 1) / kTileRows;
+        const uint64_t want = groups >= kWorkgroups ? 1 : kWorkgroups / groups;
+        p.row_parts = (uint32_t)(want < fit ? want : fit);
+        if (p.row_parts > 1) p.partial_bytes = whole256(p.row_parts * pairs * p.score_stride * 4);
+    }
     return p;
 }
 
 template <typename S, uint32_t P>
-hipError_t launch(Args<S> a, const Plan &p, uint32_t batch, uint32_t longest, hipStream_t s) {
-    const uint32_t blocks = (longest + kTokens - 1) / kTokens;
+hipError_t launch_rows(const Args<S> &a, uint32_t groups, hipStream_t s) {
+    kv_rows_kernel<S, P><<<groups * a.pairs * a.parts, kThreads, 0, s>>>(a);
+    return hipGetLastError();
+}
+template <typename S>
+hipError_t launch_rows(const Args<S> &a, uint32_t widest, uint32_t groups, hipStream_t s) {
+    if (widest <= 32) return launch_rows<S, 32>(a, groups, s);
+    if (widest <= 64) return launch_rows<S, 64>(a, groups, s);
+    if (widest <= 96) return launch_rows<S, 96>(a, groups, s);
+    if (widest <= 128) return launch_rows<S, 128>(a, groups, s);
+    if (widest <= 192) return launch_rows<S, 192>(a, groups, s);
+    return launch_rows<S, 256>(a, groups, s);
+}
+
+template <typename S>
+hipError_t launch(Args<S> a, const Plan &p, uint32_t batch, uint32_t longest, float *partial, hipStream_t s) {
+    const uint32_t blocks = (longest + kTokens - 1) / kTokens, widest = widest_of(a.c);
     // (a launch holds fewer than 2^32 threads)
     const uint32_t most = (1u << 23) / (a.pairs * p.parts) < 1 ? 1 : (1u << 23) / (a.pairs * p.parts);
     for (uint32_t g0 = 0; g0 < p.row_groups; g0 += most) {
         a.row_group0 = g0;
         const uint32_t groups = p.row_groups - g0 < most ? p.row_groups - g0 : most;
-        kv_rows_kernel<S, P><<<groups * a.pairs * p.parts, kThreads, 0, s>>>(a);
-        const hipError_t status = hipGetLastError();
+        const hipError_t status = p.tiles ? launch_tiles(a, widest, groups, s) : launch_rows(a, widest, groups, s);
         if (status != hipSuccess) return status;
     }
     if (p.parts > 1 || p.scores) {
@@ -627,26 +498,29 @@ hipError_t launch(Args<S> a, const Plan &p, uint32_t batch, uint32_t longest, hi
         const hipError_t status = hipGetLastError();
         if (status != hipSuccess) return status;
     }
-    if (a.row_ml != nullptr && blocks > 0) {
-        kv_weights_kernel<S, P><<<dim3(blocks, a.c.heads, batch), kThreads, 0, s>>>(a);
-        return hipGetLastError();
-    }
+    if (a.row_ml != nullptr && blocks > 0) return launch_weights(a, widest, batch, blocks, p.row_parts, partial, s);
     return hipSuccess;
 }
 
 template <typename S>
 hipError_t run(const View &c, const AttentionShape &sh, const void *query, void *output, void *workspace,
                hipStream_t s) {
-    const Plan p = plan_of(c, sh);
+    const Plan p = plan_of(sizeof(S) == 4, c, sh);
     Args<S> a;
     a.c = c;
     a.q = static_cast<const S *>(query);
     a.out = static_cast<S *>(output);
     char *ws = static_cast<char *>(workspace);
-    a.part_o = reinterpret_cast<float *>(ws);
-    a.part_ml = reinterpret_cast<f32x2 *>(ws + p.o_bytes);
-    a.row_ml = p.row_bytes ? reinterpret_cast<f32x2 *>(ws + p.o_bytes + p.ml_bytes) : nullptr;
-    a.scores = p.scores ? reinterpret_cast<float *>(ws + p.o_bytes + p.ml_bytes + p.row_bytes) : nullptr;
+    auto take = [&](size_t bytes) {
+        char *const at = bytes ? ws : nullptr;
+        ws += bytes;
+        return at;
+    };
+    a.part_o = reinterpret_cast<float *>(take(p.o_bytes));
+    a.part_ml = reinterpret_cast<f32x2 *>(take(p.ml_bytes));
+    a.row_ml = reinterpret_cast<f32x2 *>(take(p.row_bytes));
+    a.scores = reinterpret_cast<float *>(take(p.score_bytes));
+    float *const partial = reinterpret_cast<float *>(take(p.partial_bytes));
     a.score_stride = p.score_stride;
     a.weights = sh.weights;
     a.weight_tokens = sh.weight_tokens;
@@ -657,19 +531,12 @@ hipError_t run(const View &c, const AttentionShape &sh, const void *query, void 
     a.parts = p.parts;
     a.scale2 = (double)sh.scale * kLog2e;
     a.causal = sh.causal;
-    const uint32_t widest = c.kp > c.vp ? c.kp : c.vp;
     for (uint32_t first = 0; first < sh.batch; first += kBatchPerLaunch) {
         const uint32_t batch = sh.batch - first < kBatchPerLaunch ? sh.batch - first : kBatchPerLaunch;
         for (uint32_t b = 0; b < batch; ++b) a.count.n[b] = sh.counts ? sh.counts[first + b] : sh.n;
         a.first = first;
         a.pairs = batch * c.heads;
-        hipError_t status;
-        if (widest <= 32) status = launch<S, 32>(a, p, batch, sh.longest, s);
-        else if (widest <= 64) status = launch<S, 64>(a, p, batch, sh.longest, s);
-        else if (widest <= 96) status = launch<S, 96>(a, p, batch, sh.longest, s);
-        else if (widest <= 128) status = launch<S, 128>(a, p, batch, sh.longest, s);
-        else if (widest <= 192) status = launch<S, 192>(a, p, batch, sh.longest, s);
-        else status = launch<S, 256>(a, p, batch, sh.longest, s);
+        const hipError_t status = launch(a, p, batch, sh.longest, partial, s);
         if (status != hipSuccess) return status;
     }
     return hipSuccess;
@@ -677,10 +544,7 @@ hipError_t run(const View &c, const AttentionShape &sh, const void *query, void 
 
 }  // namespace
 
-size_t attention_workspace(const View &c, const AttentionShape &a) {
-    const Plan p = plan_of(c, a);
-    return p.o_bytes + p.ml_bytes + p.row_bytes + p.score_bytes;
-}
+size_t attention_workspace(bool f32, const View &c, const AttentionShape &a) { return plan_of(f32, c, a).bytes(); }
 
 hipError_t attention(bool f32, const View &c, const AttentionShape &a, const void *query, void *output,
                      void *workspace, hipStream_t s) {

@@ -1,0 +1,509 @@
+// Attention over the 8-bit cache for many query rows: tiles of 128 packed rows
+// and 64 keys (kv_attention.hpp, kv.hpp).
+//
+// v_mfma_f32_32x32x16_f16: A[m][k] in lane l at m = l % 32, k = 8 (l / 32) + e;
+// B[k][n] at n = l % 32 likewise; D[m][n] at n = l % 32, m = 8 (r / 4) + 4 (l / 32) +
+// r % 4. A wave of 32 rows computes, per block of 64 keys,
+//   S^T = K Q^T in two halves of 32 keys. A row m is key m with its bits 2 and 3
+//     exchanged, so that accumulator registers 8 c .. 8 c + 7 of a lane are the
+//     keys 16 c + 8 (l / 32) + 0 .. 7: consecutive, and
+//   out^T = V^T P^T takes them as B operands in their order, with the dim's same
+//     keys side by side in memory: one 16-byte LDS read per A operand.
+// A workgroup turns each block's codes to f16 once, on their way into LDS (key
+// rows 8 halves longer than the data, dim rows of 72: no bank conflicts); the next
+// block's codes are asked for before a block is computed and written to the other
+// buffer after it, one barrier per block.
+// Scores stay raw products; the block's factor k_scale * scale * log2 e enters with
+// the maximum in one fma, the ratio of its value scale to the unit as an addend of
+// the exponent (k_kv_attention.hip has the rules).
+#include "flash.hpp"
+#include "kv_attention.hpp"
+
+namespace icsdk {
+namespace kv {
+namespace {
+
+typedef float float16v __attribute__((ext_vector_type(16)));
+
+constexpr float kTiny = 1.1754944e-38f, kHuge = 3.0e38f;
+
+// 32 query rows as B operands, one per 16 dims (f32: and their rest), times `sign`
+// (the scale's; 0 where the scale is).
+template <typename S, uint32_t P> struct TileQuery {
+    static constexpr uint32_t kSteps = P / 16;
+    static constexpr bool kPair = sizeof(S) == 4;
+    half8 hi[kSteps], lo[kPair ? kSteps : 1];
+    float factor;   // the power of two that a f32 row was divided by
+
+    __device__ inline void load(const S *row, uint32_t dim, uint32_t half, float sign) {
+        factor = 1.0f;
+        if constexpr (!kPair) {
+            const _Float16 s = (_Float16)sign;
+            if (dim % 8 == 0) {
+#pragma unroll
+                for (uint32_t c = 0; c < kSteps; ++c) {
+                    const uint32_t d = 16 * c + 8 * half;
+                    hi[c] = *reinterpret_cast<const half8 *>(row + (d < dim ? d : 0));
+                }
+#pragma unroll
+                for (uint32_t c = 0; c < kSteps; ++c) {
+                    hi[c] *= s;
+                    if (16 * c + 8 * half >= dim) hi[c] = half8{};
+                }
+            } else {
+#pragma unroll
+                for (uint32_t c = 0; c < kSteps; ++c)
+#pragma unroll
+                    for (uint32_t e = 0; e < 8; ++e) {
+                        const uint32_t d = 16 * c + 8 * half + e;
+                        hi[c][e] = d < dim ? row[d] * s : (_Float16)0.0f;
+                    }
+            }
+        } else {
+            float x[kSteps][8], big = 0.0f;
+            bool finite = true;
+#pragma unroll
+            for (uint32_t c = 0; c < kSteps; ++c)
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e) {
+                    const uint32_t d = 16 * c + 8 * half + e;
+                    x[c][e] = d < dim ? row[d] * sign : 0.0f;
+                    big = fmaxf(big, fabsf(x[c][e]));
+                    finite = finite && __builtin_isfinite(x[c][e]);
+                }
+            big = flash::pair_max(finite ? big : __builtin_inff());
+            const bool usable = big > 0.0f && __builtin_isfinite(big);
+            const int exponent = usable ? __builtin_amdgcn_frexp_expf(big) : 14;
+            factor = __builtin_isfinite(big) ? __builtin_ldexpf(1.0f, exponent - 14) : __builtin_nanf("");
+#pragma unroll
+            for (uint32_t c = 0; c < kSteps; ++c)
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e) {
+                    const float y = usable ? __builtin_ldexpf(x[c][e], 14 - exponent) : 0.0f;
+                    hi[c][e] = (_Float16)y;
+                    lo[c][e] = (_Float16)(y - (float)hi[c][e]);
+                }
+        }
+    }
+    __device__ inline void clear() {
+        factor = 1.0f;
+#pragma unroll
+        for (uint32_t c = 0; c < kSteps; ++c) {
+            hi[c] = half8{};
+            if constexpr (kPair) lo[c] = half8{};
+        }
+    }
+};
+
+// A block's factor of raw products, positive (queries carry the scale's sign), and
+// what rounding took off it. A block of zero keys has raw products 0: any factor.
+__device__ inline f32x2 block_factor(float k_scale, double scale2) {
+    const double f = (k_scale == 0.0f ? 1.0 : (double)k_scale) * (scale2 == 0.0 ? 1.0 : fabs(scale2));
+    const float hi = fminf(fmaxf((float)f, kTiny), kHuge);
+    return f32x2{hi, (float)(f - (double)hi)};
+}
+
+// Key row of the block that A row m of a half reads.
+__device__ inline uint32_t swap23(uint32_t m) { return (m & 0x13u) | (m & 4u) << 1 | (m & 8u) >> 1; }
+
+template <typename S, uint32_t P>
+__global__ __launch_bounds__(kThreads, P <= 128 ? 2 : 1) void kv_tiles_kernel(Args<S> a) {
+    constexpr bool kPair = sizeof(S) == 4;
+    constexpr uint32_t KC = P / 16, VT = (P + 31) / 32;
+    constexpr uint32_t KROW = P + 8, VROW = kTokens + 8;   // LDS rows, halves
+    constexpr uint32_t KPER = (kTokens * P / 16 + kThreads - 1) / kThreads;   // 16-byte pieces of codes per thread
+    __shared__ __attribute__((aligned(16))) _Float16 ks[2][kTokens * KROW], vs[2][VT * 32 * VROW];
+    const View &c = a.c;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane(tid / kWave);
+    // workgroup -> (rows, part, (sequence, head)): the last rows, which see most
+    // keys, first; one head's workgroups on one XCD where the heads are whole eights
+    const uint32_t in_head = a.group * a.n, row_blocks = (in_head + kTileRows - 1) / kTileRows;
+    const uint32_t pair = blockIdx.x % a.pairs, rest = blockIdx.x / a.pairs + a.row_group0 * a.parts;
+    const uint32_t part = rest % a.parts, row_block = row_blocks - 1 - rest / a.parts;
+    const uint32_t b = pair / c.heads, h = pair % c.heads, seq = a.first + b;
+    const size_t head = (size_t)seq * c.heads + h;
+    const uint32_t length = c.length[seq], count = a.count.n[b];
+    const uint32_t r = row_block * kTileRows + wave * 32 + col, i = r % a.n;
+    const bool live = r < in_head && i < count;
+    const size_t row = head * in_head + min(r, in_head - 1);
+    const int seen = seen_by(i, live, length, count, a.causal);
+    // keys that some row of the wave, and of the workgroup, sees
+    int most = live ? seen : 0, least = live ? seen : (int)length;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+        most = max(most, __shfl_xor(most, d, kWave));
+        least = min(least, __shfl_xor(least, d, kWave));
+    }
+    most = __builtin_amdgcn_readfirstlane(most);
+    least = __builtin_amdgcn_readfirstlane(least);
+    __shared__ int wave_most[kWaves];
+    if (lane == 0) wave_most[wave] = most;
+    __syncthreads();
+    int all_most = wave_most[0];
+#pragma unroll
+    for (uint32_t w = 1; w < kWaves; ++w) all_most = max(all_most, wave_most[w]);
+    const uint32_t blocks = ((uint32_t)max(all_most, 0) + kTokens - 1) / kTokens, whole = length / kTokens;
+    const uint32_t share = (blocks + a.parts - 1) / a.parts;
+    const uint32_t begin = min(part * share, blocks), end = min(begin + share, blocks);
+
+    TileQuery<S, P> q;
+    q.load(a.q + row * c.dim, c.dim, half, a.scale2 > 0.0 ? 1.0f : a.scale2 < 0.0 ? -1.0f : 0.0f);
+    const Meta *const meta = c.meta + head * c.blocks;
+    const uint8_t *const kcodes = c.k + head * c.blocks * kTokens * c.kp;
+    const uint8_t *const vcodes = c.v + head * c.blocks * kTokens * c.vp;
+
+    // the thread's 16-byte pieces of a block's codes (pieces past the end repeat the
+    // last one and are not written)
+    const uint32_t kpieces = kTokens * c.kp / 16, vpieces = c.vp * 4;
+    uint32_t kto[KPER], vto[KPER];
+#pragma unroll
+    for (uint32_t u = 0; u < KPER; ++u) {
+        const uint32_t p = tid + u * kThreads;
+        kto[u] = p * 16 / c.kp * KROW + p * 16 % c.kp;
+        vto[u] = p / 4 * VROW + p % 4 * 16;
+    }
+    u32x4 kreg[KPER], vreg[KPER];
+    auto fetch = [&](uint32_t t) {
+#pragma unroll
+        for (uint32_t u = 0; u < KPER; ++u) {
+            const uint32_t p = tid + u * kThreads;
+            kreg[u] = reinterpret_cast<const u32x4 *>(kcodes + (size_t)t * kTokens * c.kp)[min(p, kpieces - 1)];
+            vreg[u] = reinterpret_cast<const u32x4 *>(vcodes + (size_t)t * kTokens * c.vp)[min(p, vpieces - 1)];
+        }
+    };
+    auto put = [&](_Float16 *to, half8 lo, half8 hi) {
+        *reinterpret_cast<half8 *>(to) = lo;
+        *reinterpret_cast<half8 *>(to + 8) = hi;
+    };
+    auto stash = [&](uint32_t buf) {
+#pragma unroll
+        for (uint32_t u = 0; u < KPER; ++u) {
+            const uint32_t p = tid + u * kThreads;
+            if (p < kpieces) put(&ks[buf][kto[u]], codes(kreg[u].x, kreg[u].y), codes(kreg[u].z, kreg[u].w));
+            if (p < vpieces) put(&vs[buf][vto[u]], codes(vreg[u].x, vreg[u].y), codes(vreg[u].z, vreg[u].w));
+        }
+    };
+    auto stash_open = [&](uint32_t buf) {   // the open block lies in f16
+        const half8 *kt = reinterpret_cast<const half8 *>(c.kt + head * kTokens * c.kp);
+        const half8 *vt = reinterpret_cast<const half8 *>(c.vt + head * kTokens * c.vp);
+#pragma unroll
+        for (uint32_t u = 0; u < KPER; ++u) {
+            const uint32_t p = tid + u * kThreads;
+            if (p < kpieces) put(&ks[buf][kto[u]], kt[2 * p], kt[2 * p + 1]);
+            if (p < vpieces) put(&vs[buf][vto[u]], vt[2 * p], vt[2 * p + 1]);
+        }
+    };
+    // columns past the padded dim meet zeros of q, and must not be NaN
+    for (uint32_t p = tid; p < kTokens * (P - c.kp) / 8; p += kThreads) {
+        const uint32_t per = (P - c.kp) / 8, t = p / per, d = c.kp + p % per * 8;
+        *reinterpret_cast<half8 *>(&ks[0][t * KROW + d]) = half8{};
+        *reinterpret_cast<half8 *>(&ks[1][t * KROW + d]) = half8{};
+    }
+
+    const float neg_inf = -__builtin_inff();
+    float16v o[VT];
+#pragma unroll
+    for (uint32_t t = 0; t < VT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[t][e] = 0.0f;
+    float big = neg_inf, sum = 0.0f, unit = 1.0f;   // (sum: of the lane's keys)
+
+    if (begin < end) {
+        if (begin < whole) {
+            fetch(begin);
+            stash(0);
+        } else {
+            stash_open(0);
+        }
+    }
+    __syncthreads();
+    for (uint32_t t = begin; t < end; ++t) {
+        const uint32_t buf = (t - begin) & 1;
+        if (t + 1 < end && t + 1 < whole) fetch(t + 1);
+        if ((int)(t * kTokens) < most) {
+            Meta m = meta[t];
+            if (t >= whole) m.k_scale = m.v_scale = 1.0f;
+            float16v st[2];
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) st[s][e] = 0.0f;
+            flash::mfma_phase_begin();
+#pragma unroll
+            for (uint32_t ch = 0; ch < KC; ++ch)
+#pragma unroll
+                for (uint32_t s = 0; s < 2; ++s) {
+                    const half8 k = *reinterpret_cast<const half8 *>(
+                        &ks[buf][(32 * s + swap23(col)) * KROW + 16 * ch + 8 * half]);
+                    st[s] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q.hi[ch], st[s], 0, 0, 0);
+                    if constexpr (kPair) st[s] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q.lo[ch], st[s], 0, 0, 0);
+                }
+            if constexpr (2 * KC > 4) flash::lds_read_ahead<2 * KC, 1, kPair ? 2 : 1>();
+            flash::mfma_phase_end();
+            const f32x2 f2 = block_factor(m.k_scale, a.scale2);
+            const float factor = f2.x * q.factor;
+            if ((int)(t * kTokens + kTokens) > least || m.marked != 0) {
+#pragma unroll
+                for (uint32_t e = 0; e < 32; ++e) {
+                    const uint32_t key = e / 8 * 16 + 8 * half + e % 8;
+                    if (m.marked >> key & 1) st[e / 16][e % 16] = __builtin_nanf("");
+                    if ((int)(t * kTokens + key) >= seen) st[e / 16][e % 16] = neg_inf;
+                }
+            }
+            float part_max[4] = {neg_inf, neg_inf, neg_inf, neg_inf};
+#pragma unroll
+            for (int e = 0; e < 32; ++e) part_max[e % 4] = fmaxf(part_max[e % 4], st[e / 16][e % 16]);
+            const float raw = fmaxf(fmaxf(part_max[0], part_max[1]), fmaxf(part_max[2], part_max[3]));
+            const float top = raw * factor;
+            if (__builtin_amdgcn_ballot_w64(top > big + kLazy<S>) != 0) {
+                const float now = flash::pair_max(fmaxf(top, big));
+                const float alpha = now == neg_inf ? 1.0f : __builtin_amdgcn_exp2f(big - now);
+                sum *= alpha;
+#pragma unroll
+                for (uint32_t v = 0; v < VT; ++v) o[v] *= alpha;
+                big = now;
+            }
+            float ratio = m.v_scale / unit;
+            if (m.v_scale == 0.0f) {
+                ratio = 1.0f;
+            } else if (ratio > kUnitRange || ratio < 1.0f / kUnitRange) {
+#pragma unroll
+                for (uint32_t v = 0; v < VT; ++v) o[v] *= unit / m.v_scale;
+                unit = m.v_scale;
+                ratio = 1.0f;
+            }
+            // exponents are relative to this; with nothing seen every score is -inf or NaN
+            const float base = (big == neg_inf ? 0.0f : big - kHeadroom<S>) - __builtin_amdgcn_logf(ratio);
+            half8 ph[4], pl[kPair ? 4 : 1];
+            float add[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+                const float s = st[e / 16][e % 16];
+                float x = __builtin_fmaf(s, factor, -base);
+                if constexpr (kPair) {
+                    const float off = s * (f2.y * q.factor);
+                    x += fabsf(off) < 1.0f ? off : 0.0f;   // (not for -inf)
+                }
+                x = __builtin_amdgcn_exp2f(x);
+                ph[e / 8][e % 8] = (_Float16)x;
+                if constexpr (kPair) {
+                    pl[e / 8][e % 8] = (_Float16)(x - (float)ph[e / 8][e % 8]);
+                    add[e % 4] += x;
+                }
+            }
+            if constexpr (!kPair) {   // the sum of P as the product has it
+                const half2_t ones = {(_Float16)1.0f, (_Float16)1.0f};
+#pragma unroll
+                for (int e = 0; e < 16; ++e)
+                    add[e % 4] = __builtin_amdgcn_fdot2(half2_t{ph[e / 4][2 * (e % 4)], ph[e / 4][2 * (e % 4) + 1]}, ones,
+                                                        add[e % 4], false);
+            }
+            sum += ((add[0] + add[1]) + (add[2] + add[3])) * (1.0f / ratio);
+            flash::mfma_phase_begin();
+#pragma unroll
+            for (uint32_t ch = 0; ch < 4; ++ch)
+#pragma unroll
+                for (uint32_t v = 0; v < VT; ++v) {
+                    const half8 vf = *reinterpret_cast<const half8 *>(&vs[buf][(32 * v + col) * VROW + 16 * ch + 8 * half]);
+                    o[v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, ph[ch], o[v], 0, 0, 0);
+                    if constexpr (kPair) o[v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pl[ch], o[v], 0, 0, 0);
+                }
+            if constexpr (4 * VT > 4) flash::lds_read_ahead<4 * VT, 1, kPair ? 2 : 1>();
+            flash::mfma_phase_end();
+        }
+        if (t + 1 < end) {
+            if (t + 1 < whole) stash(buf ^ 1);
+            else stash_open(buf ^ 1);
+        }
+        __syncthreads();
+    }
+    sum = flash::pair_sum(sum);
+    big -= kHeadroom<S>;
+    if (!live) return;
+    const bool direct = a.parts == 1;
+#pragma unroll
+    for (uint32_t v = 0; v < VT; ++v)
+#pragma unroll
+        for (uint32_t e = 0; e < 4; ++e) {
+            const f32x4 x = f32x4{o[v][4 * e], o[v][4 * e + 1], o[v][4 * e + 2], o[v][4 * e + 3]} * unit;
+            const uint32_t d = 32 * v + 8 * e + 4 * half;
+            if (direct) store_out(a.out + row * c.vdim, c.vdim, d, finish(x, big, sum));
+            else store_out(a.part_o + ((size_t)part * a.rows + row) * c.vdim, c.vdim, d, x);
+        }
+    if (half != 0) return;
+    if (!direct) a.part_ml[(size_t)part * a.rows + row] = f32x2{big, sum};
+    else if (a.row_ml != nullptr) a.row_ml[row] = weight_terms(big, sum);
+}
+
+// Softmax weights of one block's tokens, summed over the rows that see them: the
+// scores again, now with the rows' maxima and sums known. The block's keys stay in
+// registers; the waves walk the rows, 32 at a time, each with its next rows' loads
+// ahead. Where there are too few blocks for the chip, `row_parts` workgroups share
+// one's rows, and kv_weights_add_kernel adds their sums in order.
+template <typename S, uint32_t P>
+__global__ __launch_bounds__(kThreads, P <= 64 ? 4 : P <= 128 ? 2 : 1) void kv_weights_kernel(Args<S> a,
+                                                                                              uint32_t row_parts,
+                                                                                              float *partial) {
+    constexpr bool kPair = sizeof(S) == 4;
+    constexpr uint32_t KC = P / 16;
+    constexpr bool kAhead = !kPair && P <= 128;
+    __shared__ float lds_w[kWaves][kTokens];
+    const View &c = a.c;
+    const uint32_t lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const uint32_t t = blockIdx.x / row_parts, row_part = blockIdx.x % row_parts;
+    const uint32_t h = blockIdx.y, b = blockIdx.z, seq = a.first + b;
+    const size_t head = (size_t)seq * c.heads + h;
+    const uint32_t length = c.length[seq], count = a.count.n[b];
+    if (t * kTokens >= length || count == 0) return;
+    const uint32_t in_head = a.group * a.n;
+    const bool open = t == length / kTokens;
+    const Meta meta = c.meta[head * c.blocks + t];
+    half8 k[2][KC];
+#pragma unroll
+    for (uint32_t s = 0; s < 2; ++s)
+#pragma unroll
+        for (uint32_t ch = 0; ch < KC; ++ch) {
+            const uint32_t d = 16 * ch + 8 * half, at = d < c.kp ? d : 0, key = 32 * s + swap23(col);
+            if (open) {
+                k[s][ch] = *reinterpret_cast<const half8 *>(c.kt + (head * kTokens + key) * c.kp + at);
+            } else {
+                const u32x2 w = *reinterpret_cast<const u32x2 *>(c.k + ((head * c.blocks + t) * kTokens + key) * c.kp + at);
+                k[s][ch] = codes(w.x, w.y);
+            }
+        }
+    const float sign = a.scale2 > 0.0 ? 1.0f : a.scale2 < 0.0 ? -1.0f : 0.0f;
+    const f32x2 f2 = block_factor(open ? 1.0f : meta.k_scale, a.scale2);
+    float acc[32];
+#pragma unroll
+    for (int e = 0; e < 32; ++e) acc[e] = 0.0f;
+    constexpr uint32_t kStep = kWaves * 32;
+    const uint32_t stride = kStep * row_parts;
+    const uint32_t first = (row_part * kWaves + wave) * 32;
+    auto row_of = [&](uint32_t row0) { return head * in_head + min(row0 + col, in_head - 1); };
+    TileQuery<S, P> next;
+    f32x2 next_ml;
+    auto load = [&](uint32_t row0) {
+        const size_t row = row_of(row0);
+        next.load(a.q + row * c.dim, c.dim, half, sign);
+        next_ml = a.row_ml[row];
+    };
+    if (kAhead && first < in_head) load(first);
+    for (uint32_t row0 = first; row0 < in_head; row0 += stride) {
+        const uint32_t r = row0 + col, i = r % a.n;
+        const bool live = r < in_head && i < count;
+        const int seen = seen_by(i, live, length, count, a.causal);
+        const bool any = wave_any(live && seen > (int)(t * kTokens));
+        if (!kAhead && any) load(row0);
+        TileQuery<S, P> q = next;
+        f32x2 ml = next_ml;
+        if (kAhead && row0 + stride < in_head) load(row0 + stride);
+        if (!any) continue;
+        // a row that adds nothing (padding, or not finite): raw products 0, times 0
+        if (!live) ml = f32x2{0.0f, 0.0f};
+        if (ml.y == 0.0f) q.clear();
+        const float factor = f2.x * q.factor;
+        float16v st[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) st[s][e] = 0.0f;
+#pragma unroll
+        for (uint32_t ch = 0; ch < KC; ++ch)
+#pragma unroll
+            for (uint32_t s = 0; s < 2; ++s) {
+                st[s] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[s][ch], q.hi[ch], st[s], 0, 0, 0);
+                if constexpr (kPair) st[s] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[s][ch], q.lo[ch], st[s], 0, 0, 0);
+            }
+        if (wave_any(live && seen < (int)(t * kTokens + kTokens)) || meta.marked != 0) {
+#pragma unroll
+            for (uint32_t e = 0; e < 32; ++e) {
+                const uint32_t key = e / 8 * 16 + 8 * half + e % 8;
+                if ((int)(t * kTokens + key) >= seen || (meta.marked >> key & 1)) st[e / 16][e % 16] = -__builtin_inff();
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+            acc[e] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(st[e / 16][e % 16], factor, -ml.x)), ml.y, acc[e]);
+    }
+#pragma unroll
+    for (uint32_t e = 0; e < 32; ++e) {
+#pragma unroll
+        for (int d = 1; d < 32; d *= 2) acc[e] += __shfl_xor(acc[e], d, kWave);
+        if (col == 0) lds_w[wave][e / 8 * 16 + 8 * half + e % 8] = acc[e];
+    }
+    __syncthreads();
+    const uint32_t token = t * kTokens + lane;
+    if (wave == 0 && token < min(length, a.weight_tokens)) {
+        float total = 0.0f;
+        for (uint32_t w = 0; w < kWaves; ++w) total += lds_w[w][lane];
+        if (row_parts == 1) a.weights[head * a.weight_stride + token] += total;
+        else partial[(row_part * (size_t)a.c.heads * gridDim.z + ((size_t)b * c.heads + h)) * (gridDim.x / row_parts * kTokens) + token] = total;
+    }
+}
+
+template <typename S>
+__global__ __launch_bounds__(kThreads) void kv_weights_add_kernel(Args<S> a, uint32_t row_parts, uint32_t tokens,
+                                                                  const float *partial) {
+    const View &c = a.c;
+    const uint32_t t = blockIdx.x * kThreads + threadIdx.x, h = blockIdx.y, b = blockIdx.z, seq = a.first + b;
+    if (a.count.n[b] == 0 || t >= min(c.length[seq], a.weight_tokens)) return;
+    float total = 0.0f;
+    for (uint32_t p = 0; p < row_parts; ++p)
+        total += partial[(p * (size_t)c.heads * gridDim.z + ((size_t)b * c.heads + h)) * tokens + t];
+    a.weights[((size_t)seq * c.heads + h) * a.weight_stride + t] += total;
+}
+
+template <typename S, uint32_t P>
+hipError_t tiles(const Args<S> &a, uint32_t groups, hipStream_t s) {
+    kv_tiles_kernel<S, P><<<groups * a.pairs * a.parts, kThreads, 0, s>>>(a);
+    return hipGetLastError();
+}
+
+template <typename S, uint32_t P>
+hipError_t weights(const Args<S> &a, uint32_t batch, uint32_t blocks, uint32_t row_parts, float *partial, hipStream_t s) {
+    kv_weights_kernel<S, P><<<dim3(blocks * row_parts, a.c.heads, batch), kThreads, 0, s>>>(a, row_parts, partial);
+    const hipError_t status = hipGetLastError();
+    if (status != hipSuccess || row_parts == 1) return status;
+    kv_weights_add_kernel<S><<<dim3((blocks * kTokens + kThreads - 1) / kThreads, a.c.heads, batch), kThreads, 0, s>>>(
+        a, row_parts, blocks * kTokens, partial);
+    return hipGetLastError();
+}
+
+}  // namespace
+
+bool tiles_fit(bool f32, uint32_t widest) { return !f32 || widest <= 128; }
+
+template <typename S>
+hipError_t launch_tiles(const Args<S> &a, uint32_t widest, uint32_t groups, hipStream_t s) {
+    if (widest <= 32) return tiles<S, 32>(a, groups, s);
+    if (widest <= 64) return tiles<S, 64>(a, groups, s);
+    if (widest <= 96) return tiles<S, 96>(a, groups, s);
+    if (widest <= 128) return tiles<S, 128>(a, groups, s);
+    if constexpr (sizeof(S) == 2) {
+        if (widest <= 192) return tiles<S, 192>(a, groups, s);
+        return tiles<S, 256>(a, groups, s);
+    }
+    return hipErrorInvalidValue;
+}
+
+template <typename S>
+hipError_t launch_weights(const Args<S> &a, uint32_t widest, uint32_t batch, uint32_t blocks, uint32_t row_parts,
+                          float *partial, hipStream_t s) {
+    if (widest <= 32) return weights<S, 32>(a, batch, blocks, row_parts, partial, s);
+    if (widest <= 64) return weights<S, 64>(a, batch, blocks, row_parts, partial, s);
+    if (widest <= 96) return weights<S, 96>(a, batch, blocks, row_parts, partial, s);
+    if (widest <= 128) return weights<S, 128>(a, batch, blocks, row_parts, partial, s);
+    if (widest <= 192) return weights<S, 192>(a, batch, blocks, row_parts, partial, s);
+    return weights<S, 256>(a, batch, blocks, row_parts, partial, s);
+}
+
+template hipError_t launch_tiles<float>(const Args<float> &, uint32_t, uint32_t, hipStream_t);
+template hipError_t launch_tiles<_Float16>(const Args<_Float16> &, uint32_t, uint32_t, hipStream_t);
+template hipError_t launch_weights<float>(const Args<float> &, uint32_t, uint32_t, uint32_t, uint32_t, float *, hipStream_t);
+template hipError_t launch_weights<_Float16>(const Args<_Float16> &, uint32_t, uint32_t, uint32_t, uint32_t, float *,
+                                             hipStream_t);
+
+}  // namespace kv
+}  // namespace icsdk

@@ -80,7 +80,7 @@ struct AttentionShape {
     size_t weight_stride;
 };
 // Bytes of workspace of a call (0: none).
-size_t attention_workspace(const View &c, const AttentionShape &a);
+size_t attention_workspace(bool f32, const View &c, const AttentionShape &a);
 hipError_t attention(bool f32, const View &c, const AttentionShape &a, const void *query, void *output,
                      void *workspace, hipStream_t s);
 

@@ -196,7 +196,7 @@ int attention(TensorDType dtype, const TensorKvCache *c, Buf query, const uint32
                                    recording ? (uint32_t)c->capacity : longest_of(c), scale, causal != 0, counts,
                                    static_cast<float *>(dev(weights)),
                                    (uint32_t)(tokens < c->capacity ? tokens : c->capacity), tokens};
-    const size_t bytes = kv::attention_workspace(c->view, shape);
+    const size_t bytes = kv::attention_workspace(dtype == TENSOR_DTYPE_F32, c->view, shape);
     ScratchBlock workspace(bytes);
     if (bytes != 0 && workspace.get() == nullptr)
         return fail(error, capacity, "cache attention: out of device memory for its workspace");
