@@ -454,9 +454,10 @@ Plan plan_of(bool f32, const View &c, const AttentionShape &a) {
     p.score_bytes = p.scores ? whole256(p.rows * p.score_stride * 4) : 0;
     p.row_parts = 1;
     if (p.row_bytes != 0 && blocks != 0) {
-        // weights: workgroups for every CU twice over, with 32 rows for each wave at least
-        const uint64_t groups = pairs * blocks, fit = (in_head + kTileRows - 1) / kTileRows;
-        const uint64_t want = groups >= kWorkgroups ? 1 : kWorkgroups / groups;
+        // weights: workgroups (of four blocks) for every CU twice over, with four
+        // steps of 32 rows at least
+        const uint64_t groups = pairs * ((blocks + kWaves - 1) / kWaves), fit = (in_head + kTileRows - 1) / kTileRows;
+        const uint64_t want = (kWorkgroups + groups - 1) / groups;
         p.row_parts = (uint32_t)(want < fit ? want : fit);
         if (p.row_parts > 1) p.partial_bytes = whole256(p.row_parts * pairs * p.score_stride * 4);
     }

@@ -85,14 +85,6 @@ template <typename S, uint32_t P> struct TileQuery {
                 }
         }
     }
-    __device__ inline void clear() {
-        factor = 1.0f;
-#pragma unroll
-        for (uint32_t c = 0; c < kSteps; ++c) {
-            hi[c] = half8{};
-            if constexpr (kPair) lo[c] = half8{};
-        }
-    }
 };
 
 // A block's factor of raw products, positive (queries carry the scale's sign), and
@@ -336,27 +328,30 @@ __global__ __launch_bounds__(kThreads, P <= 128 ? 2 : 1) void kv_tiles_kernel(Ar
     else if (a.row_ml != nullptr) a.row_ml[row] = weight_terms(big, sum);
 }
 
-// Softmax weights of one block's tokens, summed over the rows that see them: the
-// scores again, now with the rows' maxima and sums known. The block's keys stay in
-// registers; the waves walk the rows, 32 at a time, each with its next rows' loads
-// ahead. Where there are too few blocks for the chip, `row_parts` workgroups share
-// one's rows, and kv_weights_add_kernel adds their sums in order.
+// Softmax weights of four blocks' tokens, a wave each, summed over the rows that
+// see them: the scores again, now with the rows' maxima and sums known. A block's
+// keys stay in its wave's registers as A operands; the rows pass through LDS, 32
+// at a time, the next ones' loads ahead. Where there are too few blocks for the
+// chip, `row_parts` workgroups share four blocks' rows, and
+// kv_weights_add_kernel adds their sums in order.
 template <typename S, uint32_t P>
-__global__ __launch_bounds__(kThreads, P <= 64 ? 4 : P <= 128 ? 2 : 1) void kv_weights_kernel(Args<S> a,
-                                                                                              uint32_t row_parts,
-                                                                                              float *partial) {
+__global__ __launch_bounds__(kThreads, P <= 64 ? 3 : P <= 128 ? 2 : 1) void kv_weights_kernel(Args<S> a, uint32_t row_parts,
+                                                                               float *partial) {
     constexpr bool kPair = sizeof(S) == 4;
-    constexpr uint32_t KC = P / 16;
-    constexpr bool kAhead = !kPair && P <= 128;
-    __shared__ float lds_w[kWaves][kTokens];
+    constexpr uint32_t KC = P / 16, QROW = P + 8, kStep = 32;
+    constexpr uint32_t G = (P / 8 + 7) / 8;   // groups of 8 dims of a thread: 8 threads stage a row
+    __shared__ __attribute__((aligned(16))) _Float16 qs[2][kPair ? 2 : 1][kStep * QROW];
+    __shared__ f32x4 terms[2][kStep];         // of a row: maximum, 1 / sum (0: adds nothing), factor
     const View &c = a.c;
-    const uint32_t lane = threadIdx.x & 63, col = lane & 31, half = lane >> 5;
-    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const uint32_t t = blockIdx.x / row_parts, row_part = blockIdx.x % row_parts;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
+    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane(tid / kWave);
+    const uint32_t t0 = blockIdx.x / row_parts * kWaves, row_part = blockIdx.x % row_parts;
     const uint32_t h = blockIdx.y, b = blockIdx.z, seq = a.first + b;
     const size_t head = (size_t)seq * c.heads + h;
     const uint32_t length = c.length[seq], count = a.count.n[b];
-    if (t * kTokens >= length || count == 0) return;
+    if (t0 * kTokens >= length || count == 0) return;
+    const uint32_t blocks = (length + kTokens - 1) / kTokens;
+    const uint32_t t = min(t0 + wave, blocks - 1);   // (waves past the end repeat the last block)
     const uint32_t in_head = a.group * a.n;
     const bool open = t == length / kTokens;
     const Meta meta = c.meta[head * c.blocks + t];
@@ -374,84 +369,162 @@ __global__ __launch_bounds__(kThreads, P <= 64 ? 4 : P <= 128 ? 2 : 1) void kv_w
             }
         }
     const float sign = a.scale2 > 0.0 ? 1.0f : a.scale2 < 0.0 ? -1.0f : 0.0f;
-    const f32x2 f2 = block_factor(open ? 1.0f : meta.k_scale, a.scale2);
+    const float k_factor = block_factor(open ? 1.0f : meta.k_scale, a.scale2).x;
     float acc[32];
 #pragma unroll
     for (int e = 0; e < 32; ++e) acc[e] = 0.0f;
-    constexpr uint32_t kStep = kWaves * 32;
-    const uint32_t stride = kStep * row_parts;
-    const uint32_t first = (row_part * kWaves + wave) * 32;
-    auto row_of = [&](uint32_t row0) { return head * in_head + min(row0 + col, in_head - 1); };
-    TileQuery<S, P> next;
-    f32x2 next_ml;
-    auto load = [&](uint32_t row0) {
-        const size_t row = row_of(row0);
-        next.load(a.q + row * c.dim, c.dim, half, sign);
-        next_ml = a.row_ml[row];
+
+    const uint32_t steps = (in_head + kStep - 1) / kStep;
+    // the workgroup's steps: every row_parts-th, but those whose rows end before its blocks
+    auto skip = [&](uint32_t step) {
+        if (!a.causal) return false;
+        const uint32_t i = step * kStep % a.n, last = i + kStep - 1 < a.n ? i + kStep - 1 : a.n - 1;
+        return (int)length - (int)count + (int)min(last, count - 1) + 1 <= (int)(t0 * kTokens);
     };
-    if (kAhead && first < in_head) load(first);
-    for (uint32_t row0 = first; row0 < in_head; row0 += stride) {
-        const uint32_t r = row0 + col, i = r % a.n;
-        const bool live = r < in_head && i < count;
-        const int seen = seen_by(i, live, length, count, a.causal);
-        const bool any = wave_any(live && seen > (int)(t * kTokens));
-        if (!kAhead && any) load(row0);
-        TileQuery<S, P> q = next;
-        f32x2 ml = next_ml;
-        if (kAhead && row0 + stride < in_head) load(row0 + stride);
-        if (!any) continue;
-        // a row that adds nothing (padding, or not finite): raw products 0, times 0
-        if (!live) ml = f32x2{0.0f, 0.0f};
-        if (ml.y == 0.0f) q.clear();
-        const float factor = f2.x * q.factor;
-        float16v st[2];
+    auto from = [&](uint32_t step) {
+        while (step < steps && skip(step)) step += row_parts;
+        return step;
+    };
+    // staging: row tid / 8 of the step, groups tid % 8, + 8, ... of its dims
+    const uint32_t srow = tid / 8, sub = tid % 8;
+    typedef S vec8 __attribute__((ext_vector_type(8)));
+    vec8 x[G];
+    f32x2 ml;
+    auto fetch = [&](uint32_t step) {
+        const uint32_t r = step * kStep + srow;
+        const size_t row = head * in_head + min(r, in_head - 1);
+        const S *src = a.q + row * c.dim;
+        ml = a.row_ml[row];
+        if (r >= in_head || r % a.n >= count) ml = f32x2{0.0f, 0.0f};
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+        for (uint32_t g = 0; g < G; ++g) {
+            const uint32_t d = (sub + 8 * g) * 8;
+            if (c.dim % 8 == 0) {
+                x[g] = *reinterpret_cast<const vec8 *>(src + (d < c.dim ? d : 0));
+            } else {
 #pragma unroll
-            for (int e = 0; e < 16; ++e) st[s][e] = 0.0f;
-#pragma unroll
-        for (uint32_t ch = 0; ch < KC; ++ch)
-#pragma unroll
-            for (uint32_t s = 0; s < 2; ++s) {
-                st[s] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[s][ch], q.hi[ch], st[s], 0, 0, 0);
-                if constexpr (kPair) st[s] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[s][ch], q.lo[ch], st[s], 0, 0, 0);
-            }
-        if (wave_any(live && seen < (int)(t * kTokens + kTokens)) || meta.marked != 0) {
-#pragma unroll
-            for (uint32_t e = 0; e < 32; ++e) {
-                const uint32_t key = e / 8 * 16 + 8 * half + e % 8;
-                if ((int)(t * kTokens + key) >= seen || (meta.marked >> key & 1)) st[e / 16][e % 16] = -__builtin_inff();
+                for (uint32_t e = 0; e < 8; ++e) x[g][e] = src[d + e < c.dim ? d + e : 0];
             }
         }
+    };
+    auto stash = [&](uint32_t buf) {
+        // a row that adds nothing: zeros, so that its raw products are finite
 #pragma unroll
-        for (int e = 0; e < 32; ++e)
-            acc[e] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(st[e / 16][e % 16], factor, -ml.x)), ml.y, acc[e]);
-    }
+        for (uint32_t g = 0; g < G; ++g) {
+            const uint32_t d = (sub + 8 * g) * 8;
 #pragma unroll
-    for (uint32_t e = 0; e < 32; ++e) {
+            for (uint32_t e = 0; e < 8; ++e) x[g][e] = ml.y != 0.0f && d + e < c.dim ? x[g][e] * (S)sign : (S)0.0f;
+        }
+        float factor = 1.0f;
+        if constexpr (kPair) {
+            float big = 0.0f;
 #pragma unroll
-        for (int d = 1; d < 32; d *= 2) acc[e] += __shfl_xor(acc[e], d, kWave);
-        if (col == 0) lds_w[wave][e / 8 * 16 + 8 * half + e % 8] = acc[e];
+            for (uint32_t g = 0; g < G; ++g)
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[g][e]));
+#pragma unroll
+            for (int d = 1; d < 8; d *= 2) big = fmaxf(big, __shfl_xor(big, d, kWave));
+            const int exponent = big > 0.0f ? __builtin_amdgcn_frexp_expf(big) : 14;
+            factor = __builtin_ldexpf(1.0f, exponent - 14);
+#pragma unroll
+            for (uint32_t g = 0; g < G; ++g) {
+                half8 hi, lo;
+#pragma unroll
+                for (uint32_t e = 0; e < 8; ++e) {
+                    const float y = __builtin_ldexpf(x[g][e], 14 - exponent);
+                    hi[e] = (_Float16)y;
+                    lo[e] = (_Float16)(y - (float)hi[e]);
+                }
+                const uint32_t d = (sub + 8 * g) * 8;
+                if (d < P) {
+                    *reinterpret_cast<half8 *>(&qs[buf][0][srow * QROW + d]) = hi;
+                    *reinterpret_cast<half8 *>(&qs[buf][1][srow * QROW + d]) = lo;
+                }
+            }
+        } else {
+#pragma unroll
+            for (uint32_t g = 0; g < G; ++g) {
+                const uint32_t d = (sub + 8 * g) * 8;
+                if (d < P) *reinterpret_cast<half8 *>(&qs[buf][0][srow * QROW + d]) = x[g];
+            }
+        }
+        if (sub == 0) terms[buf][srow] = f32x4{ml.x, ml.y, factor, 0.0f};
+    };
+    uint32_t step = from(row_part), buf = 0;
+    if (step < steps) {
+        fetch(step);
+        stash(0);
     }
     __syncthreads();
-    const uint32_t token = t * kTokens + lane;
-    if (wave == 0 && token < min(length, a.weight_tokens)) {
-        float total = 0.0f;
-        for (uint32_t w = 0; w < kWaves; ++w) total += lds_w[w][lane];
-        if (row_parts == 1) a.weights[head * a.weight_stride + token] += total;
-        else partial[(row_part * (size_t)a.c.heads * gridDim.z + ((size_t)b * c.heads + h)) * (gridDim.x / row_parts * kTokens) + token] = total;
+    for (uint32_t next; step < steps; step = next, buf ^= 1) {
+        next = from(step + row_parts);
+        if (next < steps) fetch(next);
+        const uint32_t r = step * kStep + col, i = r % a.n;
+        const bool live = r < in_head && i < count;
+        const int seen = seen_by(i, live, length, count, a.causal);
+        if (wave_any(live && seen > (int)(t * kTokens))) {
+            const f32x4 term = terms[buf][col];
+            const float factor = k_factor * term.z;
+            float16v st[2];
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) st[s][e] = 0.0f;
+#pragma unroll
+            for (uint32_t ch = 0; ch < KC; ++ch) {
+                const half8 hi = *reinterpret_cast<const half8 *>(&qs[buf][0][col * QROW + 16 * ch + 8 * half]);
+#pragma unroll
+                for (uint32_t s = 0; s < 2; ++s)
+                    st[s] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[s][ch], hi, st[s], 0, 0, 0);
+                if constexpr (kPair) {
+                    const half8 lo = *reinterpret_cast<const half8 *>(&qs[buf][1][col * QROW + 16 * ch + 8 * half]);
+#pragma unroll
+                    for (uint32_t s = 0; s < 2; ++s)
+                        st[s] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[s][ch], lo, st[s], 0, 0, 0);
+                }
+            }
+            if (wave_any(live && seen < (int)(t * kTokens + kTokens)) || meta.marked != 0) {
+#pragma unroll
+                for (uint32_t e = 0; e < 32; ++e) {
+                    const uint32_t key = e / 8 * 16 + 8 * half + e % 8;
+                    if ((int)(t * kTokens + key) >= seen || (meta.marked >> key & 1)) st[e / 16][e % 16] = -__builtin_inff();
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 32; ++e)
+                acc[e] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(st[e / 16][e % 16], factor, -term.x)), term.y,
+                                        acc[e]);
+        }
+        if (next < steps) stash(buf ^ 1);
+        __syncthreads();
     }
+    // sums over the 32 rows of a half wave: each exchange halves the values, and
+    // lane col ends with value col
+#pragma unroll
+    for (uint32_t n = 16; n >= 1; n /= 2)
+#pragma unroll
+        for (uint32_t j = 0; j < n; ++j) {
+            const bool upper = col & n;
+            const float mine = upper ? acc[j + n] : acc[j], other = upper ? acc[j] : acc[j + n];
+            acc[j] = mine + __shfl_xor(other, n, kWave);
+        }
+    const uint32_t token = t * kTokens + col / 8 * 16 + 8 * half + col % 8;
+    if (t0 + wave >= blocks || token >= min(length, a.weight_tokens)) return;
+    if (row_parts == 1)
+        a.weights[head * a.weight_stride + token] += acc[0];
+    else
+        partial[((size_t)row_part * a.pairs + (size_t)b * c.heads + h) * a.score_stride + token] = acc[0];
 }
 
 template <typename S>
-__global__ __launch_bounds__(kThreads) void kv_weights_add_kernel(Args<S> a, uint32_t row_parts, uint32_t tokens,
+__global__ __launch_bounds__(kThreads) void kv_weights_add_kernel(Args<S> a, uint32_t row_parts,
                                                                   const float *partial) {
     const View &c = a.c;
     const uint32_t t = blockIdx.x * kThreads + threadIdx.x, h = blockIdx.y, b = blockIdx.z, seq = a.first + b;
     if (a.count.n[b] == 0 || t >= min(c.length[seq], a.weight_tokens)) return;
     float total = 0.0f;
     for (uint32_t p = 0; p < row_parts; ++p)
-        total += partial[(p * (size_t)c.heads * gridDim.z + ((size_t)b * c.heads + h)) * tokens + t];
+        total += partial[((size_t)p * a.pairs + (size_t)b * c.heads + h) * a.score_stride + t];
     a.weights[((size_t)seq * c.heads + h) * a.weight_stride + t] += total;
 }
 
@@ -463,11 +536,12 @@ hipError_t tiles(const Args<S> &a, uint32_t groups, hipStream_t s) {
 
 template <typename S, uint32_t P>
 hipError_t weights(const Args<S> &a, uint32_t batch, uint32_t blocks, uint32_t row_parts, float *partial, hipStream_t s) {
-    kv_weights_kernel<S, P><<<dim3(blocks * row_parts, a.c.heads, batch), kThreads, 0, s>>>(a, row_parts, partial);
+    const uint32_t fours = (blocks + kWaves - 1) / kWaves;
+    kv_weights_kernel<S, P><<<dim3(fours * row_parts, a.c.heads, batch), kThreads, 0, s>>>(a, row_parts, partial);
     const hipError_t status = hipGetLastError();
     if (status != hipSuccess || row_parts == 1) return status;
     kv_weights_add_kernel<S><<<dim3((blocks * kTokens + kThreads - 1) / kThreads, a.c.heads, batch), kThreads, 0, s>>>(
-        a, row_parts, blocks * kTokens, partial);
+        a, row_parts, partial);
     return hipGetLastError();
 }
 
