@@ -177,8 +177,8 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(Args<S> a) {
             const uint32_t mine = (uint32_t)(meta.marked >> (16 * g));
 #pragma unroll
             for (uint32_t e = 0; e < 16; ++e) {
-                if (mine >> e & 1) p[e] = __builtin_nanf("");
-                if ((int)(t * kTokens + 16 * g + e) >= seen) p[e] = neg_inf;
+                p[e] = mine >> e & 1 ? __builtin_nanf("") : p[e];
+                p[e] = (int)(t * kTokens + 16 * g + e) >= seen ? neg_inf : p[e];
             }
         }
         if (a.scores != nullptr && live) {
@@ -265,14 +265,16 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(Args<S> a) {
     };
     const uint32_t end_whole = min(end, whole);
     uint32_t t = begin + wave;
+    Meta now_meta = scalar_meta(meta + min(t, c.blocks - 1));
     if (t < end_whole) {
         load_k(t);
         load_v(t);
     }
     for (; t < end_whole; t += kWaves) {
         const uint32_t next = t + kWaves;
+        const Meta next_meta = scalar_meta(meta + min(next, c.blocks - 1));   // (asked for a block ahead, as the codes are)
         step(
-            t, meta[t],
+            t, now_meta,
             [&](uint32_t u, uint32_t s) {
                 if (s / 2 < NC) return codes(kr[u][s / 2][s % 2 * 2], kr[u][s / 2][s % 2 * 2 + 1]);
                 return codes(ko[u].x, ko[u].y);
@@ -282,12 +284,13 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(Args<S> a) {
                 if (next < end_whole) load_k(next);
             });
         if (next < end_whole) load_v(next);
+        now_meta = next_meta;
     }
     if (t == whole && t < end) {   // the open block, in f16
         const _Float16 *kt = c.kt + (head * kTokens + key_of) * c.kp;
         const _Float16 *vt = c.vt + (head * c.vp + m) * kTokens + g * 16;
         step(
-            t, Meta{1.0f, 1.0f, meta[t].marked},
+            t, Meta{1.0f, 1.0f, now_meta.marked},
             [&](uint32_t u, uint32_t s) {
                 const uint32_t d = step_dim<P>(s, g);
                 return *reinterpret_cast<const half8 *>(kt + 4 * u * c.kp + (d < c.kp ? d : 0));

@@ -9,10 +9,8 @@
 //     keys 16 c + 8 (l / 32) + 0 .. 7: consecutive, and
 //   out^T = V^T P^T takes them as B operands in their order, with the dim's same
 //     keys side by side in memory: one 16-byte LDS read per A operand.
-// A workgroup turns each block's codes to f16 once, on their way into LDS (key
-// rows 8 halves longer than the data, dim rows of 72: no bank conflicts); the next
-// block's codes are asked for before a block is computed and written to the other
-// buffer after it, one barrier per block.
+// Each block's codes are turned to f16 once, on their way into LDS (key rows 8
+// halves longer than the data, dim rows of 72: no bank conflicts).
 // Scores stay raw products; the block's factor k_scale * scale * log2 e enters with
 // the maximum in one fma, the ratio of its value scale to the unit as an addend of
 // the exponent (k_kv_attention.hip has the rules).
@@ -98,13 +96,52 @@ __device__ inline f32x2 block_factor(float k_scale, double scale2) {
 // Key row of the block that A row m of a half reads.
 __device__ inline uint32_t swap23(uint32_t m) { return (m & 0x13u) | (m & 4u) << 1 | (m & 8u) >> 1; }
 
+// The mark bits of a lane's 32 keys, in its order of them (16 i + 8 half + 0 .. 7).
+__device__ inline uint32_t marks_of(uint64_t marked, uint32_t half) {
+    const uint64_t m = marked >> (8 * half);
+    return (uint32_t)(m & 255u) | (uint32_t)(m >> 8 & 0xff00u) | (uint32_t)(m >> 16 & 0xff0000u) |
+           (uint32_t)(m >> 24 & 0xff000000u);
+}
+
+// N matrix steps with other work in between: operand(i) reads step i's A operand
+// (four steps ahead), product(i, operand) issues its MFMA, work(i) is step i's share
+// of the rest, and nothing moves from one step to another. An MFMA takes 8 cycles to
+// issue and 32 to complete, and the SIMD issues 6 vector instructions (3
+// transcendental ones) meanwhile at no cost, but only if they come in between: of
+// two waves on a SIMD, one in a stretch of MFMAs and one in a stretch of vector
+// instructions, neither gained, and the compiler by itself makes such stretches.
+template <uint32_t N, typename R, typename M, typename W>
+__device__ inline void steps(R operand, M product, W work) {
+    constexpr uint32_t kAhead = 4;
+    half8 a[N];
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (uint32_t i = 0; i < kAhead && i < N; ++i) a[i] = operand(i);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (uint32_t i = 0; i < N; ++i) {
+        product(i, a[i]);
+        if (i + kAhead < N) a[i + kAhead] = operand(i + kAhead);
+        work(i);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+// A workgroup: 128 packed rows, 32 per wave, of one (sequence, kv head), and one
+// part of its blocks; the open block first. The loop is skewed: turn s multiplies
+// P of tile s - 1 with its values while it takes the maxima of tile s and turns
+// codes to f16, then multiplies the keys of tile s + 1 while it takes the
+// exponentials of tile s.
 template <typename S, uint32_t P>
-__global__ __launch_bounds__(kThreads, P <= 128 ? 2 : 1) void kv_tiles_kernel(Args<S> a) {
+__global__ __launch_bounds__(kThreads, sizeof(S) == 2 && P <= 128 ? 2 : 1) void kv_tiles_kernel(Args<S> a) {
     constexpr bool kPair = sizeof(S) == 4;
     constexpr uint32_t KC = P / 16, VT = (P + 31) / 32;
     constexpr uint32_t KROW = P + 8, VROW = kTokens + 8;   // LDS rows, halves
+    constexpr uint32_t KTILE = kTokens * KROW, VTILE = VT * 32 * VROW;
     constexpr uint32_t KPER = (kTokens * P / 16 + kThreads - 1) / kThreads;   // 16-byte pieces of codes per thread
-    __shared__ __attribute__((aligned(16))) _Float16 ks[2][kTokens * KROW], vs[2][VT * 32 * VROW];
+    // (each tile with a spare place, for pieces past the end)
+    __shared__ __attribute__((aligned(16))) _Float16 ks[2][KTILE + 16], vs[2][VTILE + 16];
+    __shared__ int wave_most[kWaves];
     const View &c = a.c;
     const uint32_t tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane(tid / kWave);
@@ -120,196 +157,243 @@ __global__ __launch_bounds__(kThreads, P <= 128 ? 2 : 1) void kv_tiles_kernel(Ar
     const bool live = r < in_head && i < count;
     const size_t row = head * in_head + min(r, in_head - 1);
     const int seen = seen_by(i, live, length, count, a.causal);
-    // keys that some row of the wave, and of the workgroup, sees
+    // keys that some row of the workgroup, and that every row of the wave, sees
     int most = live ? seen : 0, least = live ? seen : (int)length;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
         most = max(most, __shfl_xor(most, d, kWave));
         least = min(least, __shfl_xor(least, d, kWave));
     }
-    most = __builtin_amdgcn_readfirstlane(most);
     least = __builtin_amdgcn_readfirstlane(least);
-    __shared__ int wave_most[kWaves];
     if (lane == 0) wave_most[wave] = most;
     __syncthreads();
-    int all_most = wave_most[0];
+    most = wave_most[0];
 #pragma unroll
-    for (uint32_t w = 1; w < kWaves; ++w) all_most = max(all_most, wave_most[w]);
-    const uint32_t blocks = ((uint32_t)max(all_most, 0) + kTokens - 1) / kTokens, whole = length / kTokens;
+    for (uint32_t w = 1; w < kWaves; ++w) most = max(most, wave_most[w]);
+    most = __builtin_amdgcn_readfirstlane(most);
+    const uint32_t blocks = ((uint32_t)max(most, 0) + kTokens - 1) / kTokens, whole = length / kTokens;
     const uint32_t share = (blocks + a.parts - 1) / a.parts;
-    const uint32_t begin = min(part * share, blocks), end = min(begin + share, blocks);
+    const uint32_t begin = min(part * share, blocks), end = min(begin + share, blocks), tiles = end - begin;
+    // tile s is block begin + s, or with the open block among them that one first
+    const uint32_t open_first = end > whole ? 1 : 0;
+    auto block_of = [&](uint32_t s) { return open_first && s == 0 ? whole : min(begin + s - open_first, c.blocks - 1); };
 
     TileQuery<S, P> q;
     q.load(a.q + row * c.dim, c.dim, half, a.scale2 > 0.0 ? 1.0f : a.scale2 < 0.0 ? -1.0f : 0.0f);
     const Meta *const meta = c.meta + head * c.blocks;
     const uint8_t *const kcodes = c.k + head * c.blocks * kTokens * c.kp;
     const uint8_t *const vcodes = c.v + head * c.blocks * kTokens * c.vp;
+    auto meta_of = [&](uint32_t s) {
+        Meta m = scalar_meta(meta + block_of(s));
+        if (open_first && s == 0) m.k_scale = m.v_scale = 1.0f;
+        return m;
+    };
 
     // the thread's 16-byte pieces of a block's codes (pieces past the end repeat the
-    // last one and are not written)
+    // last one and go to the spare place: no branch lies between the MFMAs)
     const uint32_t kpieces = kTokens * c.kp / 16, vpieces = c.vp * 4;
     uint32_t kto[KPER], vto[KPER];
 #pragma unroll
     for (uint32_t u = 0; u < KPER; ++u) {
         const uint32_t p = tid + u * kThreads;
-        kto[u] = p * 16 / c.kp * KROW + p * 16 % c.kp;
-        vto[u] = p / 4 * VROW + p % 4 * 16;
+        kto[u] = p < kpieces ? p * 16 / c.kp * KROW + p * 16 % c.kp : KTILE;
+        vto[u] = p < vpieces ? p / 4 * VROW + p % 4 * 16 : VTILE;
     }
     u32x4 kreg[KPER], vreg[KPER];
-    auto fetch = [&](uint32_t t) {
+    // (asked for without a test, past the end some block again: the count of loads
+    // in flight is then known wherever one is waited for)
+    auto fetch_k = [&](uint32_t s) {
+        const u32x4 *from = reinterpret_cast<const u32x4 *>(kcodes + (size_t)block_of(s) * kTokens * c.kp);
 #pragma unroll
-        for (uint32_t u = 0; u < KPER; ++u) {
-            const uint32_t p = tid + u * kThreads;
-            kreg[u] = reinterpret_cast<const u32x4 *>(kcodes + (size_t)t * kTokens * c.kp)[min(p, kpieces - 1)];
-            vreg[u] = reinterpret_cast<const u32x4 *>(vcodes + (size_t)t * kTokens * c.vp)[min(p, vpieces - 1)];
-        }
+        for (uint32_t u = 0; u < KPER; ++u) kreg[u] = from[min(tid + u * kThreads, kpieces - 1)];
+    };
+    auto fetch_v = [&](uint32_t s) {
+        const u32x4 *from = reinterpret_cast<const u32x4 *>(vcodes + (size_t)block_of(s) * kTokens * c.vp);
+#pragma unroll
+        for (uint32_t u = 0; u < KPER; ++u) vreg[u] = from[min(tid + u * kThreads, vpieces - 1)];
     };
     auto put = [&](_Float16 *to, half8 lo, half8 hi) {
         *reinterpret_cast<half8 *>(to) = lo;
         *reinterpret_cast<half8 *>(to + 8) = hi;
     };
-    auto stash = [&](uint32_t buf) {
+    auto stash_k = [&](uint32_t buf) {
 #pragma unroll
-        for (uint32_t u = 0; u < KPER; ++u) {
-            const uint32_t p = tid + u * kThreads;
-            if (p < kpieces) put(&ks[buf][kto[u]], codes(kreg[u].x, kreg[u].y), codes(kreg[u].z, kreg[u].w));
-            if (p < vpieces) put(&vs[buf][vto[u]], codes(vreg[u].x, vreg[u].y), codes(vreg[u].z, vreg[u].w));
-        }
+        for (uint32_t u = 0; u < KPER; ++u)
+            put(&ks[buf][kto[u]], codes(kreg[u].x, kreg[u].y), codes(kreg[u].z, kreg[u].w));
     };
-    auto stash_open = [&](uint32_t buf) {   // the open block lies in f16
-        const half8 *kt = reinterpret_cast<const half8 *>(c.kt + head * kTokens * c.kp);
-        const half8 *vt = reinterpret_cast<const half8 *>(c.vt + head * kTokens * c.vp);
+
+    const float neg_inf = -__builtin_inff();
+    float16v o[VT], st[2];
+    half8 ph[4], pl[kPair ? 4 : 1];
 #pragma unroll
-        for (uint32_t u = 0; u < KPER; ++u) {
-            const uint32_t p = tid + u * kThreads;
-            if (p < kpieces) put(&ks[buf][kto[u]], kt[2 * p], kt[2 * p + 1]);
-            if (p < vpieces) put(&vs[buf][vto[u]], vt[2 * p], vt[2 * p + 1]);
-        }
+    for (uint32_t t = 0; t < VT; ++t)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) o[t][e] = 0.0f;
+#pragma unroll
+    for (uint32_t ch = 0; ch < 4; ++ch) {
+        ph[ch] = half8{};
+        if constexpr (kPair) pl[ch] = half8{};
+    }
+    float big = neg_inf, sum = 0.0f, unit = 1.0f;   // (sum: of the lane's keys)
+    constexpr uint32_t NS = 2 * KC, NO = 4 * VT;   // matrix steps of a tile's scores and outputs
+    auto key_operand = [&](uint32_t buf, uint32_t i) {
+        return *reinterpret_cast<const half8 *>(&ks[buf][(32 * (i % 2) + swap23(col)) * KROW + 16 * (i / 2) + 8 * half]);
     };
-    // columns past the padded dim meet zeros of q, and must not be NaN
+    auto value_operand = [&](uint32_t buf, uint32_t i) {
+        return *reinterpret_cast<const half8 *>(&vs[buf][(32 * (i % VT) + col) * VROW + 16 * (i / VT) + 8 * half]);
+    };
+    auto score = [&](float16v (&to)[2], uint32_t i, half8 k) {
+        to[i % 2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q.hi[i / 2], to[i % 2], 0, 0, 0);
+        if constexpr (kPair) to[i % 2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q.lo[i / 2], to[i % 2], 0, 0, 0);
+    };
+    auto output = [&](uint32_t i, half8 v) {
+        o[i % VT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[i / VT], o[i % VT], 0, 0, 0);
+        if constexpr (kPair) o[i % VT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[i / VT], o[i % VT], 0, 0, 0);
+    };
+    auto clear = [](float16v (&to)[2]) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) to[s][e] = 0.0f;
+    };
+    // unit u of a turn's codes: 8 of the thread's, to f16 and into LDS
+    auto unit_of_codes = [&](uint32_t u, uint32_t buf) {
+        const bool keys = u >= 2 * KPER;
+        const uint32_t piece = u / 2 % KPER, second = u % 2;
+        const u32x4 w = keys ? kreg[piece] : vreg[piece];
+        const half8 x = second ? codes(w.z, w.w) : codes(w.x, w.y);
+        _Float16 *const to = keys ? &ks[buf][kto[piece]] : &vs[buf][vto[piece]];
+        *reinterpret_cast<half8 *>(to + 8 * second) = x;
+    };
+
+    // columns past the padded dim meet zeros of q, and the first turn's P of no
+    // tile meets these values: neither may be NaN
     for (uint32_t p = tid; p < kTokens * (P - c.kp) / 8; p += kThreads) {
         const uint32_t per = (P - c.kp) / 8, t = p / per, d = c.kp + p % per * 8;
         *reinterpret_cast<half8 *>(&ks[0][t * KROW + d]) = half8{};
         *reinterpret_cast<half8 *>(&ks[1][t * KROW + d]) = half8{};
     }
-
-    const float neg_inf = -__builtin_inff();
-    float16v o[VT];
+    for (uint32_t p = tid; p < VTILE / 8; p += kThreads) reinterpret_cast<half8 *>(vs[1])[p] = half8{};
+    fetch_k(0);
+    fetch_v(0);
+    if (tiles != 0) {
+        if (open_first) {   // it lies in f16
+            const half8 *kt = reinterpret_cast<const half8 *>(c.kt + head * kTokens * c.kp);
 #pragma unroll
-    for (uint32_t t = 0; t < VT; ++t)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[t][e] = 0.0f;
-    float big = neg_inf, sum = 0.0f, unit = 1.0f;   // (sum: of the lane's keys)
-
-    if (begin < end) {
-        if (begin < whole) {
-            fetch(begin);
-            stash(0);
+            for (uint32_t u = 0; u < KPER; ++u) {
+                const uint32_t p = min(tid + u * kThreads, kpieces - 1);
+                put(&ks[0][kto[u]], kt[2 * p], kt[2 * p + 1]);
+            }
         } else {
-            stash_open(0);
+            stash_k(0);
         }
+    }
+    fetch_k(1);
+    stash_k(1);
+    fetch_k(2);
+    Meta next_meta = meta_of(0);
+    float inverse_unit = 1.0f;
+    __syncthreads();
+    clear(st);
+    steps<NS>([&](uint32_t i) { return key_operand(0, i); }, [&](uint32_t i, half8 k) { score(st, i, k); }, [](uint32_t) {});
+    auto turn = [&](uint32_t s, float16v (&now)[2], float16v (&ahead)[2]) {
+        const Meta m = next_meta;
+        const uint32_t t = block_of(s);
+        next_meta = meta_of(s + 1);
+        __syncthreads();
+        if ((int)(t * kTokens + kTokens) > least || m.marked != 0) {
+            const int last = seen - (int)(t * kTokens);
+            const uint32_t mine = marks_of(m.marked, half);
+#pragma unroll
+            for (uint32_t e = 0; e < 32; ++e) {
+                const uint32_t key = e / 8 * 16 + 8 * half + e % 8;
+                const float x = mine >> e & 1 ? __builtin_nanf("") : now[e / 16][e % 16];
+                now[e / 16][e % 16] = (int)key >= last ? neg_inf : x;
+            }
+        }
+        const f32x2 f2 = block_factor(m.k_scale, a.scale2);
+        const float factor = f2.x * q.factor;
+        float part_max[4] = {neg_inf, neg_inf, neg_inf, neg_inf};
+        steps<NO>([&](uint32_t i) { return value_operand((s + 1) & 1, i); }, [&](uint32_t i, half8 v) { output(i, v); },
+                  [&](uint32_t i) {
+#pragma unroll
+                      for (uint32_t u = i * 4 * KPER / NO; u < (i + 1) * 4 * KPER / NO; ++u) unit_of_codes(u, s & 1);
+#pragma unroll
+                      for (uint32_t e = i * 32 / NO; e < (i + 1) * 32 / NO; ++e)
+                          part_max[e % 4] = fmaxf(part_max[e % 4], now[e / 16][e % 16]);
+                  });
+        const float raw = fmaxf(fmaxf(part_max[0], part_max[1]), fmaxf(part_max[2], part_max[3]));
+        fetch_v(s + 1);
+        fetch_k(s + 3);
+        const float top = raw * factor;
+        if (__builtin_amdgcn_ballot_w64(top > big + kLazy<S>) != 0) {
+            const float up = flash::pair_max(fmaxf(top, big));
+            const float alpha = up == neg_inf ? 1.0f : __builtin_amdgcn_exp2f(big - up);
+            sum *= alpha;
+#pragma unroll
+            for (uint32_t v = 0; v < VT; ++v) o[v] *= alpha;
+            big = up;
+        }
+        float ratio = m.v_scale * inverse_unit;
+        if (m.v_scale == 0.0f) {
+            ratio = 1.0f;
+        } else if (ratio > kUnitRange || ratio < 1.0f / kUnitRange) {
+#pragma unroll
+            for (uint32_t v = 0; v < VT; ++v) o[v] *= unit / m.v_scale;
+            unit = m.v_scale;
+            inverse_unit = 1.0f / unit;
+            ratio = 1.0f;
+        }
+        // exponents are relative to this; with nothing seen every score is -inf or NaN
+        const float base = (big == neg_inf ? 0.0f : big - kHeadroom<S>) - __builtin_amdgcn_logf(ratio);
+        float add[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        clear(ahead);
+        // (after the last tile: the scores of an old one, not used)
+        steps<NS>([&](uint32_t i) { return key_operand((s + 1) & 1, i); }, [&](uint32_t i, half8 k) { score(ahead, i, k); },
+                  [&](uint32_t i) {
+#pragma unroll
+                      for (uint32_t e = i * 32 / NS; e < (i + 1) * 32 / NS; ++e) {
+                          const float raw_score = now[e / 16][e % 16];
+                          float x = __builtin_fmaf(raw_score, factor, -base);
+                          if constexpr (kPair) {
+                              const float off = raw_score * (f2.y * q.factor);
+                              x += fabsf(off) < 1.0f ? off : 0.0f;   // (not for -inf)
+                          }
+                          x = __builtin_amdgcn_exp2f(x);
+                          ph[e / 8][e % 8] = (_Float16)x;
+                          if constexpr (kPair) {
+                              pl[e / 8][e % 8] = (_Float16)(x - (float)ph[e / 8][e % 8]);
+                              add[e % 4] += x;
+                          } else if (e % 2 == 1) {   // the sum of P as the product has it
+                              const half2_t ones = {(_Float16)1.0f, (_Float16)1.0f};
+                              add[e / 2 % 4] = __builtin_amdgcn_fdot2(half2_t{ph[e / 8][e % 8 - 1], ph[e / 8][e % 8]}, ones,
+                                                                      add[e / 2 % 4], false);
+                          }
+                          // (taken here, not moved to where it is used)
+                          if (e % 8 == 7) {
+                              asm volatile("" : "+v"(ph[e / 8]));
+                              if constexpr (kPair) asm volatile("" : "+v"(pl[e / 8]));
+                          }
+                      }
+                  });
+        sum += ((add[0] + add[1]) + (add[2] + add[3])) * fast_rcp(ratio);
+    };
+    float16v other[2];
+    for (uint32_t s = 0; s < tiles; s += 2) {   // (two score tiles in turn: no copies)
+        turn(s, st, other);
+        if (open_first && s == 0) {   // its values, over what turn 0 wrote in their place
+            const half8 *vt = reinterpret_cast<const half8 *>(c.vt + head * kTokens * c.vp);
+#pragma unroll
+            for (uint32_t u = 0; u < KPER; ++u) {
+                const uint32_t p = min(tid + u * kThreads, vpieces - 1);
+                put(&vs[0][vto[u]], vt[2 * p], vt[2 * p + 1]);
+            }
+        }
+        if (s + 1 < tiles) turn(s + 1, other, st);
     }
     __syncthreads();
-    for (uint32_t t = begin; t < end; ++t) {
-        const uint32_t buf = (t - begin) & 1;
-        if (t + 1 < end && t + 1 < whole) fetch(t + 1);
-        if ((int)(t * kTokens) < most) {
-            Meta m = meta[t];
-            if (t >= whole) m.k_scale = m.v_scale = 1.0f;
-            float16v st[2];
-#pragma unroll
-            for (int s = 0; s < 2; ++s)
-#pragma unroll
-                for (int e = 0; e < 16; ++e) st[s][e] = 0.0f;
-            flash::mfma_phase_begin();
-#pragma unroll
-            for (uint32_t ch = 0; ch < KC; ++ch)
-#pragma unroll
-                for (uint32_t s = 0; s < 2; ++s) {
-                    const half8 k = *reinterpret_cast<const half8 *>(
-                        &ks[buf][(32 * s + swap23(col)) * KROW + 16 * ch + 8 * half]);
-                    st[s] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q.hi[ch], st[s], 0, 0, 0);
-                    if constexpr (kPair) st[s] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q.lo[ch], st[s], 0, 0, 0);
-                }
-            if constexpr (2 * KC > 4) flash::lds_read_ahead<2 * KC, 1, kPair ? 2 : 1>();
-            flash::mfma_phase_end();
-            const f32x2 f2 = block_factor(m.k_scale, a.scale2);
-            const float factor = f2.x * q.factor;
-            if ((int)(t * kTokens + kTokens) > least || m.marked != 0) {
-#pragma unroll
-                for (uint32_t e = 0; e < 32; ++e) {
-                    const uint32_t key = e / 8 * 16 + 8 * half + e % 8;
-                    if (m.marked >> key & 1) st[e / 16][e % 16] = __builtin_nanf("");
-                    if ((int)(t * kTokens + key) >= seen) st[e / 16][e % 16] = neg_inf;
-                }
-            }
-            float part_max[4] = {neg_inf, neg_inf, neg_inf, neg_inf};
-#pragma unroll
-            for (int e = 0; e < 32; ++e) part_max[e % 4] = fmaxf(part_max[e % 4], st[e / 16][e % 16]);
-            const float raw = fmaxf(fmaxf(part_max[0], part_max[1]), fmaxf(part_max[2], part_max[3]));
-            const float top = raw * factor;
-            if (__builtin_amdgcn_ballot_w64(top > big + kLazy<S>) != 0) {
-                const float now = flash::pair_max(fmaxf(top, big));
-                const float alpha = now == neg_inf ? 1.0f : __builtin_amdgcn_exp2f(big - now);
-                sum *= alpha;
-#pragma unroll
-                for (uint32_t v = 0; v < VT; ++v) o[v] *= alpha;
-                big = now;
-            }
-            float ratio = m.v_scale / unit;
-            if (m.v_scale == 0.0f) {
-                ratio = 1.0f;
-            } else if (ratio > kUnitRange || ratio < 1.0f / kUnitRange) {
-#pragma unroll
-                for (uint32_t v = 0; v < VT; ++v) o[v] *= unit / m.v_scale;
-                unit = m.v_scale;
-                ratio = 1.0f;
-            }
-            // exponents are relative to this; with nothing seen every score is -inf or NaN
-            const float base = (big == neg_inf ? 0.0f : big - kHeadroom<S>) - __builtin_amdgcn_logf(ratio);
-            half8 ph[4], pl[kPair ? 4 : 1];
-            float add[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-                const float s = st[e / 16][e % 16];
-                float x = __builtin_fmaf(s, factor, -base);
-                if constexpr (kPair) {
-                    const float off = s * (f2.y * q.factor);
-                    x += fabsf(off) < 1.0f ? off : 0.0f;   // (not for -inf)
-                }
-                x = __builtin_amdgcn_exp2f(x);
-                ph[e / 8][e % 8] = (_Float16)x;
-                if constexpr (kPair) {
-                    pl[e / 8][e % 8] = (_Float16)(x - (float)ph[e / 8][e % 8]);
-                    add[e % 4] += x;
-                }
-            }
-            if constexpr (!kPair) {   // the sum of P as the product has it
-                const half2_t ones = {(_Float16)1.0f, (_Float16)1.0f};
-#pragma unroll
-                for (int e = 0; e < 16; ++e)
-                    add[e % 4] = __builtin_amdgcn_fdot2(half2_t{ph[e / 4][2 * (e % 4)], ph[e / 4][2 * (e % 4) + 1]}, ones,
-                                                        add[e % 4], false);
-            }
-            sum += ((add[0] + add[1]) + (add[2] + add[3])) * (1.0f / ratio);
-            flash::mfma_phase_begin();
-#pragma unroll
-            for (uint32_t ch = 0; ch < 4; ++ch)
-#pragma unroll
-                for (uint32_t v = 0; v < VT; ++v) {
-                    const half8 vf = *reinterpret_cast<const half8 *>(&vs[buf][(32 * v + col) * VROW + 16 * ch + 8 * half]);
-                    o[v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, ph[ch], o[v], 0, 0, 0);
-                    if constexpr (kPair) o[v] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, pl[ch], o[v], 0, 0, 0);
-                }
-            if constexpr (4 * VT > 4) flash::lds_read_ahead<4 * VT, 1, kPair ? 2 : 1>();
-            flash::mfma_phase_end();
-        }
-        if (t + 1 < end) {
-            if (t + 1 < whole) stash(buf ^ 1);
-            else stash_open(buf ^ 1);
-        }
-        __syncthreads();
-    }
+    steps<NO>([&](uint32_t i) { return value_operand((tiles + 1) & 1, i); }, [&](uint32_t i, half8 v) { output(i, v); },
+              [](uint32_t) {});
     sum = flash::pair_sum(sum);
     big -= kHeadroom<S>;
     if (!live) return;
@@ -484,10 +568,12 @@ __global__ __launch_bounds__(kThreads, P <= 64 ? 3 : P <= 128 ? 2 : 1) void kv_w
                 }
             }
             if (wave_any(live && seen < (int)(t * kTokens + kTokens)) || meta.marked != 0) {
+                const int last = seen - (int)(t * kTokens);
+                const uint32_t mine = marks_of(meta.marked, half);
 #pragma unroll
                 for (uint32_t e = 0; e < 32; ++e) {
                     const uint32_t key = e / 8 * 16 + 8 * half + e % 8;
-                    if ((int)(t * kTokens + key) >= seen || (meta.marked >> key & 1)) st[e / 16][e % 16] = -__builtin_inff();
+                    st[e / 16][e % 16] = (mine >> e & 1) != 0 || (int)key >= last ? -__builtin_inff() : st[e / 16][e % 16];
                 }
             }
 #pragma unroll

@@ -47,6 +47,13 @@ template <typename S> struct Args {
     Counts count;
 };
 
+// A block's Meta through the scalar cache (no kernel writes it while one that
+// reads it runs): a vector load would wait in line with the codes asked for ahead.
+__device__ inline Meta scalar_meta(const Meta *at) {
+    typedef const __attribute__((address_space(4))) u32x4 Constant;
+    return __builtin_bit_cast(Meta, *(Constant *)(uintptr_t)at);
+}
+
 // Eight codes (as bytes + 128) as f16, exact.
 __device__ inline half8 codes(uint32_t a, uint32_t b) {
     const uint32_t one = 0x64646464u;
