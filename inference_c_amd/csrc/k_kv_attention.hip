@@ -144,15 +144,18 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(Args<S> a) {
     f32x4 o[NV];
 #pragma unroll
     for (uint32_t j = 0; j < NV; ++j) o[j] = f32x4{0, 0, 0, 0};
-    float big = neg_inf, sum = 0.0f, unit = 1.0f;
+    float big = neg_inf, sum = 0.0f, unit = 1.0f, inverse_unit = 1.0f;
 
     // one block: kf(u, s) and vf(j, s) give the A operands
     auto step = [&](uint32_t t, Meta meta, auto kf, auto vf, auto keys_done) {
-        const double factor2 = (double)meta.k_scale * a.scale2;
-        const float factor = (float)factor2 * q.factor;
         // f32: what rounding takes off the factor and the scores is added back in
         // the exponent (scores of 10 would be off by 1e-6 of their weight)
-        const float factor_rest = (float)(factor2 - (double)(float)factor2) * q.factor;
+        float factor = meta.k_scale * (float)a.scale2, factor_rest = 0.0f;
+        if constexpr (kPair) {
+            const double exact = (double)meta.k_scale * a.scale2;
+            factor = (float)exact * q.factor;
+            factor_rest = (float)(exact - (double)(float)exact) * q.factor;
+        }
         float p[16], rest[kPair ? 16 : 1];
 #pragma unroll
         for (uint32_t u = 0; u < 4; ++u) {
@@ -200,13 +203,14 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(Args<S> a) {
         }
         // nothing seen yet: every score is -inf (p = 0) or NaN
         const float base = big == neg_inf ? 0.0f : big - kHeadroom<S>;
-        float ratio = meta.v_scale / unit;
+        float ratio = meta.v_scale * inverse_unit;
         if (meta.v_scale == 0.0f) {
             ratio = 1.0f;   // its codes are zeros
         } else if (ratio > kUnitRange || ratio < 1.0f / kUnitRange) {
 #pragma unroll
             for (uint32_t j = 0; j < NV; ++j) o[j] *= unit / meta.v_scale;
             unit = meta.v_scale;
+            inverse_unit = 1.0f / unit;
             ratio = 1.0f;
         }
         half8 ph[2], pl[kPair ? 2 : 1];
@@ -225,7 +229,7 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(Args<S> a) {
                 add += (float)ph[e / 8][e % 8];   // the sum of P as the product has it
             }
         }
-        sum += kPair ? add : add * (1.0f / ratio);
+        sum += kPair ? add : add * fast_rcp(ratio);
 #pragma unroll
         for (uint32_t j = 0; j < NV; ++j) {
             if (j * 16 >= c.vp) continue;
@@ -272,7 +276,7 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(Args<S> a) {
     }
     for (; t < end_whole; t += kWaves) {
         const uint32_t next = t + kWaves;
-        const Meta next_meta = scalar_meta(meta + min(next, c.blocks - 1));   // (asked for a block ahead, as the codes are)
+        Meta next_meta;
         step(
             t, now_meta,
             [&](uint32_t u, uint32_t s) {
@@ -281,6 +285,9 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(Args<S> a) {
             },
             [&](uint32_t j, uint32_t s) { return codes(vr[j][2 * s], vr[j][2 * s + 1]); },
             [&] {
+                // (asked for a block ahead as the codes are, but where this block's is in:
+                // a wait for one scalar load waits for all)
+                next_meta = scalar_meta(meta + min(next, c.blocks - 1));
                 if (next < end_whole) load_k(next);
             });
         if (next < end_whole) load_v(next);

@@ -85,12 +85,19 @@ template <typename S, uint32_t P> struct TileQuery {
     }
 };
 
-// A block's factor of raw products, positive (queries carry the scale's sign), and
-// what rounding took off it. A block of zero keys has raw products 0: any factor.
-__device__ inline f32x2 block_factor(float k_scale, double scale2) {
-    const double f = (k_scale == 0.0f ? 1.0 : (double)k_scale) * (scale2 == 0.0 ? 1.0 : fabs(scale2));
-    const float hi = fminf(fmaxf((float)f, kTiny), kHuge);
-    return f32x2{hi, (float)(f - (double)hi)};
+// A block's factor of raw products, positive (queries carry the scale's sign), and,
+// for f32, what rounding took off it. A block of zero keys has raw products 0: any
+// factor.
+template <typename S> __device__ inline f32x2 block_factor(float k_scale, double scale2) {
+    const float k = k_scale == 0.0f ? 1.0f : k_scale;
+    const double scale = scale2 == 0.0 ? 1.0 : fabs(scale2);
+    if constexpr (sizeof(S) == 2) {
+        return f32x2{fminf(fmaxf(k * (float)scale, kTiny), kHuge), 0.0f};
+    } else {
+        const double f = (double)k * scale;
+        const float hi = fminf(fmaxf((float)f, kTiny), kHuge);
+        return f32x2{hi, (float)(f - (double)hi)};
+    }
 }
 
 // Key row of the block that A row m of a half reads.
@@ -183,8 +190,20 @@ __global__ __launch_bounds__(kThreads, sizeof(S) == 2 && P <= 128 ? 2 : 1) void 
     const Meta *const meta = c.meta + head * c.blocks;
     const uint8_t *const kcodes = c.k + head * c.blocks * kTokens * c.kp;
     const uint8_t *const vcodes = c.v + head * c.blocks * kTokens * c.vp;
-    auto meta_of = [&](uint32_t s) {
-        Meta m = scalar_meta(meta + block_of(s));
+    // A tile's Meta comes by a vector load ahead of the codes of the turn before,
+    // and is there when they are: a scalar load, which may return before or after any
+    // LDS read, would have to be waited for by the next of those.
+    uint32_t zero = 0;
+    asm volatile("" : "+v"(zero));   // (a lane's address: no scalar load)
+    u32x4 meta_ahead;
+    auto fetch_meta = [&](uint32_t s) {
+        meta_ahead = *reinterpret_cast<const u32x4 *>(reinterpret_cast<const char *>(meta + block_of(s)) + zero);
+    };
+    auto take_meta = [&](uint32_t s) {
+        u32x4 w;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = (uint32_t)__builtin_amdgcn_readfirstlane((int)meta_ahead[i]);
+        Meta m = __builtin_bit_cast(Meta, w);
         if (open_first && s == 0) m.k_scale = m.v_scale = 1.0f;
         return m;
     };
@@ -274,6 +293,7 @@ __global__ __launch_bounds__(kThreads, sizeof(S) == 2 && P <= 128 ? 2 : 1) void 
         *reinterpret_cast<half8 *>(&ks[1][t * KROW + d]) = half8{};
     }
     for (uint32_t p = tid; p < VTILE / 8; p += kThreads) reinterpret_cast<half8 *>(vs[1])[p] = half8{};
+    fetch_meta(0);
     fetch_k(0);
     fetch_v(0);
     if (tiles != 0) {
@@ -290,8 +310,9 @@ __global__ __launch_bounds__(kThreads, sizeof(S) == 2 && P <= 128 ? 2 : 1) void 
     }
     fetch_k(1);
     stash_k(1);
+    Meta next_meta = take_meta(0);
+    fetch_meta(1);
     fetch_k(2);
-    Meta next_meta = meta_of(0);
     float inverse_unit = 1.0f;
     __syncthreads();
     clear(st);
@@ -299,7 +320,6 @@ __global__ __launch_bounds__(kThreads, sizeof(S) == 2 && P <= 128 ? 2 : 1) void 
     auto turn = [&](uint32_t s, float16v (&now)[2], float16v (&ahead)[2]) {
         const Meta m = next_meta;
         const uint32_t t = block_of(s);
-        next_meta = meta_of(s + 1);
         __syncthreads();
         if ((int)(t * kTokens + kTokens) > least || m.marked != 0) {
             const int last = seen - (int)(t * kTokens);
@@ -311,7 +331,7 @@ __global__ __launch_bounds__(kThreads, sizeof(S) == 2 && P <= 128 ? 2 : 1) void 
                 now[e / 16][e % 16] = (int)key >= last ? neg_inf : x;
             }
         }
-        const f32x2 f2 = block_factor(m.k_scale, a.scale2);
+        const f32x2 f2 = block_factor<S>(m.k_scale, a.scale2);
         const float factor = f2.x * q.factor;
         float part_max[4] = {neg_inf, neg_inf, neg_inf, neg_inf};
         steps<NO>([&](uint32_t i) { return value_operand((s + 1) & 1, i); }, [&](uint32_t i, half8 v) { output(i, v); },
@@ -323,6 +343,8 @@ __global__ __launch_bounds__(kThreads, sizeof(S) == 2 && P <= 128 ? 2 : 1) void 
                           part_max[e % 4] = fmaxf(part_max[e % 4], now[e / 16][e % 16]);
                   });
         const float raw = fmaxf(fmaxf(part_max[0], part_max[1]), fmaxf(part_max[2], part_max[3]));
+        next_meta = take_meta(s + 1);
+        fetch_meta(s + 2);
         fetch_v(s + 1);
         fetch_k(s + 3);
         const float top = raw * factor;
@@ -453,7 +475,7 @@ __global__ __launch_bounds__(kThreads, P <= 64 ? 3 : P <= 128 ? 2 : 1) void kv_w
             }
         }
     const float sign = a.scale2 > 0.0 ? 1.0f : a.scale2 < 0.0 ? -1.0f : 0.0f;
-    const float k_factor = block_factor(open ? 1.0f : meta.k_scale, a.scale2).x;
+    const float k_factor = block_factor<S>(open ? 1.0f : meta.k_scale, a.scale2).x;
     float acc[32];
 #pragma unroll
     for (int e = 0; e < 32; ++e) acc[e] = 0.0f;
