@@ -100,10 +100,14 @@ template <typename S, uint32_t P> struct Query {
     }
 };
 
+template <bool kStream, typename V> __device__ inline V load_codes(const V *p) {
+    return kStream ? __builtin_nontemporal_load(p) : *p;
+}
+
 // One workgroup: 16 packed rows of one (sequence, kv head) and one part of its
 // blocks; wave w takes blocks w, w + 4, ... of the part and the waves' results
 // meet in LDS.
-template <typename S, uint32_t P>
+template <typename S, uint32_t P, bool kStream>
 __global__ __launch_bounds__(kThreads) void kv_rows_kernel(Args<S> a) {
     constexpr bool kPair = sizeof(S) == 4;
     constexpr uint32_t NC = P / 64, NV = P / 16;
@@ -113,30 +117,61 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(Args<S> a) {
     const View &c = a.c;
     const uint32_t lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const uint32_t part = blockIdx.x % a.parts, pr = blockIdx.x / a.parts;
-    const uint32_t pair = pr % a.pairs, row0 = (a.row_group0 + pr / a.pairs) * kRows;
-    const uint32_t b = pair / c.heads, h = pair % c.heads, seq = a.first + b;
-    const size_t head = (size_t)seq * c.heads + h;
+    const uint32_t h = blockIdx.y, b = blockIdx.z, seq = a.first + b;
     const uint32_t length = c.length[seq], count = a.count.n[b];
+    const uint32_t part = blockIdx.x % a.parts, row0 = (a.row_group0 + blockIdx.x / a.parts) * kRows;
+    const size_t head = (size_t)seq * c.heads + h;
     const uint32_t in_head = a.group * a.n;
-    const uint32_t r = row0 + m, i = r % a.n;
-    const bool live = r < in_head && i < count;
-    if (!wave_any(live)) return;
-    const size_t row = head * in_head + (r < in_head ? r : in_head - 1);   // (rows past the head repeat its last)
-    const int seen = seen_by(i, live, length, count, a.causal);
-    int most = live ? seen : 0, least = live ? seen : (int)length;
-#pragma unroll
-    for (int d = 1; d < 16; d *= 2) {
-        most = max(most, __shfl_xor(most, d, kWave));
-        least = min(least, __shfl_xor(least, d, kWave));
-    }
-    most = __builtin_amdgcn_readfirstlane(most);
-    least = __builtin_amdgcn_readfirstlane(least);
+    // what the rows see, from the first one's place among its query head's n (the
+    // first loads wait for this: no lane's arithmetic, only scalars)
+    const uint32_t i0 = a.n == 1 ? 0 : row0 % a.n;
+    const bool another = row0 + (a.n - i0) < in_head && i0 + kRows > a.n;   // rows of a next query head too
+    if (count == 0 || (i0 >= count && !another)) return;
+    const uint32_t last = i0 + kRows >= a.n ? a.n - 1 : i0 + kRows - 1;
+    const int before = (int)length - (int)count;
+    const int most = a.causal ? before + (int)min(last, count - 1) + 1 : (int)length;
+    const int least = a.causal ? before + (int)(another ? 0 : i0) + 1 : (int)length;
     const uint32_t blocks = ((uint32_t)max(most, 0) + kTokens - 1) / kTokens;
     const uint32_t whole = length / kTokens;   // blocks held as codes
     const uint32_t share = ((blocks + a.parts - 1) / a.parts + kWaves - 1) / kWaves * kWaves;
     const uint32_t begin = min(part * share, blocks), end = min(begin + share, blocks);
+    const uint32_t end_whole = min(end, whole);
+    uint32_t t = begin + wave;
 
+    const Meta *const meta = c.meta + head * c.blocks;
+    const uint32_t key_of = (m / 4) * 16 + m % 4;   // + 4 u: the lane's key row
+    u32x4 kr[4][NC > 0 ? NC : 1], vr[NV];
+    u32x2 ko[4];
+    auto load_k = [&](uint32_t t) {
+        const uint8_t *base = c.k + ((head * c.blocks + t) * kTokens + key_of) * c.kp;
+#pragma unroll
+        for (uint32_t u = 0; u < 4; ++u) {
+#pragma unroll
+            for (uint32_t ch = 0; ch < NC; ++ch) {
+                const uint32_t d = ch * 64 + g * 16;   // past the row: its start, against zeros of q
+                kr[u][ch] = load_codes<kStream>(reinterpret_cast<const u32x4 *>(base + 4 * u * c.kp + (d < c.kp ? d : 0)));
+            }
+            if constexpr (kOdd) {
+                const uint32_t d = NC * 64 + g * 8;
+                ko[u] = load_codes<kStream>(reinterpret_cast<const u32x2 *>(base + 4 * u * c.kp + (d < c.kp ? d : 0)));
+            }
+        }
+    };
+    auto load_v = [&](uint32_t t) {
+        const uint8_t *base = c.v + ((head * c.blocks + t) * c.vp + m) * kTokens + g * 16;
+#pragma unroll
+        for (uint32_t j = 0; j < NV; ++j)
+            if (j * 16 < c.vp) vr[j] = load_codes<kStream>(reinterpret_cast<const u32x4 *>(base + j * 16 * kTokens));
+    };
+    Meta now_meta = scalar_meta(meta + min(t, c.blocks - 1));
+    if (t < end_whole) {
+        load_k(t);
+        load_v(t);
+    }
+    const uint32_t r = row0 + m, i = a.n == 1 ? 0 : r % a.n;
+    const bool live = r < in_head && i < count;
+    const size_t row = head * in_head + (r < in_head ? r : in_head - 1);   // (rows past the head repeat its last)
+    const int seen = seen_by(i, live, length, count, a.causal);
     Query<S, P> q;
     q.load(a.q + row * c.dim, c.dim, g);
 
@@ -242,38 +277,6 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(Args<S> a) {
         }
     };
 
-    const Meta *const meta = c.meta + head * c.blocks;
-    const uint32_t key_of = (m / 4) * 16 + m % 4;   // + 4 u: the lane's key row
-    u32x4 kr[4][NC > 0 ? NC : 1], vr[NV];
-    u32x2 ko[4];
-    auto load_k = [&](uint32_t t) {
-        const uint8_t *base = c.k + ((head * c.blocks + t) * kTokens + key_of) * c.kp;
-#pragma unroll
-        for (uint32_t u = 0; u < 4; ++u) {
-#pragma unroll
-            for (uint32_t ch = 0; ch < NC; ++ch) {
-                const uint32_t d = ch * 64 + g * 16;   // past the row: its start, against zeros of q
-                kr[u][ch] = *reinterpret_cast<const u32x4 *>(base + 4 * u * c.kp + (d < c.kp ? d : 0));
-            }
-            if constexpr (kOdd) {
-                const uint32_t d = NC * 64 + g * 8;
-                ko[u] = *reinterpret_cast<const u32x2 *>(base + 4 * u * c.kp + (d < c.kp ? d : 0));
-            }
-        }
-    };
-    auto load_v = [&](uint32_t t) {
-        const uint8_t *base = c.v + ((head * c.blocks + t) * c.vp + m) * kTokens + g * 16;
-#pragma unroll
-        for (uint32_t j = 0; j < NV; ++j)
-            if (j * 16 < c.vp) vr[j] = *reinterpret_cast<const u32x4 *>(base + j * 16 * kTokens);
-    };
-    const uint32_t end_whole = min(end, whole);
-    uint32_t t = begin + wave;
-    Meta now_meta = scalar_meta(meta + min(t, c.blocks - 1));
-    if (t < end_whole) {
-        load_k(t);
-        load_v(t);
-    }
     for (; t < end_whole; t += kWaves) {
         const uint32_t next = t + kWaves;
         Meta next_meta;
@@ -360,12 +363,14 @@ __device__ inline f32x2 fold_ml(const f32x2 *ml, uint32_t parts, size_t rows, ui
     return f32x2{top, wave_sum(total)};
 }
 
-// Merges the parts of a row, one workgroup per row: its waves take every fourth
-// part, a lane four output elements. The workgroups after `folds` do 256 tokens
-// of one (sequence, head) each: their weights from the stored scores.
-template <typename S>
-__global__ __launch_bounds__(kThreads) void kv_fold_kernel(Args<S> a, uint32_t folds, uint32_t token_groups) {
-    __shared__ f32x4 lds_o[kWaves][kWave];
+// Merges the parts of a row, one workgroup per row: its waves take the parts in
+// turn, a lane four output elements. The workgroups after `folds` do a token per
+// thread of one (sequence, head): their weights from the stored scores. Bound by
+// its chain of memory latencies: 16 waves from 16 parts on.
+template <typename S, uint32_t kFoldWaves>
+__global__ __launch_bounds__(kFoldWaves *kWave) void kv_fold_kernel(Args<S> a, uint32_t folds, uint32_t token_groups) {
+    constexpr uint32_t kFoldThreads = kFoldWaves * kWave;
+    __shared__ f32x4 lds_o[kFoldWaves][kWave];
     __shared__ f32x2 lds_ml[kRows];
     const View &c = a.c;
     const uint32_t lane = threadIdx.x & 63, wave = (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -374,15 +379,15 @@ __global__ __launch_bounds__(kThreads) void kv_fold_kernel(Args<S> a, uint32_t f
         const uint32_t tg = (blockIdx.x - folds) % token_groups, pair = (blockIdx.x - folds) / token_groups;
         const uint32_t b = pair / c.heads, seq = a.first + b, length = min(c.length[seq], a.weight_tokens);
         const size_t head = (size_t)seq * c.heads + pair % c.heads;
-        if (tg * kThreads >= length) return;
-        for (uint32_t r = wave; r < in_head; r += kWaves) {
+        if (tg * kFoldThreads >= length) return;
+        for (uint32_t r = wave; r < in_head; r += kFoldWaves) {
             const size_t row = head * in_head + r;
             const f32x2 ml = r % a.n < a.count.n[b] ? fold_ml(a.part_ml + row, a.parts, a.rows, lane)
                                                     : f32x2{-__builtin_inff(), 0.0f};
             if (lane == 0) lds_ml[r] = weight_terms(ml.x, ml.y);
         }
         __syncthreads();
-        const uint32_t t = tg * kThreads + threadIdx.x;
+        const uint32_t t = tg * kFoldThreads + threadIdx.x;
         if (t >= length) return;
         float total = 0.0f;
         for (uint32_t r = 0; r < in_head; ++r) {
@@ -401,7 +406,7 @@ __global__ __launch_bounds__(kThreads) void kv_fold_kernel(Args<S> a, uint32_t f
     const uint32_t d = 4 * lane;
     const bool fours = c.vdim % 4 == 0;
 #pragma unroll 4
-    for (uint32_t s = wave; s < a.parts; s += kWaves) {
+    for (uint32_t s = wave; s < a.parts; s += kFoldWaves) {
         const float m = a.part_ml[(size_t)s * a.rows + row].x;
         const float w = all.x == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - all.x);
         const float *src = a.part_o + ((size_t)s * a.rows + row) * c.vdim;
@@ -416,7 +421,7 @@ __global__ __launch_bounds__(kThreads) void kv_fold_kernel(Args<S> a, uint32_t f
     lds_o[wave][lane] = v;
     __syncthreads();
     if (wave != 0) return;
-    for (uint32_t k = 1; k < kWaves; ++k) v += lds_o[k][lane];
+    for (uint32_t k = 1; k < kFoldWaves; ++k) v += lds_o[k][lane];
     store_out(a.out + row * c.vdim, c.vdim, d, finish(v, all.x, all.y));
     if (a.row_ml != nullptr && lane == 0) a.row_ml[row] = weight_terms(all.x, all.y);
 }
@@ -474,9 +479,17 @@ Plan plan_of(bool f32, const View &c, const AttentionShape &a) {
     return p;
 }
 
+// Codes past what the 256 MB cache behind the L2s holds to the next call are read
+// as a stream. One sequence of 131000 tokens (268 MB): 62.5 -> 56.6 us; 8 x 4096
+// (67 MB, found there by calls in a row): 19.5, as a stream 20.6.
+constexpr size_t kStreamBytes = size_t{192} << 20;
+
 template <typename S, uint32_t P>
 hipError_t launch_rows(const Args<S> &a, uint32_t groups, hipStream_t s) {
-    kv_rows_kernel<S, P><<<groups * a.pairs * a.parts, kThreads, 0, s>>>(a);
+    const dim3 grid(groups * a.parts, a.c.heads, a.pairs / a.c.heads);
+    const size_t bytes = (size_t)a.pairs * a.longest * (a.c.kp + a.c.vp);
+    if (bytes > kStreamBytes) kv_rows_kernel<S, P, true><<<grid, kThreads, 0, s>>>(a);
+    else kv_rows_kernel<S, P, false><<<grid, kThreads, 0, s>>>(a);
     return hipGetLastError();
 }
 template <typename S>
@@ -503,9 +516,12 @@ hipError_t launch(Args<S> a, const Plan &p, uint32_t batch, uint32_t longest, fl
     if (p.parts > 1 || p.scores) {
         // (at most 512 row groups where there are parts)
         const uint32_t folds = p.parts > 1 ? a.pairs * a.group * a.n : 0;
-        const uint32_t token_groups = p.scores ? (blocks * kTokens + kThreads - 1) / kThreads : 0;
-        if (folds + a.pairs * token_groups == 0) return hipSuccess;
-        kv_fold_kernel<S><<<folds + a.pairs * token_groups, kThreads, 0, s>>>(a, folds, token_groups);
+        const uint32_t threads = p.parts >= 16 ? 16 * kWave : kThreads;
+        const uint32_t token_groups = p.scores ? (blocks * kTokens + threads - 1) / threads : 0;
+        const uint32_t grid = folds + a.pairs * token_groups;
+        if (grid == 0) return hipSuccess;
+        if (threads == kThreads) kv_fold_kernel<S, kWaves><<<grid, threads, 0, s>>>(a, folds, token_groups);
+        else kv_fold_kernel<S, 16><<<grid, threads, 0, s>>>(a, folds, token_groups);
         const hipError_t status = hipGetLastError();
         if (status != hipSuccess) return status;
     }
@@ -540,6 +556,7 @@ hipError_t run(const View &c, const AttentionShape &sh, const void *query, void 
     a.group = sh.q_heads / c.heads;
     a.n = sh.n;
     a.parts = p.parts;
+    a.longest = sh.longest;
     a.scale2 = (double)sh.scale * kLog2e;
     a.causal = sh.causal;
     for (uint32_t first = 0; first < sh.batch; first += kBatchPerLaunch) {
