@@ -363,13 +363,13 @@ __device__ inline f32x2 fold_ml(const f32x2 *ml, uint32_t parts, size_t rows, ui
     return f32x2{top, wave_sum(total)};
 }
 
-// Merges the parts of a row, one workgroup per row: its waves take the parts in
+// Merges the parts of rows, kRowWaves waves for each: the waves take the parts in
 // turn, a lane four output elements. The workgroups after `folds` do a token per
 // thread of one (sequence, head): their weights from the stored scores. Bound by
-// its chain of memory latencies: 16 waves from 16 parts on.
-template <typename S, uint32_t kFoldWaves>
+// its chain of memory latencies: up to 4 parts one wave per row, up to 16 four.
+template <typename S, uint32_t kFoldWaves, uint32_t kRowWaves>
 __global__ __launch_bounds__(kFoldWaves *kWave) void kv_fold_kernel(Args<S> a, uint32_t folds, uint32_t token_groups) {
-    constexpr uint32_t kFoldThreads = kFoldWaves * kWave;
+    constexpr uint32_t kFoldThreads = kFoldWaves * kWave, kHeld = 4;
     __shared__ f32x4 lds_o[kFoldWaves][kWave];
     __shared__ f32x2 lds_ml[kRows];
     const View &c = a.c;
@@ -398,30 +398,46 @@ __global__ __launch_bounds__(kFoldWaves *kWave) void kv_fold_kernel(Args<S> a, u
         a.weights[head * a.weight_stride + t] += total;
         return;
     }
-    const uint32_t b = blockIdx.x / (in_head * c.heads);
-    if (blockIdx.x % a.n >= a.count.n[b]) return;
-    const size_t row = (size_t)a.first * c.heads * in_head + blockIdx.x;
-    const f32x2 all = fold_ml(a.part_ml + row, a.parts, a.rows, lane);
-    f32x4 v = {0, 0, 0, 0};
-    const uint32_t d = 4 * lane;
-    const bool fours = c.vdim % 4 == 0;
-#pragma unroll 4
-    for (uint32_t s = wave; s < a.parts; s += kFoldWaves) {
-        const float m = a.part_ml[(size_t)s * a.rows + row].x;
-        const float w = all.x == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - all.x);
-        const float *src = a.part_o + ((size_t)s * a.rows + row) * c.vdim;
-        if (fours) {
-            v += *reinterpret_cast<const f32x4 *>(src + (d < c.vdim ? d : 0)) * w;
+    const uint32_t of_pairs = blockIdx.x * (kFoldWaves / kRowWaves) + wave / kRowWaves, first = wave % kRowWaves;
+    const uint32_t b = of_pairs / (in_head * c.heads);
+    // (a row past the end or of padding: with one row per workgroup all its waves)
+    if (of_pairs >= a.pairs * in_head || of_pairs % a.n >= a.count.n[b]) return;
+    const size_t row = (size_t)a.first * c.heads * in_head + of_pairs;
+    // four of the wave's parts are asked for along with all parts' maxima (a part
+    // past the last one again, left out of the sums)
+    f32x4 v = {0, 0, 0, 0}, held[kHeld];
+    float held_m[kHeld];
+    const uint32_t d = 4 * lane, last = a.parts - 1;
+    auto load = [&](uint32_t s) {
+        const float *src = a.part_o + ((size_t)min(s, last) * a.rows + row) * c.vdim;
+        f32x4 x;
+        if (c.vdim % 4 == 0) {
+            x = *reinterpret_cast<const f32x4 *>(src + (d < c.vdim ? d : 0));
         } else {
 #pragma unroll
-            for (uint32_t e = 0; e < 4; ++e)
-                if (d + e < c.vdim) v[e] += src[d + e] * w;
+            for (uint32_t e = 0; e < 4; ++e) x[e] = src[d + e < c.vdim ? d + e : 0];
         }
+        return x;
+    };
+#pragma unroll
+    for (uint32_t k = 0; k < kHeld; ++k) {
+        held[k] = load(first + k * kRowWaves);
+        held_m[k] = a.part_ml[(size_t)min(first + k * kRowWaves, last) * a.rows + row].x;
     }
-    lds_o[wave][lane] = v;
-    __syncthreads();
-    if (wave != 0) return;
-    for (uint32_t k = 1; k < kFoldWaves; ++k) v += lds_o[k][lane];
+    const f32x2 all = fold_ml(a.part_ml + row, a.parts, a.rows, lane);
+    auto weight = [&](float m) { return all.x == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - all.x); };
+#pragma unroll
+    for (uint32_t k = 0; k < kHeld; ++k)
+        if (first + k * kRowWaves < a.parts) v += held[k] * weight(held_m[k]);
+#pragma unroll 4
+    for (uint32_t s = first + kHeld * kRowWaves; s < a.parts; s += kRowWaves)
+        v += load(s) * weight(a.part_ml[(size_t)s * a.rows + row].x);
+    if constexpr (kRowWaves > 1) {
+        lds_o[wave][lane] = v;
+        __syncthreads();
+        if (first != 0) return;
+        for (uint32_t k = 1; k < kRowWaves; ++k) v += lds_o[k][lane];
+    }
     store_out(a.out + row * c.vdim, c.vdim, d, finish(v, all.x, all.y));
     if (a.row_ml != nullptr && lane == 0) a.row_ml[row] = weight_terms(all.x, all.y);
 }
@@ -516,12 +532,14 @@ hipError_t launch(Args<S> a, const Plan &p, uint32_t batch, uint32_t longest, fl
     if (p.parts > 1 || p.scores) {
         // (at most 512 row groups where there are parts)
         const uint32_t folds = p.parts > 1 ? a.pairs * a.group * a.n : 0;
-        const uint32_t threads = p.parts >= 16 ? 16 * kWave : kThreads;
+        const uint32_t threads = p.parts > 16 ? 16 * kWave : kThreads;
         const uint32_t token_groups = p.scores ? (blocks * kTokens + threads - 1) / threads : 0;
-        const uint32_t grid = folds + a.pairs * token_groups;
+        const uint32_t workgroups = p.parts <= kWaves ? (folds + kWaves - 1) / kWaves : folds;
+        const uint32_t grid = workgroups + a.pairs * token_groups;
         if (grid == 0) return hipSuccess;
-        if (threads == kThreads) kv_fold_kernel<S, kWaves><<<grid, threads, 0, s>>>(a, folds, token_groups);
-        else kv_fold_kernel<S, 16><<<grid, threads, 0, s>>>(a, folds, token_groups);
+        if (p.parts <= kWaves) kv_fold_kernel<S, kWaves, 1><<<grid, threads, 0, s>>>(a, workgroups, token_groups);
+        else if (threads == kThreads) kv_fold_kernel<S, kWaves, kWaves><<<grid, threads, 0, s>>>(a, workgroups, token_groups);
+        else kv_fold_kernel<S, 16, 16><<<grid, threads, 0, s>>>(a, workgroups, token_groups);
         const hipError_t status = hipGetLastError();
         if (status != hipSuccess) return status;
     }
