@@ -107,8 +107,15 @@ template <bool kStream, typename V> __device__ inline V load_codes(const V *p) {
 // One workgroup: 16 packed rows of one (sequence, kv head) and one part of its
 // blocks; wave w takes blocks w, w + 4, ... of the part and the waves' results
 // meet in LDS.
+// What the first loads wait for comes as leading arguments, which are in scalar
+// registers when a wave starts: the struct behind them takes a microsecond to
+// arrive. (8 x 4096 tokens, from the wave's start to its first loads' issue: 2 us
+// out of 12 with the struct alone.)
 template <typename S, uint32_t P, bool kStream>
-__global__ __launch_bounds__(kThreads) void kv_rows_kernel(Args<S> a) {
+__global__ __launch_bounds__(kThreads) void kv_rows_kernel(const uint8_t *keys, const uint8_t *values,
+                                                           const uint32_t *lengths, const Meta *metas, const S *queries,
+                                                           uint32_t all_blocks, uint32_t heads, uint32_t parts_first,
+                                                           uint32_t pitches, uint32_t n, uint32_t group, Args<S> a) {
     constexpr bool kPair = sizeof(S) == 4;
     constexpr uint32_t NC = P / 64, NV = P / 16;
     constexpr bool kOdd = P % 64 != 0;
@@ -117,63 +124,65 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(Args<S> a) {
     const View &c = a.c;
     const uint32_t lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const uint32_t h = blockIdx.y, b = blockIdx.z, seq = a.first + b;
-    const uint32_t length = c.length[seq], count = a.count.n[b];
-    const uint32_t part = blockIdx.x % a.parts, row0 = (a.row_group0 + blockIdx.x / a.parts) * kRows;
-    const size_t head = (size_t)seq * c.heads + h;
-    const uint32_t in_head = a.group * a.n;
-    // what the rows see, from the first one's place among its query head's n (the
-    // first loads wait for this: no lane's arithmetic, only scalars)
-    const uint32_t i0 = a.n == 1 ? 0 : row0 % a.n;
-    const bool another = row0 + (a.n - i0) < in_head && i0 + kRows > a.n;   // rows of a next query head too
-    if (count == 0 || (i0 >= count && !another)) return;
-    const uint32_t last = i0 + kRows >= a.n ? a.n - 1 : i0 + kRows - 1;
-    const int before = (int)length - (int)count;
-    const int most = a.causal ? before + (int)min(last, count - 1) + 1 : (int)length;
-    const int least = a.causal ? before + (int)(another ? 0 : i0) + 1 : (int)length;
-    const uint32_t blocks = ((uint32_t)max(most, 0) + kTokens - 1) / kTokens;
-    const uint32_t whole = length / kTokens;   // blocks held as codes
-    const uint32_t share = ((blocks + a.parts - 1) / a.parts + kWaves - 1) / kWaves * kWaves;
-    const uint32_t begin = min(part * share, blocks), end = min(begin + share, blocks);
-    const uint32_t end_whole = min(end, whole);
+    const uint32_t parts = parts_first & 0xffffu, kp = pitches & 0xffffu, vp = pitches >> 16;
+    const uint32_t h = blockIdx.y, b = blockIdx.z, seq = (parts_first >> 16) + b;
+    const uint32_t length = lengths[seq];
+    const uint32_t part = blockIdx.x % parts;
+    const size_t head = (size_t)seq * heads + h;
+    // the part's blocks, the open one (the last, in f16) among them
+    const uint32_t whole = length / kTokens, held = (length + kTokens - 1) / kTokens;
+    const uint32_t share = ((held + parts - 1) / parts + kWaves - 1) / kWaves * kWaves;
+    const uint32_t begin = min(part * share, held);
     uint32_t t = begin + wave;
 
-    const Meta *const meta = c.meta + head * c.blocks;
+    const Meta *const meta = metas + head * all_blocks;
     const uint32_t key_of = (m / 4) * 16 + m % 4;   // + 4 u: the lane's key row
     u32x4 kr[4][NC > 0 ? NC : 1], vr[NV];
     u32x2 ko[4];
     auto load_k = [&](uint32_t t) {
-        const uint8_t *base = c.k + ((head * c.blocks + t) * kTokens + key_of) * c.kp;
+        const uint8_t *base = keys + ((head * all_blocks + t) * kTokens + key_of) * kp;
 #pragma unroll
         for (uint32_t u = 0; u < 4; ++u) {
 #pragma unroll
             for (uint32_t ch = 0; ch < NC; ++ch) {
                 const uint32_t d = ch * 64 + g * 16;   // past the row: its start, against zeros of q
-                kr[u][ch] = load_codes<kStream>(reinterpret_cast<const u32x4 *>(base + 4 * u * c.kp + (d < c.kp ? d : 0)));
+                kr[u][ch] = load_codes<kStream>(reinterpret_cast<const u32x4 *>(base + 4 * u * kp + (d < kp ? d : 0)));
             }
             if constexpr (kOdd) {
                 const uint32_t d = NC * 64 + g * 8;
-                ko[u] = load_codes<kStream>(reinterpret_cast<const u32x2 *>(base + 4 * u * c.kp + (d < c.kp ? d : 0)));
+                ko[u] = load_codes<kStream>(reinterpret_cast<const u32x2 *>(base + 4 * u * kp + (d < kp ? d : 0)));
             }
         }
     };
     auto load_v = [&](uint32_t t) {
-        const uint8_t *base = c.v + ((head * c.blocks + t) * c.vp + m) * kTokens + g * 16;
+        const uint8_t *base = values + ((head * all_blocks + t) * vp + m) * kTokens + g * 16;
 #pragma unroll
         for (uint32_t j = 0; j < NV; ++j)
-            if (j * 16 < c.vp) vr[j] = load_codes<kStream>(reinterpret_cast<const u32x4 *>(base + j * 16 * kTokens));
+            if (j * 16 < vp) vr[j] = load_codes<kStream>(reinterpret_cast<const u32x4 *>(base + j * 16 * kTokens));
     };
-    Meta now_meta = scalar_meta(meta + min(t, c.blocks - 1));
-    if (t < end_whole) {
+    Meta now_meta = scalar_meta(meta + min(t, all_blocks - 1));
+    // (a part of rows that see less than it holds asks for a block it does not use)
+    if (t < min(begin + share, whole)) {
         load_k(t);
         load_v(t);
     }
-    const uint32_t r = row0 + m, i = a.n == 1 ? 0 : r % a.n;
+    const uint32_t in_head = group * n, row0 = (a.row_group0 + blockIdx.x / parts) * kRows, count = a.count.n[b];
+    // what the rows see, from the first one's place among its query head's n
+    const uint32_t i0 = n == 1 ? 0 : row0 % n;
+    const bool another = row0 + (n - i0) < in_head && i0 + kRows > n;   // rows of a next query head too
+    if (count == 0 || (i0 >= count && !another)) return;
+    const uint32_t last = i0 + kRows >= n ? n - 1 : i0 + kRows - 1;
+    const int before = (int)length - (int)count;
+    const int most = a.causal ? before + (int)min(last, count - 1) + 1 : (int)length;
+    const int least = a.causal ? before + (int)(another ? 0 : i0) + 1 : (int)length;
+    const uint32_t blocks = ((uint32_t)max(most, 0) + kTokens - 1) / kTokens;
+    const uint32_t end = min(begin + share, blocks), end_whole = min(end, whole);
+    const uint32_t r = row0 + m, i = n == 1 ? 0 : r % n;
     const bool live = r < in_head && i < count;
     const size_t row = head * in_head + (r < in_head ? r : in_head - 1);   // (rows past the head repeat its last)
     const int seen = seen_by(i, live, length, count, a.causal);
     Query<S, P> q;
-    q.load(a.q + row * c.dim, c.dim, g);
+    q.load(queries + row * c.dim, c.dim, g);
 
     const float neg_inf = -__builtin_inff();
     f32x4 o[NV];
@@ -267,7 +276,7 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(Args<S> a) {
         sum += kPair ? add : add * fast_rcp(ratio);
 #pragma unroll
         for (uint32_t j = 0; j < NV; ++j) {
-            if (j * 16 >= c.vp) continue;
+            if (j * 16 >= vp) continue;
 #pragma unroll
             for (uint32_t s = 0; s < 2; ++s) {
                 const half8 v = vf(j, s);
@@ -290,7 +299,7 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(Args<S> a) {
             [&] {
                 // (asked for a block ahead as the codes are, but where this block's is in:
                 // a wait for one scalar load waits for all)
-                next_meta = scalar_meta(meta + min(next, c.blocks - 1));
+                next_meta = scalar_meta(meta + min(next, all_blocks - 1));
                 if (next < end_whole) load_k(next);
             });
         if (next < end_whole) load_v(next);
@@ -325,7 +334,7 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(Args<S> a) {
         total += w[k] * lds_ml[k][m].y;
     }
     const bool writes = live && r < in_head;
-    if (a.parts == 1) {
+    if (parts == 1) {
         S *const out = a.out + row * c.vdim;
 #pragma unroll
         for (uint32_t j = wave; j < NV; j += kWaves) {
@@ -368,13 +377,15 @@ __device__ inline f32x2 fold_ml(const f32x2 *ml, uint32_t parts, size_t rows, ui
 // thread of one (sequence, head): their weights from the stored scores. Bound by
 // its chain of memory latencies: up to 4 parts one wave per row, up to 16 four.
 template <typename S, uint32_t kFoldWaves, uint32_t kRowWaves>
-__global__ __launch_bounds__(kFoldWaves *kWave) void kv_fold_kernel(Args<S> a, uint32_t folds, uint32_t token_groups) {
+__global__ __launch_bounds__(kFoldWaves *kWave) void kv_fold_kernel(const float *part_o, const f32x2 *part_ml, size_t rows,
+                                                                  uint32_t parts, uint32_t n, uint32_t in_head,
+                                                                  uint32_t vdim, uint32_t folds, uint32_t first_row,
+                                                                  uint32_t token_groups, uint32_t all_rows, Args<S> a) {
     constexpr uint32_t kFoldThreads = kFoldWaves * kWave, kHeld = 4;
     __shared__ f32x4 lds_o[kFoldWaves][kWave];
     __shared__ f32x2 lds_ml[kRows];
     const View &c = a.c;
     const uint32_t lane = threadIdx.x & 63, wave = (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const uint32_t in_head = a.group * a.n;
     if (blockIdx.x >= folds) {
         const uint32_t tg = (blockIdx.x - folds) % token_groups, pair = (blockIdx.x - folds) / token_groups;
         const uint32_t b = pair / c.heads, seq = a.first + b, length = min(c.length[seq], a.weight_tokens);
@@ -399,46 +410,48 @@ __global__ __launch_bounds__(kFoldWaves *kWave) void kv_fold_kernel(Args<S> a, u
         return;
     }
     const uint32_t of_pairs = blockIdx.x * (kFoldWaves / kRowWaves) + wave / kRowWaves, first = wave % kRowWaves;
-    const uint32_t b = of_pairs / (in_head * c.heads);
-    // (a row past the end or of padding: with one row per workgroup all its waves)
-    if (of_pairs >= a.pairs * in_head || of_pairs % a.n >= a.count.n[b]) return;
-    const size_t row = (size_t)a.first * c.heads * in_head + of_pairs;
+    if (of_pairs >= all_rows) return;   // (with one row per workgroup, none)
+    const size_t row = (size_t)first_row + of_pairs;
     // four of the wave's parts are asked for along with all parts' maxima (a part
     // past the last one again, left out of the sums)
     f32x4 v = {0, 0, 0, 0}, held[kHeld];
     float held_m[kHeld];
-    const uint32_t d = 4 * lane, last = a.parts - 1;
+    const uint32_t d = 4 * lane, last = parts - 1;
     auto load = [&](uint32_t s) {
-        const float *src = a.part_o + ((size_t)min(s, last) * a.rows + row) * c.vdim;
+        const float *src = part_o + ((size_t)min(s, last) * rows + row) * vdim;
         f32x4 x;
-        if (c.vdim % 4 == 0) {
-            x = *reinterpret_cast<const f32x4 *>(src + (d < c.vdim ? d : 0));
+        if (vdim % 4 == 0) {
+            x = *reinterpret_cast<const f32x4 *>(src + (d < vdim ? d : 0));
         } else {
 #pragma unroll
-            for (uint32_t e = 0; e < 4; ++e) x[e] = src[d + e < c.vdim ? d + e : 0];
+            for (uint32_t e = 0; e < 4; ++e) x[e] = src[d + e < vdim ? d + e : 0];
         }
         return x;
     };
 #pragma unroll
     for (uint32_t k = 0; k < kHeld; ++k) {
         held[k] = load(first + k * kRowWaves);
-        held_m[k] = a.part_ml[(size_t)min(first + k * kRowWaves, last) * a.rows + row].x;
+        held_m[k] = part_ml[(size_t)min(first + k * kRowWaves, last) * rows + row].x;
     }
-    const f32x2 all = fold_ml(a.part_ml + row, a.parts, a.rows, lane);
+    // a row of padding has no parts: what is there is read, and not used
+    const uint32_t b = of_pairs / (in_head * c.heads);
+    const bool there = of_pairs % n < a.count.n[b];
+    const f32x2 all = fold_ml(part_ml + row, parts, rows, lane);
     auto weight = [&](float m) { return all.x == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - all.x); };
 #pragma unroll
     for (uint32_t k = 0; k < kHeld; ++k)
-        if (first + k * kRowWaves < a.parts) v += held[k] * weight(held_m[k]);
+        if (first + k * kRowWaves < parts) v += held[k] * weight(held_m[k]);
 #pragma unroll 4
-    for (uint32_t s = first + kHeld * kRowWaves; s < a.parts; s += kRowWaves)
-        v += load(s) * weight(a.part_ml[(size_t)s * a.rows + row].x);
+    for (uint32_t s = first + kHeld * kRowWaves; s < parts; s += kRowWaves)
+        v += load(s) * weight(part_ml[(size_t)s * rows + row].x);
     if constexpr (kRowWaves > 1) {
         lds_o[wave][lane] = v;
         __syncthreads();
         if (first != 0) return;
         for (uint32_t k = 1; k < kRowWaves; ++k) v += lds_o[k][lane];
     }
-    store_out(a.out + row * c.vdim, c.vdim, d, finish(v, all.x, all.y));
+    if (!there) return;
+    store_out(a.out + row * vdim, vdim, d, finish(v, all.x, all.y));
     if (a.row_ml != nullptr && lane == 0) a.row_ml[row] = weight_terms(all.x, all.y);
 }
 
@@ -504,8 +517,9 @@ template <typename S, uint32_t P>
 hipError_t launch_rows(const Args<S> &a, uint32_t groups, hipStream_t s) {
     const dim3 grid(groups * a.parts, a.c.heads, a.pairs / a.c.heads);
     const size_t bytes = (size_t)a.pairs * a.longest * (a.c.kp + a.c.vp);
-    if (bytes > kStreamBytes) kv_rows_kernel<S, P, true><<<grid, kThreads, 0, s>>>(a);
-    else kv_rows_kernel<S, P, false><<<grid, kThreads, 0, s>>>(a);
+    const auto kernel = bytes > kStreamBytes ? kv_rows_kernel<S, P, true> : kv_rows_kernel<S, P, false>;
+    kernel<<<grid, kThreads, 0, s>>>(a.c.k, a.c.v, a.c.length, a.c.meta, a.q, a.c.blocks, a.c.heads,
+                                     a.parts | a.first << 16, a.c.kp | a.c.vp << 16, a.n, a.group, a);
     return hipGetLastError();
 }
 template <typename S>
@@ -537,9 +551,13 @@ hipError_t launch(Args<S> a, const Plan &p, uint32_t batch, uint32_t longest, fl
         const uint32_t workgroups = p.parts <= kWaves ? (folds + kWaves - 1) / kWaves : folds;
         const uint32_t grid = workgroups + a.pairs * token_groups;
         if (grid == 0) return hipSuccess;
-        if (p.parts <= kWaves) kv_fold_kernel<S, kWaves, 1><<<grid, threads, 0, s>>>(a, workgroups, token_groups);
-        else if (threads == kThreads) kv_fold_kernel<S, kWaves, kWaves><<<grid, threads, 0, s>>>(a, workgroups, token_groups);
-        else kv_fold_kernel<S, 16, 16><<<grid, threads, 0, s>>>(a, workgroups, token_groups);
+        auto fold = [&](auto kernel) {
+            kernel<<<grid, threads, 0, s>>>(a.part_o, a.part_ml, a.rows, p.parts, a.n, a.group * a.n, a.c.vdim, workgroups,
+                                            a.first * a.c.heads * a.group * a.n, token_groups, folds, a);
+        };
+        if (p.parts <= kWaves) fold(kv_fold_kernel<S, kWaves, 1>);
+        else if (threads == kThreads) fold(kv_fold_kernel<S, kWaves, kWaves>);
+        else fold(kv_fold_kernel<S, 16, 16>);
         const hipError_t status = hipGetLastError();
         if (status != hipSuccess) return status;
     }
