@@ -166,7 +166,9 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(const uint8_t *keys, 
         load_k(t);
         load_v(t);
     }
-    const uint32_t in_head = group * n, row0 = (a.row_group0 + blockIdx.x / parts) * kRows, count = a.count.n[b];
+    const uint32_t in_head = group * n, count = a.count.n[b];
+    // (the last rows, which see most keys, first)
+    const uint32_t row0 = (a.row_groups - 1 - a.row_group0 - blockIdx.x / parts) * kRows;
     // what the rows see, from the first one's place among its query head's n
     const uint32_t i0 = n == 1 ? 0 : row0 % n;
     const bool another = row0 + (n - i0) < in_head && i0 + kRows > n;   // rows of a next query head too
@@ -469,7 +471,14 @@ struct Plan {
 size_t whole256(size_t bytes) { return (bytes + 255) / 256 * 256; }
 uint32_t widest_of(const View &c) { return c.kp > c.vp ? c.kp : c.vp; }
 
-constexpr uint32_t kMinTileRows = 64;   // packed rows of a head from which tiles are used
+// Products of a call from which the kernel of 128-row tiles is used: it reads each
+// operand for twice the rows and takes each code to f16 once for 128, but a
+// workgroup's turn lasts long. Measured (us, rows kernel and tiles, causal): f16 D 128,
+// 8 heads x 512 rows x 2000 keys (1.0e9) 22 and 29, 8 x 384 x 8000 (3.1e9) 54 and 48,
+// 32 x 512 x 8000 175 and 89; D 64, 32 x 384 x 2000 (1.6e9) 23 and 38, 32 x 256 x 8000
+// (4.2e9) 52 and 43; f32 D 80, 8 x 1024 x 8000 (5.2e9) 86 and 94, 8 x 2048 x 8000
+// (1.0e10) 160 and 133.
+constexpr double kTileProducts = 2.6e9, kTileProductsF32 = 7.0e9;
 constexpr uint32_t kWorkgroups = 512;   // two for every CU
 
 Plan plan_of(bool f32, const View &c, const AttentionShape &a) {
@@ -477,7 +486,10 @@ Plan plan_of(bool f32, const View &c, const AttentionShape &a) {
     const uint32_t in_head = a.q_heads / c.heads * a.n;
     const uint32_t blocks = (a.longest + kTokens - 1) / kTokens;
     const uint64_t pairs = (uint64_t)a.batch * c.heads;
-    p.tiles = in_head >= kMinTileRows && tiles_fit(f32, widest_of(c));
+    // keys that a row sees on average
+    const double keys = a.longest - (a.causal ? 0.5 * (a.n < a.longest ? a.n : a.longest) : 0.0);
+    const double products = (double)pairs * in_head * keys * widest_of(c);
+    p.tiles = products >= (f32 ? kTileProductsF32 : kTileProducts) && tiles_fit(f32, widest_of(c));
     const uint32_t rows_each = p.tiles ? kTileRows : kRows;
     p.row_groups = (in_head + rows_each - 1) / rows_each;
     // parts: workgroups for every CU twice over, with a block for each wave (tiles:
@@ -593,6 +605,7 @@ hipError_t run(const View &c, const AttentionShape &sh, const void *query, void 
     a.n = sh.n;
     a.parts = p.parts;
     a.longest = sh.longest;
+    a.row_groups = p.row_groups;
     a.scale2 = (double)sh.scale * kLog2e;
     a.causal = sh.causal;
     for (uint32_t first = 0; first < sh.batch; first += kBatchPerLaunch) {

@@ -494,10 +494,14 @@ __global__ __launch_bounds__(kThreads, P <= 64 ? 3 : P <= 128 ? 2 : 1) void kv_w
     // staging: row tid / 8 of the step, groups tid % 8, + 8, ... of its dims
     const uint32_t srow = tid / 8, sub = tid % 8;
     typedef S vec8 __attribute__((ext_vector_type(8)));
-    vec8 x[G];
-    f32x2 ml;
-    auto fetch = [&](uint32_t step) {
-        const uint32_t r = step * kStep + srow;
+    struct Staged {
+        vec8 x[G];
+        f32x2 ml;
+    };
+    auto fetch = [&](uint32_t step, Staged &to) {
+        vec8 (&x)[G] = to.x;
+        f32x2 &ml = to.ml;
+        const uint32_t r = min(step, steps - 1) * kStep + srow;
         const size_t row = head * in_head + min(r, in_head - 1);
         const S *src = a.q + row * c.dim;
         ml = a.row_ml[row];
@@ -513,7 +517,9 @@ __global__ __launch_bounds__(kThreads, P <= 64 ? 3 : P <= 128 ? 2 : 1) void kv_w
             }
         }
     };
-    auto stash = [&](uint32_t buf) {
+    auto stash = [&](uint32_t buf, Staged &from) {
+        vec8 (&x)[G] = from.x;
+        const f32x2 ml = from.ml;
         // a row that adds nothing: zeros, so that its raw products are finite
 #pragma unroll
         for (uint32_t g = 0; g < G; ++g) {
@@ -556,15 +562,18 @@ __global__ __launch_bounds__(kThreads, P <= 64 ? 3 : P <= 128 ? 2 : 1) void kv_w
         }
         if (sub == 0) terms[buf][srow] = f32x4{ml.x, ml.y, factor, 0.0f};
     };
-    uint32_t step = from(row_part), buf = 0;
-    if (step < steps) {
-        fetch(step);
-        stash(0);
-    }
+    // two steps' rows are on their way while a step is computed
+    Staged even, odd;
+    const uint32_t first = from(row_part);
+    uint32_t second = from(first + row_parts);
+    fetch(first, even);
+    stash(0, even);
+    fetch(second, odd);
     __syncthreads();
-    for (uint32_t next; step < steps; step = next, buf ^= 1) {
-        next = from(step + row_parts);
-        if (next < steps) fetch(next);
+    // one step, from LDS buffer buf; `next` is staged, the one after it asked for
+    auto turn = [&](uint32_t step, uint32_t next, uint32_t buf, Staged &staged, Staged &ahead) {
+        const uint32_t after = from(next + row_parts);
+        fetch(after, ahead);
         const uint32_t r = step * kStep + col, i = r % a.n;
         const bool live = r < in_head && i < count;
         const int seen = seen_by(i, live, length, count, a.causal);
@@ -603,8 +612,16 @@ __global__ __launch_bounds__(kThreads, P <= 64 ? 3 : P <= 128 ? 2 : 1) void kv_w
                 acc[e] = __builtin_fmaf(__builtin_amdgcn_exp2f(__builtin_fmaf(st[e / 16][e % 16], factor, -term.x)), term.y,
                                         acc[e]);
         }
-        if (next < steps) stash(buf ^ 1);
+        stash(buf ^ 1, staged);
         __syncthreads();
+        return after;
+    };
+    for (uint32_t step = first; step < steps;) {
+        const uint32_t third = turn(step, second, 0, odd, even);
+        step = second;
+        if (step >= steps) break;
+        second = turn(step, third, 1, even, odd);
+        step = third;
     }
     // sums over the 32 rows of a half wave: each exchange halves the values, and
     // lane col ends with value col

@@ -41,7 +41,7 @@ template <typename S> struct Args {
     size_t score_stride;
     size_t weight_stride;
     uint32_t weight_tokens;
-    uint32_t first, pairs, group, n, parts, row_group0, longest;
+    uint32_t first, pairs, group, n, parts, row_group0, row_groups, longest;
     double scale2;       // scale * log2 e
     int causal;
     Counts count;

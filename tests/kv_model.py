@@ -156,37 +156,40 @@ class Model:
         weights, wtol = np.zeros((batch, heads, longest)), np.zeros((batch, heads, longest))
         for b in range(batch):
             count, length = n if counts is None else counts[b], self.length(b)
+            i = np.arange(count)
+            seen = np.maximum(length - count + i + 1, 0) if causal else np.full(count, length)
+            hidden = np.arange(length)[None, :] >= seen[:, None]
             for j in range(hq):
                 h = j // (hq // heads)
                 k, v = self.k[b][h].held(), self.v[b][h].held()
-                for i in range(count):
-                    seen = length - count + i + 1 if causal else length
-                    seen = max(seen, 0)
-                    with np.errstate(invalid="ignore", over="ignore"):
-                        s = k[:seen] @ q[b, j, i] * scale
-                        big_a = float((np.abs(k[:seen]) @ np.abs(q[b, j, i])).max(initial=0.0)) * abs(scale)
-                    s[self.marked[b][h][:seen]] = np.nan
-                    top = np.nanmax(s) if seen and not np.isnan(s).all() else -np.inf
-                    if not np.isfinite(top):
-                        out[b, j, i] = 0.0
-                        continue
-                    if np.isnan(s).any():
-                        continue      # a NaN row (out is NaN there)
-                    p = np.exp(s - top)
-                    total = p.sum()
-                    p /= total
-                    o, mass = p @ v[:seen], p @ np.abs(v[:seen])
-                    out[b, j, i] = o
-                    score = 2 * (dim + 16) * u * (big_a + 1)
-                    rel = score + 2 * seen * u
-                    if half:
-                        tol[b, j, i] = (rel + 2.0 ** -10) * mass + 2.0 ** -11 * np.abs(o) \
-                            + 2.0 ** -26 * (np.abs(v[:seen]).sum(0) + seen * np.abs(o)) / total + 2.0 ** -24
-                    else:
-                        tol[b, j, i] = (rel + 2.0 ** -21) * mass + 4 * u * np.abs(o) \
-                            + 2.0 ** -34 * np.abs(v[:seen]).sum(0) / total + 1e-40
-                    weights[b, h, :seen] += p
-                    # (f16: the sum is that of the rounded P)
-                    wtol[b, h, :seen] += (rel + 16 * u + (2.0 ** -11 if half else 0)) * p \
-                        + (2.0 ** -26 * seen / total * p if half else 0)
+                with np.errstate(invalid="ignore", over="ignore"):
+                    s = q[b, j, :count] @ k.T * scale
+                    size = np.where(hidden, 0.0, np.abs(q[b, j, :count]) @ np.abs(k).T * abs(scale))
+                s[:, self.marked[b][h]] = np.nan
+                s[hidden] = -np.inf
+                has_nan = np.isnan(s).any(-1)
+                top = np.where(np.isnan(s), -np.inf, s).max(-1, initial=-np.inf)
+                zero = ~np.isfinite(top)
+                plain = ~zero & ~has_nan
+                out[b, j, :count][zero] = 0.0
+                if not plain.any():
+                    continue
+                s, big_a, n_seen = s[plain], size[plain].max(-1)[:, None], seen[plain][:, None]
+                p = np.exp(s - top[plain][:, None])
+                total = p.sum(-1, keepdims=True)
+                p /= total
+                o, mass = p @ v, p @ np.abs(v)
+                out[b, j, :count][plain] = o
+                in_sight = np.cumsum(np.abs(v), axis=0)[seen[plain] - 1]
+                rel = 2 * (dim + 16) * u * (big_a + 1) + 2 * n_seen * u
+                if half:
+                    t = (rel + 2.0 ** -10) * mass + 2.0 ** -11 * np.abs(o) \
+                        + 2.0 ** -26 * (in_sight + n_seen * np.abs(o)) / total + 2.0 ** -24
+                else:
+                    t = (rel + 2.0 ** -21) * mass + 4 * u * np.abs(o) + 2.0 ** -34 * in_sight / total + 1e-40
+                tol[b, j, :count][plain] = t
+                weights[b, h, :length] += p.sum(0)
+                # (f16: the sum is that of the rounded P)
+                w = rel + 16 * u + (2.0 ** -11 + 2.0 ** -26 * n_seen / total if half else 0)
+                wtol[b, h, :length] += (w * p).sum(0)
         return out, tol, weights, wtol

@@ -93,6 +93,71 @@ def test_chunks(sdk, shape, dtype):
     run(pair, dtype, heads, n, causal=False, what="all seen")
 
 
+# kv heads, query heads, length, n, dim, value dim: enough products for the kernel
+# of 128-row tiles, in few row groups (parts of the keys) and in many (none)
+TILES = [(1, 2, 17000, 600, 128, 128), (1, 3, 16448, 470, 120, 100), (2, 2, 21000, 1000, 64, 64),
+         (1, 1, 41000, 1000, 64, 40), (1, 2, 50001, 830, 20, 32), (1, 2, 20010, 700, 80, 96),
+         (1, 1, 21000, 650, 192, 160), (1, 2, 9000, 601, 256, 200), (64, 64, 1300, 512, 32, 32),
+         (32, 64, 641, 641, 64, 64), (8, 16, 2100, 2100, 33, 50)]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("shape", TILES, ids=str)
+def test_tiles(sdk, shape, causal):
+    kv, heads, length, n, dim, vdim = shape
+    pair = Pair(sdk, 2 if kv == 64 else 1, kv, length, dim, vdim, n)
+    pair.append(length)
+    run(pair, "f16", heads, n, causal=causal, weighted=True, what="f16")
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("shape", [(1, 2, 30000, 1001, 128, 128), (1, 2, 40010, 1000, 80, 96), (2, 2, 50000, 1150, 64, 60),
+                                   (1, 4, 64000, 1000, 30, 17), (64, 64, 1700, 1024, 32, 32)], ids=str)
+def test_tiles_f32(sdk, shape, causal):
+    kv, heads, length, n, dim, vdim = shape
+    pair = Pair(sdk, 2 if kv == 64 else 1, kv, length, dim, vdim, n)
+    pair.append(length)
+    run(pair, "f32", heads, n, causal=causal, weighted=True, what="f32")
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_tiles_ragged(sdk, dtype):
+    """Sequences of other lengths and row counts in one call, one empty, one whose
+    rows are more than its tokens, with marked tokens, zero and far value scales and
+    query rows that are not finite."""
+    long = 70000 if dtype == "f32" else 30000
+    pair = Pair(sdk, 4, 1, long, 64, 64, 31)
+    k = rows_of(pair.rng, (4, 1, long, 64), "f16")
+    v = rows_of(pair.rng, (4, 1, long, 64), "f16")
+    v[:, :, 128:192] = 0
+    v[:, :, 640:704] *= np.float16(2.0 ** -12)
+    v[:, :, 704:768] *= np.float16(64.0)
+    lengths = [long, 6400, 0, 300]
+    k[0, 0, long - 700, 3] = np.nan       # the first rows do not see it
+    v[1, 0, 6399, 0] = np.inf             # the last row's own token
+    k[3, 0, 299, 9] = np.nan
+    pair.append(long, counts=lengths, key=k, value=v)
+    n, counts = 1000, [1000, 700, 5, 900]
+    run(pair, dtype, 3, n, counts=counts, weighted=True, what="causal")
+    run(pair, dtype, 3, n, counts=counts, causal=False, what="all seen")
+    q = pair.rng.standard_normal((4, 3, n, 64)).astype(DTYPES[dtype])
+    q[0, 0, 0, 3], q[1, 1, 100, 0], q[3, 2, 899, 39] = np.nan, np.inf, -np.inf
+    got, _ = attend(sdk, pair.cache, q, 0.2, True, counts, None, 64)
+    assert (got[0, 0, 0] == 0).all() and (got[1, 1, 100] == 0).all() and (got[3, 2, 899] == 0).all()
+    good = np.isfinite(q).all(-1)
+    clean = np.where(np.isfinite(q), q, 0)
+    want, tol, _, _ = pair.model.attention(clean, 0.2, True, counts)
+    good &= ~np.isnan(want).any(-1)
+    assert (np.abs(got.astype(np.float64) - want) <= tol)[good].all()
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 4.0])
+def test_tiles_scales(sdk, scale):
+    pair = Pair(sdk, 1, 1, 30000, 64, 64, 32)
+    pair.append(29000)
+    run(pair, "f16", 2, 900, scale=scale, weighted=True)
+
+
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
 @pytest.mark.parametrize("n", [1, 4, 40, 130])
 def test_ragged_batch(sdk, n, dtype):
@@ -212,7 +277,7 @@ def test_calls_give_the_same_bits(sdk):
     """No sum depends on the order in which workgroups end."""
     pair = Pair(sdk, 2, 2, 3000, 64, 64, 20)
     pair.append(2900)
-    for n in (1, 70):
+    for n in (1, 70, 1800):
         q = pair.rng.standard_normal((2, 6, n, 64)).astype(np.float16)
         w0 = np.zeros((2, 2, 2900), np.float32)
         first = attend(sdk, pair.cache, q, 0.125, True, None, w0, 64)
@@ -222,7 +287,7 @@ def test_calls_give_the_same_bits(sdk):
 
 
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
-@pytest.mark.parametrize("shape", [(4, 1), (4, 40), (8, 200)], ids=str)
+@pytest.mark.parametrize("shape", [(4, 1), (4, 40), (8, 900)], ids=str)
 def test_recorded_attention_follows_the_cache(sdk, shape, dtype):
     """A replay attends to what the cache then holds: after appends (tokens of
     the open block have become codes), cuts and eager calls in between."""
