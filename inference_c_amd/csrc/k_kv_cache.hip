@@ -5,12 +5,13 @@
 // rows into dim rows.
 //
 // Codes. With a the largest |x| of the block (f16), code = rne(127 x / a). The
-// kernels compute q = x * fl(127 / a), whose relative error is below 2^-23, and
-// round that. A quotient that is no tie lies at least 2^(k - 20) from one where
-// |code| < 2^(k + 1) (127 x and (2 c + 1) a / 2 are whole multiples of a
-// common unit, x and a having 11 significant bits), four times q's error, so
-// only exact ties need a second look: r = 127 x - c a is exact in f32 (18-bit
-// products), a tie is |2 r| = a, and the odd one of its two codes gives way.
+// kernels compute the quotient as a division does: q = 127 x * fl(1 / a), its exact
+// remainder by one fma, and q + remainder * fl(1 / a), which is the correctly
+// rounded quotient; then its rounding to a whole number by adding 1.5 * 2^23. Ties
+// (x = a / 2 is one) come out exactly, being representable, and a quotient that is
+// none lies at least 2^(k - 20) from one where |code| < 2^(k + 1) (127 x and
+// (2 c + 1) a / 2 are whole multiples of a common unit, x and a having 11
+// significant bits), eight times the f32 step there.
 #include "kern_common.hpp"
 #include "kv.hpp"
 
@@ -37,14 +38,22 @@ __device__ inline float value_of(float code, float scale) {
     return v;
 }
 
-// Code of x (f16 as f32) in a block of largest |x| a > 0; inverse = 127 / a.
-__device__ inline int code_of(float x, float a, float inverse) {
-    const float c = rintf(x * inverse);
-    const float r = __builtin_fmaf(-c, a, 127.0f * x);
-    int code = (int)c;
-    if (fabsf(r) * 2.0f == a && (code & 1)) code += r > 0.0f ? 1 : -1;
-    return code;
-}
+// What makes codes of a block's elements; an all-zero block's are all 0.
+struct Coder {
+    float a, inverse;
+    __device__ explicit Coder(float largest) : a(largest), inverse(largest > 0.0f ? 1.0f / largest : 0.0f) {}
+    // code + 128 in the low byte
+    __device__ inline uint32_t byte(float x) const {
+        const float x127 = 127.0f * x, q = x127 * inverse;
+        const float quotient = __builtin_fmaf(__builtin_fmaf(-q, a, x127), inverse, q);
+        return __builtin_bit_cast(uint32_t, quotient + (12582912.0f + 128.0f));
+    }
+    __device__ inline uint32_t four(float x0, float x1, float x2, float x3) const {
+        const uint32_t lo = __builtin_amdgcn_perm(byte(x1), byte(x0), 0x0c0c0400u);
+        const uint32_t hi = __builtin_amdgcn_perm(byte(x3), byte(x2), 0x04000c0cu);
+        return lo | hi;
+    }
+};
 
 // Largest of the workgroup's values (all >= 0), for every thread.
 __device__ inline float block_max(float v, float *slots) {
@@ -168,8 +177,7 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(AppendArgs<S> a) {
             vmax = block_max(vmax, slots);
             k_scale = kmax / 127.0f;
             v_scale = vmax / 127.0f;
-            // (an all-zero block: inverse 0 makes every code 0)
-            const float kinv = kmax > 0.0f ? 127.0f / kmax : 0.0f, vinv = vmax > 0.0f ? 127.0f / vmax : 0.0f;
+            const Coder kcoder(kmax), vcoder(vmax);
             const size_t block = head * c.blocks + j;
             u32x4 *const ko = reinterpret_cast<u32x4 *>(c.k + block * kTokens * kp);
             u32x4 *const vo = reinterpret_cast<u32x4 *>(c.v + block * kTokens * vp);
@@ -177,11 +185,8 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(AppendArgs<S> a) {
                 u32x4 out;
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
-                    uint32_t word = 0;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        word |= (uint32_t)(code_of((float)half_of(rk[i * 16 + w * 4 + e]), kmax, kinv) + 128) << (8 * e);
-                    out[w] = word;
+                    const uint16_t *x = &rk[i * 16 + w * 4];
+                    out[w] = kcoder.four((float)half_of(x[0]), (float)half_of(x[1]), (float)half_of(x[2]), (float)half_of(x[3]));
                 }
                 ko[i] = out;
             }
@@ -190,12 +195,9 @@ __global__ __launch_bounds__(kThreads) void kv_append_kernel(AppendArgs<S> a) {
                 u32x4 out;
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
-                    uint32_t word = 0;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        word |= (uint32_t)(code_of((float)half_of(rv[(t0 + w * 4 + e) * vpitch + d]), vmax, vinv) + 128)
-                                << (8 * e);
-                    out[w] = word;
+                    const uint16_t *x = &rv[(t0 + w * 4) * vpitch + d];
+                    out[w] = vcoder.four((float)half_of(x[0]), (float)half_of(x[vpitch]), (float)half_of(x[2 * vpitch]),
+                                         (float)half_of(x[3 * vpitch]));
                 }
                 vo[i] = out;
             }
@@ -235,25 +237,18 @@ template <typename S> __device__ inline half8 load8(const S *p) {
         return r;
     }
 }
-__device__ inline bool finite8(half8 v) {
+// Bits of the largest |element|; 0x7c00 and more: one is not finite.
+__device__ inline uint32_t largest8(half8 v) {
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
     const u32x4 w = __builtin_bit_cast(u32x4, v);
-    bool good = true;
+    u16x2 m[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-        good = good && (w[i] & 0x7c00u) != 0x7c00u && (w[i] & 0x7c000000u) != 0x7c000000u;
-    return good;
+    for (int i = 0; i < 4; ++i) m[i] = __builtin_bit_cast(u16x2, w[i] & 0x7fff7fffu);
+    const u16x2 x = __builtin_elementwise_max(__builtin_elementwise_max(m[0], m[1]), __builtin_elementwise_max(m[2], m[3]));
+    return x.x > x.y ? x.x : x.y;
 }
-__device__ inline float largest8(half8 v, float m) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) m = fmaxf(m, fabsf((float)v[e]));
-    return m;
-}
-// Bytes code + 128 of four elements.
-__device__ inline uint32_t pack4(half8 v, int first, float a, float inverse) {
-    uint32_t word = 0;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) word |= (uint32_t)(code_of((float)v[first + e], a, inverse) + 128) << (8 * e);
-    return word;
+__device__ inline uint32_t pack4(half8 v, int first, const Coder &coder) {
+    return coder.four((float)v[first], (float)v[first + 1], (float)v[first + 2], (float)v[first + 3]);
 }
 // Rows w[0..3] of four bytes each become columns.
 __device__ inline void transpose4(uint32_t (&w)[4]) {
@@ -266,7 +261,7 @@ __device__ inline void transpose4(uint32_t (&w)[4]) {
 }
 
 template <typename S, uint32_t P>
-__global__ __launch_bounds__(2 * kThreads) void kv_append_groups_kernel(AppendArgs<S> a) {
+__global__ __launch_bounds__(2 * kThreads, P <= 128 ? 4 : 2) void kv_append_groups_kernel(AppendArgs<S> a) {
     constexpr uint32_t N = P <= 128 ? 4 : 8;   // groups of a thread: 64 P / 8 / 256, whole fours
     constexpr uint32_t kPitch = kTokens + 4;
     __shared__ __attribute__((aligned(16))) uint8_t turned[P * kPitch];
@@ -307,6 +302,7 @@ __global__ __launch_bounds__(2 * kThreads) void kv_append_groups_kernel(AppendAr
         // new read one that is, so that no load waits for a test
         const S *const rows = memory + ((ptrdiff_t)(head * a.n) + (ptrdiff_t)j * kTokens - start) * (ptrdiff_t)width;
         half8 x[N];
+        uint32_t largest[N];
 #pragma unroll
         for (uint32_t u = 0; u < N; ++u)
             if (values || u < P / 32) x[u] = load8(rows + (size_t)min(max(token[u], from), to - 1) * width + dim[u]);
@@ -315,7 +311,8 @@ __global__ __launch_bounds__(2 * kThreads) void kv_append_groups_kernel(AppendAr
         for (uint32_t u = 0; u < N; ++u) {
             const uint32_t t = token[u];
             if (t < from || t >= to) x[u] = half8{};   // (and those past the block)
-            else if (!finite8(x[u])) atomicOr(&marks[t / 32], 1u << (t % 32));
+            largest[u] = largest8(x[u]);
+            if (largest[u] >= 0x7c00u) atomicOr(&marks[t / 32], 1u << (t % 32));
         }
         if (closed && from != 0) {   // the rows the open block had
 #pragma unroll
@@ -327,6 +324,7 @@ __global__ __launch_bounds__(2 * kThreads) void kv_append_groups_kernel(AppendAr
 #pragma unroll
                     for (uint32_t e = 0; e < 8; ++e) x[u][e] = vt[(dim[u] + e) * kTokens + token[u]];
                 }
+                largest[u] = largest8(x[u]);
             }
         }
         __syncthreads();
@@ -335,29 +333,31 @@ __global__ __launch_bounds__(2 * kThreads) void kv_append_groups_kernel(AppendAr
         if (fresh != 0) {   // marked rows are held as zeros
 #pragma unroll
             for (uint32_t u = 0; u < N; ++u)
-                if (fresh >> (token[u] & 63) & 1) x[u] = half8{};
+                if (fresh >> (token[u] & 63) & 1) {
+                    x[u] = half8{};
+                    largest[u] = 0;
+                }
         }
         float scale = 1.0f;
         if (closed) {
-            float big = 0.0f;
+            uint32_t most = 0;
 #pragma unroll
-            for (uint32_t u = 0; u < N; ++u) big = largest8(x[u], big);
-            big = wave_max(big);
+            for (uint32_t u = 0; u < N; ++u) most = max(most, largest[u]);
+            float big = wave_max((float)half_of((uint16_t)most));
             if ((threadIdx.x & (kWave - 1)) == 0) slots[wave] = big;
             __syncthreads();
             big = slots[values * kWaves];
 #pragma unroll
             for (uint32_t i = 1; i < kWaves; ++i) big = fmaxf(big, slots[values * kWaves + i]);
             scale = big / 127.0f;
-            // (an all-zero block: inverse 0 makes every code 0)
-            const float inverse = big > 0.0f ? 127.0f / big : 0.0f;
+            const Coder coder(big);
             if (!values) {
                 uint8_t *const out = c.k + (head * c.blocks + j) * kTokens * kp;
 #pragma unroll
                 for (uint32_t u = 0; u < N; ++u)
                     if (token[u] < kTokens)
                         *reinterpret_cast<uint2 *>(out + token[u] * kp + dim[u]) =
-                            uint2{pack4(x[u], 0, big, inverse), pack4(x[u], 4, big, inverse)};
+                            uint2{pack4(x[u], 0, coder), pack4(x[u], 4, coder)};
             } else {
 #pragma unroll
                 for (uint32_t u = 0; u < N; u += 4) {
@@ -366,7 +366,7 @@ __global__ __launch_bounds__(2 * kThreads) void kv_append_groups_kernel(AppendAr
                     for (uint32_t half = 0; half < 2; ++half) {
                         uint32_t w[4];
 #pragma unroll
-                        for (uint32_t r = 0; r < 4; ++r) w[r] = pack4(x[u + r], 4 * half, big, inverse);
+                        for (uint32_t r = 0; r < 4; ++r) w[r] = pack4(x[u + r], 4 * half, coder);
                         transpose4(w);
 #pragma unroll
                         for (uint32_t e = 0; e < 4; ++e)
@@ -709,7 +709,9 @@ struct MoveArgs {
 // the values one kept token (a lane each) in four neighbouring dims of every
 // sixteen, byte by byte: the lanes' tokens lie in a few 64-byte rows of the
 // source. Four lanes turn their new codes of four dims into four tokens of one
-// dim each, and store words.
+// dim each, and store words. (The source's blocks brought to LDS whole and the bytes
+// read there: 56 against 48 us, since blocks of which half the tokens go are read
+// whole.)
 __device__ inline uint32_t value_dim(uint32_t u, uint32_t wave) { return u / 4 * 16 + wave * 4 + u % 4; }
 // Bytes (dims 0 .. 3 of one lane's token) to bytes (tokens of four lanes) of the
 // dim lane % 4: exchanges with lane ^ 1, then lane ^ 2.
@@ -725,14 +727,27 @@ __device__ inline double wave_max_f64(double v) {
     return v;
 }
 
-// A value anew: x is a code with its block's scale, or (scale 1) an f16.
-struct Held {
-    float x;
-    __device__ inline uint32_t code(float scale, float ratio, double big) const {
-        const float q = x * ratio;
-        float n = rintf(q);
-        if (fabsf(fabsf(q - n) - 0.5f) < 0x1p-12f) n = (float)rint(127.0 * ((double)x * (double)scale) / big);
-        return (uint32_t)((int)n + 128);
+// Values anew: x is a code with its block's scale, or (scale 1) an f16.
+struct Recoder {
+    float scale, ratio;   // ratio = 127 scale / largest; an all-zero block's is 0
+    double big;
+    // Codes + 128 of four elements as bytes.
+    __device__ inline uint32_t four(const _Float16 *x) const {
+        constexpr float kWhole = 12582912.0f + 128.0f;   // 1.5 * 2^23: rounds to whole numbers
+        uint32_t b[4];
+        bool near = false;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float q = (float)x[e] * ratio, n = q + kWhole;
+            near = near || fabsf(q - (n - kWhole)) > 0.5f - 0x1p-12f;
+            b[e] = __builtin_bit_cast(uint32_t, n);
+        }
+        if (near) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                b[e] = big > 0.0 ? (uint32_t)(int)rint(127.0 * ((double)(float)x[e] * (double)scale) / big) + 128u : 128u;
+        }
+        return __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u) | __builtin_amdgcn_perm(b[3], b[2], 0x04000c0cu);
     }
 };
 
@@ -833,27 +848,24 @@ __global__ __launch_bounds__(kThreads) void kv_move_kernel(MoveArgs a) {
     for (uint32_t w = 0; w < kWaves; ++w)
 #pragma unroll
         for (int i = 0; i < 2; ++i) big[i] = fmax(big[i], biggest[i][w]);
-    // (an all-zero block: ratio 0 makes every code 0, and no tie is near)
-    const float k_ratio = big[0] > 0.0 ? (float)(127.0 * (double)k_old / big[0]) : 0.0f;
-    const float v_ratio = big[1] > 0.0 ? (float)(127.0 * (double)v_old / big[1]) : 0.0f;
+    const Recoder keys{k_old, big[0] > 0.0 ? (float)(127.0 * (double)k_old / big[0]) : 0.0f, big[0]};
+    const Recoder values{v_old, big[1] > 0.0 ? (float)(127.0 * (double)v_old / big[1]) : 0.0f, big[1]};
     const size_t block = head * c.blocks + j;
 #pragma unroll
     for (uint32_t u = 0; u < P / 64; ++u) {
         const uint32_t d = (tid % 4 + 4 * u) * 16;
         if (d >= kp) continue;
-        u32x4 w = {0, 0, 0, 0};
+        u32x4 w;
 #pragma unroll
-        for (int e = 0; e < 16; ++e) w[e / 4] |= Held{(float)kx[u][e]}.code(k_old, k_ratio, big[0]) << (8 * (e % 4));
+        for (int e = 0; e < 4; ++e) w[e] = keys.four(&kx[u][4 * e]);
         *reinterpret_cast<u32x4 *>(c.k + (block * kTokens + row) * kp + d) = w;
     }
 #pragma unroll
     for (uint32_t u = 0; u < P / 4; u += 4) {
         const uint32_t d = value_dim(u, wave);
         if (d >= vp) continue;
-        uint32_t w = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w |= Held{(float)vx[u + e]}.code(v_old, v_ratio, big[1]) << (8 * e);
-        *reinterpret_cast<uint32_t *>(c.v + (block * vp + d + lane % 4) * kTokens + lane / 4 * 4) = quad_transpose(w, lane);
+        *reinterpret_cast<uint32_t *>(c.v + (block * vp + d + lane % 4) * kTokens + lane / 4 * 4) =
+            quad_transpose(values.four(&vx[u]), lane);
     }
     if (tid == 0)
         c.meta[block] = Meta{(float)(big[0] / 127.0), (float)(big[1] / 127.0), marks[0] | (uint64_t)marks[1] << 32};
