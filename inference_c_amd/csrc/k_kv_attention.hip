@@ -23,9 +23,13 @@
 // v (the output rescaled) when the ratio leaves 2^-3 .. 2^3, so P keeps f16's
 // range whatever the blocks' scales are.
 //
-// f32: q and P each are a pair of f16 (q scaled by a power of two to a largest
-// element of 2^13 .. 2^14), 22 significant bits, and codes are exact: two MFMAs
-// in place of one.
+// f32: q is three f16 operands (scaled by a power of two to a largest element of 2^13 ..
+// 2^14), P a pair, 22 significant bits, and codes are exact. A block's output is added
+// to the running one in f32, rounded to nearest, as the MFMA does not.
+//
+// f16: the output is divided by the sum of P as rounded to f16, so that a row with one
+// large weight has its value exactly; accumulated token weights, which are f32, go by the
+// sum before that rounding.
 #include "kv_attention.hpp"
 
 namespace icsdk {
@@ -48,11 +52,11 @@ template <uint32_t P> __device__ inline uint32_t step_dim(uint32_t s, uint32_t g
     return s / 2 < P / 64 ? s / 2 * 64 + g * 16 + s % 2 * 8 : P / 64 * 64 + g * 8;
 }
 
-// A wave's 16 query rows as B operands, one per k step (f32: and their rest).
+// A wave's 16 query rows as B operands, one per k step and piece.
 template <typename S, uint32_t P> struct Query {
     static constexpr uint32_t kSteps = P / 32;
     static constexpr bool kPair = sizeof(S) == 4;
-    half8 hi[kSteps], lo[kPair ? kSteps : 1];
+    half8 piece[kPieces<S>][kSteps];
     float factor;   // the power of two that a f32 row was divided by
 
     __device__ inline void load(const S *row, uint32_t dim, uint32_t g) {
@@ -62,11 +66,11 @@ template <typename S, uint32_t P> struct Query {
             for (uint32_t s = 0; s < kSteps; ++s) {
                 const uint32_t d = step_dim<P>(s, g);
                 if (dim % 8 == 0) {
-                    hi[s] = *reinterpret_cast<const half8 *>(row + (d < dim ? d : 0));
-                    if (d >= dim) hi[s] = half8{};
+                    piece[0][s] = *reinterpret_cast<const half8 *>(row + (d < dim ? d : 0));
+                    if (d >= dim) piece[0][s] = half8{};
                 } else {
 #pragma unroll
-                    for (uint32_t e = 0; e < 8; ++e) hi[s][e] = d + e < dim ? row[d + e] : (_Float16)0.0f;
+                    for (uint32_t e = 0; e < 8; ++e) piece[0][s][e] = d + e < dim ? row[d + e] : (_Float16)0.0f;
                 }
             }
         } else {
@@ -93,8 +97,7 @@ template <typename S, uint32_t P> struct Query {
 #pragma unroll
                 for (uint32_t e = 0; e < 8; ++e) {
                     const float y = usable ? __builtin_ldexpf(x[s][e], 14 - exponent) : 0.0f;
-                    hi[s][e] = (_Float16)y;
-                    lo[s][e] = (_Float16)(y - (float)hi[s][e]);
+                    pieces_of(y, piece[0][s], piece[1][s], piece[2][s], e);
                 }
         }
     }
@@ -120,7 +123,7 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(const uint8_t *keys, 
     constexpr uint32_t NC = P / 64, NV = P / 16;
     constexpr bool kOdd = P % 64 != 0;
     __shared__ f32x4 lds_o[kWaves][NV][kWave];
-    __shared__ f32x2 lds_ml[kWaves][kRows];
+    __shared__ f32x4 lds_ml[kWaves][kRows];   // maximum, sums of P rounded and not
     const View &c = a.c;
     const uint32_t lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -190,28 +193,30 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(const uint8_t *keys, 
     f32x4 o[NV];
 #pragma unroll
     for (uint32_t j = 0; j < NV; ++j) o[j] = f32x4{0, 0, 0, 0};
-    float big = neg_inf, sum = 0.0f, unit = 1.0f, inverse_unit = 1.0f;
+    float big = neg_inf, sum = 0.0f, exact = 0.0f, unit = 1.0f, inverse_unit = 1.0f;
 
     // one block: kf(u, s) and vf(j, s) give the A operands
     auto step = [&](uint32_t t, Meta meta, auto kf, auto vf, auto keys_done) {
         // f32: what rounding takes off the factor and the scores is added back in
         // the exponent (scores of 10 would be off by 1e-6 of their weight)
-        float factor = meta.k_scale * (float)a.scale2, factor_rest = 0.0f;
+        const double whole_factor = (double)meta.k_scale * a.scale2;
+        float factor = (float)whole_factor, factor_rest = 0.0f;
         if constexpr (kPair) {
-            const double exact = (double)meta.k_scale * a.scale2;
-            factor = (float)exact * q.factor;
-            factor_rest = (float)(exact - (double)(float)exact) * q.factor;
+            factor_rest = (float)(whole_factor - (double)factor) * q.factor;
+            factor *= q.factor;
         }
         float p[16], rest[kPair ? 16 : 1];
 #pragma unroll
         for (uint32_t u = 0; u < 4; ++u) {
             f32x4 acc = {0, 0, 0, 0};
+            half8 k[Query<S, P>::kSteps];
 #pragma unroll
-            for (uint32_t s = 0; s < Query<S, P>::kSteps; ++s) {
-                const half8 k = kf(u, s);
-                acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q.hi[s], acc, 0, 0, 0);
-                if constexpr (kPair) acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, q.lo[s], acc, 0, 0, 0);
-            }
+            for (uint32_t s = 0; s < Query<S, P>::kSteps; ++s) k[s] = kf(u, s);
+#pragma unroll
+            for (uint32_t i = 0; i < kPieces<S>; ++i)
+#pragma unroll
+                for (uint32_t s = 0; s < Query<S, P>::kSteps; ++s)
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(k[s], q.piece[i][s], acc, 0, 0, 0);
 #pragma unroll
             for (uint32_t e = 0; e < 4; ++e) {
                 p[4 * u + e] = acc[e] * factor;
@@ -243,6 +248,7 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(const uint8_t *keys, 
             const float now = groups_max(fmaxf(top, big));
             const float alpha = now == neg_inf ? 1.0f : __builtin_amdgcn_exp2f(big - now);
             sum *= alpha;
+            exact *= alpha;
 #pragma unroll
             for (uint32_t j = 0; j < NV; ++j) o[j] *= alpha;
             big = now;
@@ -265,8 +271,11 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(const uint8_t *keys, 
         for (uint32_t e = 0; e < 16; ++e) {
             float x = p[e] - base;
             if constexpr (kPair) x += rest[e];
-            x = __builtin_amdgcn_exp2f(x);
-            const float y = x * ratio;
+            x = p[e] = __builtin_amdgcn_exp2f(x);
+            float y = x * (ratio * kPairScale<S>);
+            // (an f32 here: the compiler may take one f16 from the product's f32 and
+            // another, elsewhere, from the product itself, and the rest of the wrong one)
+            if constexpr (kPair) asm("" : "+v"(y));
             ph[e / 8][e % 8] = (_Float16)y;
             if constexpr (kPair) {
                 pl[e / 8][e % 8] = (_Float16)(y - (float)ph[e / 8][e % 8]);
@@ -276,14 +285,26 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(const uint8_t *keys, 
             }
         }
         sum += kPair ? add : add * fast_rcp(ratio);
+        if (!kPair && a.part_exact != nullptr) {
+            add = 0.0f;
+#pragma unroll
+            for (uint32_t e = 0; e < 16; ++e) add += p[e];
+            exact += add;
+        }
 #pragma unroll
         for (uint32_t j = 0; j < NV; ++j) {
             if (j * 16 >= vp) continue;
+            if constexpr (kPair) {
+                const half8 v[2] = {vf(j, 0), vf(j, 1)};
+                f32x4 x = {0, 0, 0, 0};
 #pragma unroll
-            for (uint32_t s = 0; s < 2; ++s) {
-                const half8 v = vf(j, s);
-                o[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, ph[s], o[j], 0, 0, 0);
-                if constexpr (kPair) o[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, pl[s], o[j], 0, 0, 0);
+                for (uint32_t s = 0; s < 2; ++s) x = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[s], pl[s], x, 0, 0, 0);
+#pragma unroll
+                for (uint32_t s = 0; s < 2; ++s) x = __builtin_amdgcn_mfma_f32_16x16x32_f16(v[s], ph[s], x, 0, 0, 0);
+                o[j] += x;
+            } else {
+#pragma unroll
+                for (uint32_t s = 0; s < 2; ++s) o[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vf(j, s), ph[s], o[j], 0, 0, 0);
             }
         }
     };
@@ -321,12 +342,13 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(const uint8_t *keys, 
 
     // the waves meet
     sum = groups_sum(sum);
+    exact = kPair ? sum : groups_sum(exact);
     big -= kHeadroom<S>;   // what P's exponents are relative to
-    if (g == 0) lds_ml[wave][m] = f32x2{big, sum};
+    if (g == 0) lds_ml[wave][m] = f32x4{big, sum, exact, 0.0f};
 #pragma unroll
-    for (uint32_t j = 0; j < NV; ++j) lds_o[wave][j][lane] = o[j] * unit;
+    for (uint32_t j = 0; j < NV; ++j) lds_o[wave][j][lane] = o[j] * (unit / kPairScale<S>);
     __syncthreads();
-    float top = neg_inf, total = 0.0f, w[kWaves];
+    float top = neg_inf, total = 0.0f, total_exact = 0.0f, w[kWaves];
 #pragma unroll
     for (uint32_t k = 0; k < kWaves; ++k) top = fmaxf(top, lds_ml[k][m].x);
 #pragma unroll
@@ -334,6 +356,7 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(const uint8_t *keys, 
         // (a wave that saw nothing has weight 0, and a NaN in it stays)
         w[k] = top == neg_inf ? 1.0f : __builtin_amdgcn_exp2f(lds_ml[k][m].x - top);
         total += w[k] * lds_ml[k][m].y;
+        total_exact += w[k] * lds_ml[k][m].z;
     }
     const bool writes = live && r < in_head;
     if (parts == 1) {
@@ -346,8 +369,11 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(const uint8_t *keys, 
             if (writes) store_out(out, c.vdim, 16 * j + 4 * g, finish(v, top, total));
         }
         if (writes && g == 0 && wave == 0) {
-            if (a.row_ml != nullptr) a.row_ml[row] = weight_terms(top, total);
-            if (a.scores != nullptr) a.part_ml[row] = f32x2{top, total};
+            if (a.row_ml != nullptr) a.row_ml[row] = weight_terms(top, total_exact);
+            if (a.scores != nullptr) {
+                a.part_ml[row] = f32x2{top, total};
+                a.part_exact[row] = total_exact;
+            }
         }
     } else {
         float *const out = a.part_o + ((size_t)part * a.rows + row) * c.vdim;
@@ -358,18 +384,23 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(const uint8_t *keys, 
             for (uint32_t k = 0; k < kWaves; ++k) v += lds_o[k][j][lane] * w[k];
             if (writes) store_out(out, c.vdim, 16 * j + 4 * g, v);
         }
-        if (writes && g == 0 && wave == 0) a.part_ml[(size_t)part * a.rows + row] = f32x2{top, total};
+        if (writes && g == 0 && wave == 0) {
+            a.part_ml[(size_t)part * a.rows + row] = f32x2{top, total};
+            if (a.part_exact != nullptr) a.part_exact[(size_t)part * a.rows + row] = total_exact;
+        }
     }
 }
 
-// Maximum and sum of a row from its parts', by one wave.
-__device__ inline f32x2 fold_ml(const f32x2 *ml, uint32_t parts, size_t rows, uint32_t lane) {
+// Maximum and sum (`exact`: the one before P's rounding) of a row from its parts',
+// by one wave.
+__device__ inline f32x2 fold_ml(const f32x2 *ml, const float *exact, uint32_t parts, size_t rows, uint32_t lane) {
     float top = -__builtin_inff(), total = 0.0f;
     for (uint32_t s = lane; s < parts; s += kWave) top = fmaxf(top, ml[s * rows].x);
     top = wave_max(top);
     for (uint32_t s = lane; s < parts; s += kWave) {
         const f32x2 v = ml[s * rows];
-        total += (top == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(v.x - top)) * v.y;
+        total += (top == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(v.x - top)) *
+                 (exact != nullptr ? exact[s * rows] : v.y);
     }
     return f32x2{top, wave_sum(total)};
 }
@@ -395,7 +426,7 @@ __global__ __launch_bounds__(kFoldWaves *kWave) void kv_fold_kernel(const float 
         if (tg * kFoldThreads >= length) return;
         for (uint32_t r = wave; r < in_head; r += kFoldWaves) {
             const size_t row = head * in_head + r;
-            const f32x2 ml = r % a.n < a.count.n[b] ? fold_ml(a.part_ml + row, a.parts, a.rows, lane)
+            const f32x2 ml = r % a.n < a.count.n[b] ? fold_ml(a.part_ml + row, a.part_exact + row, a.parts, a.rows, lane)
                                                     : f32x2{-__builtin_inff(), 0.0f};
             if (lane == 0) lds_ml[r] = weight_terms(ml.x, ml.y);
         }
@@ -438,7 +469,7 @@ __global__ __launch_bounds__(kFoldWaves *kWave) void kv_fold_kernel(const float 
     // a row of padding has no parts: what is there is read, and not used
     const uint32_t b = of_pairs / (in_head * c.heads);
     const bool there = of_pairs % n < a.count.n[b];
-    const f32x2 all = fold_ml(part_ml + row, parts, rows, lane);
+    const f32x2 all = fold_ml(part_ml + row, nullptr, parts, rows, lane);
     auto weight = [&](float m) { return all.x == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - all.x); };
 #pragma unroll
     for (uint32_t k = 0; k < kHeld; ++k)
@@ -454,7 +485,10 @@ __global__ __launch_bounds__(kFoldWaves *kWave) void kv_fold_kernel(const float 
     }
     if (!there) return;
     store_out(a.out + row * vdim, vdim, d, finish(v, all.x, all.y));
-    if (a.row_ml != nullptr && lane == 0) a.row_ml[row] = weight_terms(all.x, all.y);
+    if (a.row_ml != nullptr) {
+        const f32x2 whole = fold_ml(part_ml + row, a.part_exact + row, parts, rows, lane);
+        if (lane == 0) a.row_ml[row] = weight_terms(whole.x, whole.y);
+    }
 }
 
 // ---- plan and launch ---------------------------------------------------------------
@@ -464,8 +498,8 @@ struct Plan {
     bool scores;   // the weights come from scores that the rows kernel stores
     uint32_t row_groups, parts, row_parts;
     size_t rows, score_stride;
-    size_t o_bytes, ml_bytes, row_bytes, score_bytes, partial_bytes;
-    size_t bytes() const { return o_bytes + ml_bytes + row_bytes + score_bytes + partial_bytes; }
+    size_t o_bytes, ml_bytes, exact_bytes, row_bytes, score_bytes, partial_bytes;
+    size_t bytes() const { return o_bytes + ml_bytes + exact_bytes + row_bytes + score_bytes + partial_bytes; }
 };
 
 size_t whole256(size_t bytes) { return (bytes + 255) / 256 * 256; }
@@ -506,6 +540,7 @@ Plan plan_of(bool f32, const View &c, const AttentionShape &a) {
     p.scores = a.weights != nullptr && in_head <= kRows;
     p.score_stride = (size_t)blocks * kTokens;
     p.ml_bytes = p.parts > 1 || p.scores ? whole256(p.parts * p.rows * sizeof(f32x2)) : 0;
+    p.exact_bytes = a.weights != nullptr ? whole256(p.parts * p.rows * sizeof(float)) : 0;
     p.row_bytes = a.weights != nullptr && !p.scores ? whole256(p.rows * sizeof(f32x2)) : 0;
     p.score_bytes = p.scores ? whole256(p.rows * p.score_stride * 4) : 0;
     p.row_parts = 1;
@@ -593,6 +628,7 @@ hipError_t run(const View &c, const AttentionShape &sh, const void *query, void 
     };
     a.part_o = reinterpret_cast<float *>(take(p.o_bytes));
     a.part_ml = reinterpret_cast<f32x2 *>(take(p.ml_bytes));
+    a.part_exact = reinterpret_cast<float *>(take(p.exact_bytes));
     a.row_ml = reinterpret_cast<f32x2 *>(take(p.row_bytes));
     a.scores = reinterpret_cast<float *>(take(p.score_bytes));
     float *const partial = reinterpret_cast<float *>(take(p.partial_bytes));

@@ -25,12 +25,12 @@ typedef float float16v __attribute__((ext_vector_type(16)));
 
 constexpr float kTiny = 1.1754944e-38f, kHuge = 3.0e38f;
 
-// 32 query rows as B operands, one per 16 dims (f32: and their rest), times `sign`
+// 32 query rows as B operands, one per 16 dims and piece, times `sign`
 // (the scale's; 0 where the scale is).
 template <typename S, uint32_t P> struct TileQuery {
     static constexpr uint32_t kSteps = P / 16;
     static constexpr bool kPair = sizeof(S) == 4;
-    half8 hi[kSteps], lo[kPair ? kSteps : 1];
+    half8 piece[kPieces<S>][kSteps];
     float factor;   // the power of two that a f32 row was divided by
 
     __device__ inline void load(const S *row, uint32_t dim, uint32_t half, float sign) {
@@ -41,12 +41,12 @@ template <typename S, uint32_t P> struct TileQuery {
 #pragma unroll
                 for (uint32_t c = 0; c < kSteps; ++c) {
                     const uint32_t d = 16 * c + 8 * half;
-                    hi[c] = *reinterpret_cast<const half8 *>(row + (d < dim ? d : 0));
+                    piece[0][c] = *reinterpret_cast<const half8 *>(row + (d < dim ? d : 0));
                 }
 #pragma unroll
                 for (uint32_t c = 0; c < kSteps; ++c) {
-                    hi[c] *= s;
-                    if (16 * c + 8 * half >= dim) hi[c] = half8{};
+                    piece[0][c] *= s;
+                    if (16 * c + 8 * half >= dim) piece[0][c] = half8{};
                 }
             } else {
 #pragma unroll
@@ -54,7 +54,7 @@ template <typename S, uint32_t P> struct TileQuery {
 #pragma unroll
                     for (uint32_t e = 0; e < 8; ++e) {
                         const uint32_t d = 16 * c + 8 * half + e;
-                        hi[c][e] = d < dim ? row[d] * s : (_Float16)0.0f;
+                        piece[0][c][e] = d < dim ? row[d] * s : (_Float16)0.0f;
                     }
             }
         } else {
@@ -78,8 +78,7 @@ template <typename S, uint32_t P> struct TileQuery {
 #pragma unroll
                 for (uint32_t e = 0; e < 8; ++e) {
                     const float y = usable ? __builtin_ldexpf(x[c][e], 14 - exponent) : 0.0f;
-                    hi[c][e] = (_Float16)y;
-                    lo[c][e] = (_Float16)(y - (float)hi[c][e]);
+                    pieces_of(y, piece[0][c], piece[1][c], piece[2][c], e);
                 }
         }
     }
@@ -88,10 +87,10 @@ template <typename S, uint32_t P> struct TileQuery {
 // A block's factor of raw products, positive (queries carry the scale's sign), and,
 // for f32, what rounding took off it. A block of zero keys has raw products 0: any
 // factor.
-template <typename S> __device__ inline f32x2 block_factor(float k_scale, double scale2) {
+template <typename S, bool kExact> __device__ inline f32x2 block_factor(float k_scale, double scale2) {
     const float k = k_scale == 0.0f ? 1.0f : k_scale;
     const double scale = scale2 == 0.0 ? 1.0 : fabs(scale2);
-    if constexpr (sizeof(S) == 2) {
+    if constexpr (sizeof(S) == 2 && !kExact) {
         return f32x2{fminf(fmaxf(k * (float)scale, kTiny), kHuge), 0.0f};
     } else {
         const double f = (double)k * scale;
@@ -139,9 +138,11 @@ __device__ inline void steps(R operand, M product, W work) {
 // P of tile s - 1 with its values while it takes the maxima of tile s and turns
 // codes to f16, then multiplies the keys of tile s + 1 while it takes the
 // exponentials of tile s.
-template <typename S, uint32_t P>
+// kExact: with the sum of P before its rounding to f16 too, for the weights.
+template <typename S, uint32_t P, bool kExact>
 __global__ __launch_bounds__(kThreads, sizeof(S) == 2 && P <= 128 ? 2 : 1) void kv_tiles_kernel(Args<S> a) {
     constexpr bool kPair = sizeof(S) == 4;
+    static_assert(!kPair || !kExact);   // (its sum is exact by itself)
     constexpr uint32_t KC = P / 16, VT = (P + 31) / 32;
     constexpr uint32_t KROW = P + 8, VROW = kTokens + 8;   // LDS rows, halves
     constexpr uint32_t KTILE = kTokens * KROW, VTILE = VT * 32 * VROW;
@@ -253,21 +254,38 @@ __global__ __launch_bounds__(kThreads, sizeof(S) == 2 && P <= 128 ? 2 : 1) void 
         ph[ch] = half8{};
         if constexpr (kPair) pl[ch] = half8{};
     }
-    float big = neg_inf, sum = 0.0f, unit = 1.0f;   // (sum: of the lane's keys)
-    constexpr uint32_t NS = 2 * KC, NO = 4 * VT;   // matrix steps of a tile's scores and outputs
+    float big = neg_inf, sum = 0.0f, exact = 0.0f, unit = 1.0f;   // (sums of the lane's keys)
+    // matrix steps of a tile's scores (piece by piece) and outputs (f32: P's rests first)
+    constexpr uint32_t NS1 = 2 * KC, NO1 = 4 * VT, NS = kPieces<S> * NS1, NO = kPair ? 2 * NO1 : NO1;
+    float16v fresh[kPair ? VT : 1];   // f32: a tile's outputs
     auto key_operand = [&](uint32_t buf, uint32_t i) {
+        i %= NS1;
         return *reinterpret_cast<const half8 *>(&ks[buf][(32 * (i % 2) + swap23(col)) * KROW + 16 * (i / 2) + 8 * half]);
     };
     auto value_operand = [&](uint32_t buf, uint32_t i) {
+        i %= NO1;
         return *reinterpret_cast<const half8 *>(&vs[buf][(32 * (i % VT) + col) * VROW + 16 * (i / VT) + 8 * half]);
     };
     auto score = [&](float16v (&to)[2], uint32_t i, half8 k) {
-        to[i % 2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q.hi[i / 2], to[i % 2], 0, 0, 0);
-        if constexpr (kPair) to[i % 2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q.lo[i / 2], to[i % 2], 0, 0, 0);
+        to[i % 2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q.piece[i / NS1][i % NS1 / 2], to[i % 2], 0, 0, 0);
     };
     auto output = [&](uint32_t i, half8 v) {
-        o[i % VT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, ph[i / VT], o[i % VT], 0, 0, 0);
-        if constexpr (kPair) o[i % VT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pl[i / VT], o[i % VT], 0, 0, 0);
+        const bool rest = kPair && i < NO1;
+        const half8 x = rest ? pl[kPair ? i % NO1 / VT : 0] : ph[i % NO1 / VT];
+        float16v &to = kPair ? fresh[kPair ? i % VT : 0] : o[i % VT];
+        to = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, x, to, 0, 0, 0);
+    };
+    auto clear_fresh = [&] {
+        if constexpr (kPair)
+#pragma unroll
+            for (uint32_t t = 0; t < VT; ++t)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) fresh[t][e] = 0.0f;
+    };
+    auto add_fresh = [&] {
+        if constexpr (kPair)
+#pragma unroll
+            for (uint32_t t = 0; t < VT; ++t) o[t] += fresh[t];
     };
     auto clear = [](float16v (&to)[2]) {
 #pragma unroll
@@ -331,9 +349,10 @@ __global__ __launch_bounds__(kThreads, sizeof(S) == 2 && P <= 128 ? 2 : 1) void 
                 now[e / 16][e % 16] = (int)key >= last ? neg_inf : x;
             }
         }
-        const f32x2 f2 = block_factor<S>(m.k_scale, a.scale2);
+        const f32x2 f2 = block_factor<S, kExact>(m.k_scale, a.scale2);
         const float factor = f2.x * q.factor;
         float part_max[4] = {neg_inf, neg_inf, neg_inf, neg_inf};
+        clear_fresh();
         steps<NO>([&](uint32_t i) { return value_operand((s + 1) & 1, i); }, [&](uint32_t i, half8 v) { output(i, v); },
                   [&](uint32_t i) {
 #pragma unroll
@@ -342,6 +361,7 @@ __global__ __launch_bounds__(kThreads, sizeof(S) == 2 && P <= 128 ? 2 : 1) void 
                       for (uint32_t e = i * 32 / NO; e < (i + 1) * 32 / NO; ++e)
                           part_max[e % 4] = fmaxf(part_max[e % 4], now[e / 16][e % 16]);
                   });
+        add_fresh();
         const float raw = fmaxf(fmaxf(part_max[0], part_max[1]), fmaxf(part_max[2], part_max[3]));
         next_meta = take_meta(s + 1);
         fetch_meta(s + 2);
@@ -352,6 +372,7 @@ __global__ __launch_bounds__(kThreads, sizeof(S) == 2 && P <= 128 ? 2 : 1) void 
             const float up = flash::pair_max(fmaxf(top, big));
             const float alpha = up == neg_inf ? 1.0f : __builtin_amdgcn_exp2f(big - up);
             sum *= alpha;
+            exact *= alpha;
 #pragma unroll
             for (uint32_t v = 0; v < VT; ++v) o[v] *= alpha;
             big = up;
@@ -366,9 +387,13 @@ __global__ __launch_bounds__(kThreads, sizeof(S) == 2 && P <= 128 ? 2 : 1) void 
             inverse_unit = 1.0f / unit;
             ratio = 1.0f;
         }
-        // exponents are relative to this; with nothing seen every score is -inf or NaN
-        const float base = (big == neg_inf ? 0.0f : big - kHeadroom<S>) - __builtin_amdgcn_logf(ratio);
-        float add[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        // exponents are relative to this; with nothing seen every score is -inf or NaN.
+        // The ratio is an addend of the exponent where f16's P is all that comes of it.
+        constexpr bool kInExponent = !kPair && !kExact;
+        const float base = (big == neg_inf ? 0.0f : big - kHeadroom<S>) -
+                           (kInExponent ? __builtin_amdgcn_logf(ratio) : 0.0f);
+        const float to_p = ratio * kPairScale<S>;
+        float add[4] = {0.0f, 0.0f, 0.0f, 0.0f}, add_exact = 0.0f;
         clear(ahead);
         // (after the last tile: the scores of an old one, not used)
         steps<NS>([&](uint32_t i) { return key_operand((s + 1) & 1, i); }, [&](uint32_t i, half8 k) { score(ahead, i, k); },
@@ -382,23 +407,28 @@ __global__ __launch_bounds__(kThreads, sizeof(S) == 2 && P <= 128 ? 2 : 1) void 
                               x += fabsf(off) < 1.0f ? off : 0.0f;   // (not for -inf)
                           }
                           x = __builtin_amdgcn_exp2f(x);
-                          ph[e / 8][e % 8] = (_Float16)x;
-                          if constexpr (kPair) {
-                              pl[e / 8][e % 8] = (_Float16)(x - (float)ph[e / 8][e % 8]);
-                              add[e % 4] += x;
-                          } else if (e % 2 == 1) {   // the sum of P as the product has it
+                          if constexpr (kExact) add_exact += x;
+                          if constexpr (kPair) add[e % 4] += x;
+                          float y = kInExponent ? x : x * to_p;
+                          if constexpr (kPair) asm volatile("" : "+v"(y));   // (one f32 for both its f16s)
+                          ph[e / 8][e % 8] = (_Float16)y;
+                          if constexpr (kPair) pl[e / 8][e % 8] = (_Float16)(y - (float)ph[e / 8][e % 8]);
+                          if (!kPair && e % 2 == 1) {   // the sum of P as the product has it
                               const half2_t ones = {(_Float16)1.0f, (_Float16)1.0f};
-                              add[e / 2 % 4] = __builtin_amdgcn_fdot2(half2_t{ph[e / 8][e % 8 - 1], ph[e / 8][e % 8]}, ones,
-                                                                      add[e / 2 % 4], false);
+                              float &to = add[kExact ? 0 : e / 2 % 4];   // (registers are short)
+                              to = __builtin_amdgcn_fdot2(half2_t{ph[e / 8][e % 8 - 1], ph[e / 8][e % 8]}, ones,
+                                                          to, false);
                           }
                           // (taken here, not moved to where it is used)
                           if (e % 8 == 7) {
                               asm volatile("" : "+v"(ph[e / 8]));
                               if constexpr (kPair) asm volatile("" : "+v"(pl[e / 8]));
+                              if constexpr (kExact) asm volatile("" : "+v"(add_exact));
                           }
                       }
                   });
-        sum += ((add[0] + add[1]) + (add[2] + add[3])) * fast_rcp(ratio);
+        sum += ((add[0] + add[1]) + (add[2] + add[3])) * (kPair ? 1.0f : fast_rcp(ratio));
+        if constexpr (kExact) exact += add_exact;
     };
     float16v other[2];
     for (uint32_t s = 0; s < tiles; s += 2) {   // (two score tiles in turn: no copies)
@@ -414,9 +444,12 @@ __global__ __launch_bounds__(kThreads, sizeof(S) == 2 && P <= 128 ? 2 : 1) void 
         if (s + 1 < tiles) turn(s + 1, other, st);
     }
     __syncthreads();
+    clear_fresh();
     steps<NO>([&](uint32_t i) { return value_operand((tiles + 1) & 1, i); }, [&](uint32_t i, half8 v) { output(i, v); },
               [](uint32_t) {});
+    add_fresh();
     sum = flash::pair_sum(sum);
+    exact = kExact ? flash::pair_sum(exact) : sum;
     big -= kHeadroom<S>;
     if (!live) return;
     const bool direct = a.parts == 1;
@@ -424,14 +457,18 @@ __global__ __launch_bounds__(kThreads, sizeof(S) == 2 && P <= 128 ? 2 : 1) void 
     for (uint32_t v = 0; v < VT; ++v)
 #pragma unroll
         for (uint32_t e = 0; e < 4; ++e) {
-            const f32x4 x = f32x4{o[v][4 * e], o[v][4 * e + 1], o[v][4 * e + 2], o[v][4 * e + 3]} * unit;
+            const f32x4 x = f32x4{o[v][4 * e], o[v][4 * e + 1], o[v][4 * e + 2], o[v][4 * e + 3]} * (unit / kPairScale<S>);
             const uint32_t d = 32 * v + 8 * e + 4 * half;
             if (direct) store_out(a.out + row * c.vdim, c.vdim, d, finish(x, big, sum));
             else store_out(a.part_o + ((size_t)part * a.rows + row) * c.vdim, c.vdim, d, x);
         }
     if (half != 0) return;
-    if (!direct) a.part_ml[(size_t)part * a.rows + row] = f32x2{big, sum};
-    else if (a.row_ml != nullptr) a.row_ml[row] = weight_terms(big, sum);
+    if (!direct) {
+        a.part_ml[(size_t)part * a.rows + row] = f32x2{big, sum};
+        if (a.part_exact != nullptr) a.part_exact[(size_t)part * a.rows + row] = exact;
+    } else if (a.row_ml != nullptr) {
+        a.row_ml[row] = weight_terms(big, exact);
+    }
 }
 
 // Softmax weights of four blocks' tokens, a wave each, summed over the rows that
@@ -446,7 +483,7 @@ __global__ __launch_bounds__(kThreads, P <= 64 ? 3 : P <= 128 ? 2 : 1) void kv_w
     constexpr bool kPair = sizeof(S) == 4;
     constexpr uint32_t KC = P / 16, QROW = P + 8, kStep = 32;
     constexpr uint32_t G = (P / 8 + 7) / 8;   // groups of 8 dims of a thread: 8 threads stage a row
-    __shared__ __attribute__((aligned(16))) _Float16 qs[2][kPair ? 2 : 1][kStep * QROW];
+    __shared__ __attribute__((aligned(16))) _Float16 qs[2][kPieces<S>][kStep * QROW];
     __shared__ f32x4 terms[2][kStep];         // of a row: maximum, 1 / sum (0: adds nothing), factor
     const View &c = a.c;
     const uint32_t tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
@@ -475,7 +512,7 @@ __global__ __launch_bounds__(kThreads, P <= 64 ? 3 : P <= 128 ? 2 : 1) void kv_w
             }
         }
     const float sign = a.scale2 > 0.0 ? 1.0f : a.scale2 < 0.0 ? -1.0f : 0.0f;
-    const float k_factor = block_factor<S>(open ? 1.0f : meta.k_scale, a.scale2).x;
+    const float k_factor = block_factor<S, true>(open ? 1.0f : meta.k_scale, a.scale2).x;
     float acc[32];
 #pragma unroll
     for (int e = 0; e < 32; ++e) acc[e] = 0.0f;
@@ -540,18 +577,14 @@ __global__ __launch_bounds__(kThreads, P <= 64 ? 3 : P <= 128 ? 2 : 1) void kv_w
             factor = __builtin_ldexpf(1.0f, exponent - 14);
 #pragma unroll
             for (uint32_t g = 0; g < G; ++g) {
-                half8 hi, lo;
+                half8 piece[3];
 #pragma unroll
-                for (uint32_t e = 0; e < 8; ++e) {
-                    const float y = __builtin_ldexpf(x[g][e], 14 - exponent);
-                    hi[e] = (_Float16)y;
-                    lo[e] = (_Float16)(y - (float)hi[e]);
-                }
+                for (uint32_t e = 0; e < 8; ++e)
+                    pieces_of(__builtin_ldexpf(x[g][e], 14 - exponent), piece[0], piece[1], piece[2], e);
                 const uint32_t d = (sub + 8 * g) * 8;
-                if (d < P) {
-                    *reinterpret_cast<half8 *>(&qs[buf][0][srow * QROW + d]) = hi;
-                    *reinterpret_cast<half8 *>(&qs[buf][1][srow * QROW + d]) = lo;
-                }
+                if (d < P)
+#pragma unroll
+                    for (uint32_t i = 0; i < 3; ++i) *reinterpret_cast<half8 *>(&qs[buf][i][srow * QROW + d]) = piece[i];
             }
         } else {
 #pragma unroll
@@ -586,18 +619,14 @@ __global__ __launch_bounds__(kThreads, P <= 64 ? 3 : P <= 128 ? 2 : 1) void kv_w
 #pragma unroll
                 for (int e = 0; e < 16; ++e) st[s][e] = 0.0f;
 #pragma unroll
-            for (uint32_t ch = 0; ch < KC; ++ch) {
-                const half8 hi = *reinterpret_cast<const half8 *>(&qs[buf][0][col * QROW + 16 * ch + 8 * half]);
+            for (uint32_t i = 0; i < kPieces<S>; ++i)
 #pragma unroll
-                for (uint32_t s = 0; s < 2; ++s)
-                    st[s] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[s][ch], hi, st[s], 0, 0, 0);
-                if constexpr (kPair) {
-                    const half8 lo = *reinterpret_cast<const half8 *>(&qs[buf][1][col * QROW + 16 * ch + 8 * half]);
+                for (uint32_t ch = 0; ch < KC; ++ch) {
+                    const half8 x = *reinterpret_cast<const half8 *>(&qs[buf][i][col * QROW + 16 * ch + 8 * half]);
 #pragma unroll
                     for (uint32_t s = 0; s < 2; ++s)
-                        st[s] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[s][ch], lo, st[s], 0, 0, 0);
+                        st[s] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k[s][ch], x, st[s], 0, 0, 0);
                 }
-            }
             if (wave_any(live && seen < (int)(t * kTokens + kTokens)) || meta.marked != 0) {
                 const int last = seen - (int)(t * kTokens);
                 const uint32_t mine = marks_of(meta.marked, half);
@@ -655,7 +684,14 @@ __global__ __launch_bounds__(kThreads) void kv_weights_add_kernel(Args<S> a, uin
 
 template <typename S, uint32_t P>
 hipError_t tiles(const Args<S> &a, uint32_t groups, hipStream_t s) {
-    kv_tiles_kernel<S, P><<<groups * a.pairs * a.parts, kThreads, 0, s>>>(a);
+    const dim3 grid(groups * a.pairs * a.parts);
+    if constexpr (sizeof(S) == 2) {
+        if (a.weights != nullptr) {
+            kv_tiles_kernel<S, P, true><<<grid, kThreads, 0, s>>>(a);
+            return hipGetLastError();
+        }
+    }
+    kv_tiles_kernel<S, P, false><<<grid, kThreads, 0, s>>>(a);
     return hipGetLastError();
 }
 

@@ -20,13 +20,16 @@ constexpr uint32_t kWaves = 4;
 constexpr uint32_t kRows = 16;         // packed rows of a wave
 constexpr double kLog2e = 1.4426950408889634;
 constexpr float kUnitRange = 8.0f;     // a value scale further from the unit moves it
-// P of a row whose maximum is M is 2^(s - M + kHeadroom): as far up in f16 as the
-// unit's range and the lazy rescale of the maximum (by more than 2^kLazy) leave
-// room for, 2^15 in all, so that small weights keep their bits: absolute
-// errors of P, relative to the row's largest, are below 2^-26 (f16; P is rounded
-// to 2^-11 anyway) and 2^-34 (f32, whose maximum is never left behind).
+// f16: P of a row whose maximum is M is 2^(s - M + kHeadroom): as far up as the unit's
+// range and the lazy rescale of the maximum (by more than 2^kLazy) leave room for, 2^15
+// in all, so that small weights keep their bits: absolute errors of P, relative to the
+// row's largest, are below 2^-26 (P is rounded to 2^-11 anyway). f32, whose maximum
+// is never left behind: the weight 2^(s - M), with its exponent near 0 for the largest
+// ones, times kPairScale; errors below 2^-34.
 template <typename S> constexpr float kLazy = sizeof(S) == 4 ? 0.0f : 8.0f;
-template <typename S> constexpr float kHeadroom = sizeof(S) == 4 ? 12.0f : 4.0f;
+template <typename S> constexpr float kHeadroom = sizeof(S) == 4 ? 0.0f : 4.0f;
+template <typename S> constexpr float kPairScale = sizeof(S) == 4 ? 4096.0f : 1.0f;
+
 // Arguments of a launch over sequences first .. (pairs / heads of them).
 template <typename S> struct Args {
     View c;
@@ -34,6 +37,7 @@ template <typename S> struct Args {
     S *out;
     float *part_o;       // [part][row][vdim], rows of all sequences
     f32x2 *part_ml;      // [part][row] running maximum (log2 units) and sum
+    float *part_exact;   // [part][row] sum of the weights before P's rounding, or null
     f32x2 *row_ml;       // [row] maximum and 1 / sum (0: the row adds no weight), or null
     float *weights;
     float *scores;       // [row][score_stride] scores in log2 units, or null
@@ -64,6 +68,22 @@ __device__ inline half8 codes(uint32_t a, uint32_t b) {
     r[2] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(one, b, 0x04010400u)) - bias);
     r[3] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2_t, __builtin_amdgcn_perm(one, b, 0x04030402u)) - bias);
     return __builtin_bit_cast(half8, r);
+}
+
+// Element e of a query row as f16 operands: an f16 one as it is. An f32 one (|x| <
+// 2^14) as three that add up to it to 2^-21 and 2^-33 of it or better, the last a multiple
+// of 8. An MFMA cuts its products off at 2^-24 or so of the largest one, and with a
+// pair (x rounded to f16, and the rest) f32 attention was off by 2e-6, twice as far as its
+// plain f32 form. Multiples of one power of two, 11 bits of them, times codes add up
+// exactly, and what is cut off the small parts' products does not count: 5e-7. The
+// small parts' products come first.
+template <typename S> constexpr uint32_t kPieces = sizeof(S) == 4 ? 3 : 1;
+__device__ inline void pieces_of(float x, half8 &p0, half8 &p1, half8 &p2, uint32_t e) {
+    constexpr float kEights = 1.5f * 0x1p26f;   // its f32 neighbours are 8 apart
+    const float most = (x + kEights) - kEights, rest = x - most;
+    p2[e] = (_Float16)most;
+    p1[e] = (_Float16)rest;
+    p0[e] = (_Float16)(rest - (float)p1[e]);
 }
 
 // How many keys packed row r sees (0 or fewer: none); padded rows and rows past

@@ -134,7 +134,7 @@ class Model:
         in `out` and to be compared apart.
 
         Tolerances, from the roundings that the kernels make (u = 2^-24):
-          scores   s = sum of dim products: each add rounds, and the f32 q pair, the
+          scores   s = sum of dim products: each add rounds, and the f32 q's pieces, the
                    block factor and the scaling round: at most (dim + 16) u times
                    A = scale * sum |q k|; it enters p = exp(s - max) as a relative
                    error, for the row's own p and for its sum;
@@ -189,7 +189,6 @@ class Model:
                     t = (rel + 2.0 ** -21) * mass + 4 * u * np.abs(o) + 2.0 ** -34 * in_sight / total + 1e-40
                 tol[b, j, :count][plain] = t
                 weights[b, h, :length] += p.sum(0)
-                # (f16: the sum is that of the rounded P)
-                w = rel + 16 * u + (2.0 ** -11 + 2.0 ** -26 * n_seen / total if half else 0)
+                w = rel + 16 * u   # (f16 too: these go by the sum before P's rounding)
                 wtol[b, h, :length] += (w * p).sum(0)
         return out, tol, weights, wtol
