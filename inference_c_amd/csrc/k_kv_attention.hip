@@ -508,11 +508,12 @@ uint32_t widest_of(const View &c) { return c.kp > c.vp ? c.kp : c.vp; }
 // Products of a call from which the kernel of 128-row tiles is used: it reads each
 // operand for twice the rows and takes each code to f16 once for 128, but a
 // workgroup's turn lasts long. Measured (us, rows kernel and tiles, causal): f16 D 128,
-// 8 heads x 512 rows x 2000 keys (1.0e9) 22 and 29, 8 x 384 x 8000 (3.1e9) 54 and 48,
-// 32 x 512 x 8000 175 and 89; D 64, 32 x 384 x 2000 (1.6e9) 23 and 38, 32 x 256 x 8000
-// (4.2e9) 52 and 43; f32 D 80, 8 x 1024 x 8000 (5.2e9) 86 and 94, 8 x 2048 x 8000
-// (1.0e10) 160 and 133.
-constexpr double kTileProducts = 2.6e9, kTileProductsF32 = 7.0e9;
+// 8 heads x 512 rows x 2000 keys (1.0e9) 22 and 30, 8 x 384 x 8000 (3.1e9) 54 and 48,
+// 32 x 512 x 8000 175 and 90; D 64, 32 x 384 x 2000 (1.6e9) 23 and 38, 32 x 256 x 8000
+// (4.2e9) 53 and 43; D 256, 8 x 512 x 2000 (1.8e9) 50 and 42; f32 D 80, 32 x 512 x 2000
+// (2.3e9) 58 and 63, 32 x 1024 x 2000 (3.9e9) 102 and 87; D 128, 32 x 256 x 2000
+// (2.0e9) 44 and 52, 8 x 512 x 8000 (4.1e9) 72 and 74, 32 x 512 x 8000 226 and 201.
+constexpr double kTileProducts = 2.6e9, kTileProductsF32 = 3.5e9;
 constexpr uint32_t kWorkgroups = 512;   // two for every CU
 
 Plan plan_of(bool f32, const View &c, const AttentionShape &a) {
@@ -526,10 +527,12 @@ Plan plan_of(bool f32, const View &c, const AttentionShape &a) {
     p.tiles = products >= (f32 ? kTileProductsF32 : kTileProducts) && tiles_fit(f32, widest_of(c));
     const uint32_t rows_each = p.tiles ? kTileRows : kRows;
     p.row_groups = (in_head + rows_each - 1) / rows_each;
-    // parts: workgroups for every CU twice over, with a block for each wave (tiles:
-    // four blocks) at least
+    // parts: workgroups for every CU twice over (tiles of which a CU holds one: once;
+    // f32 D 128, 8 heads x 512 rows x 8000 keys 74 us, twice over 87), with a block for
+    // each wave (tiles: four blocks) at least
     const uint64_t base = pairs * p.row_groups;
-    uint64_t parts = base >= kWorkgroups ? 1 : kWorkgroups / base;
+    const uint32_t fill = p.tiles && !tiles_twice(f32, widest_of(c)) ? kWorkgroups / 2 : kWorkgroups;
+    uint64_t parts = base >= fill ? 1 : fill / base;
     const uint32_t most = (blocks + kWaves - 1) / kWaves;
     parts = parts < most ? parts : most;
     p.parts = parts < 1 ? 1 : (uint32_t)parts;

@@ -140,7 +140,7 @@ __device__ inline void steps(R operand, M product, W work) {
 // exponentials of tile s.
 // kExact: with the sum of P before its rounding to f16 too, for the weights.
 template <typename S, uint32_t P, bool kExact>
-__global__ __launch_bounds__(kThreads, sizeof(S) == 2 && P <= 128 ? 2 : 1) void kv_tiles_kernel(Args<S> a) {
+__global__ __launch_bounds__(kThreads, tiles_twice(sizeof(S) == 4, P) ? 2 : 1) void kv_tiles_kernel(Args<S> a) {
     constexpr bool kPair = sizeof(S) == 4;
     static_assert(!kPair || !kExact);   // (its sum is exact by itself)
     constexpr uint32_t KC = P / 16, VT = (P + 31) / 32;

@@ -121,6 +121,8 @@ __device__ inline f32x2 weight_terms(float big, float total) {
 // the wider of the padded dims. False where no such kernel is built.
 constexpr uint32_t kTileRows = 128;
 bool tiles_fit(bool f32, uint32_t widest);
+// Whether a CU holds two of its workgroups (their registers decide).
+constexpr bool tiles_twice(bool f32, uint32_t widest) { return !f32 && widest <= 128; }
 template <typename S>
 hipError_t launch_tiles(const Args<S> &a, uint32_t widest, uint32_t groups, hipStream_t s);
 // Weights from the rows' maxima and sums; row_parts > 1: `partial` holds row_parts
