@@ -7,9 +7,9 @@
  * scale: with a the largest |x| of the block, x being the appended elements
  * rounded to f16,
  *     scale = a / 127,   code = 127 x / a rounded to nearest, ties to even,
- * and stand for the f32 product code * scale. The tokens of the last, partial block are held
- * in f16 until the block is full, so what a cache holds does not depend on
- * how its tokens were split over calls.
+ * and stand for the f32 product code * scale. The tokens of the last, partial
+ * block are held in f16 until the block is full, so what a cache holds does not
+ * depend on how its tokens were split over calls.
  *
  * A token whose key or value holds, in some head, an element that is no
  * finite f16 (NaN, infinite, or an f32 of 65520 and more) is marked in that
@@ -51,7 +51,8 @@ extern "C" {
 typedef struct TensorKvCache TensorKvCache;
 
 /* An empty cache. head_dim (of keys) and value_dim: 1 to 256, any number;
-   capacity up to 2^29, batch up to 65535, kv_heads up to 4096. */
+   capacity up to 2^27, batch up to 65535, kv_heads up to 4096, and batch *
+   kv_heads * capacity (in whole blocks) up to 2^31. */
 int tensor_kv_cache_create(size_t batch, size_t kv_heads, size_t capacity,
                            size_t head_dim, size_t value_dim,
                            TensorKvCache **result, char *error,

@@ -11,9 +11,9 @@
 // Keys lie by token and values by dim because that is how the two matrix
 // products of attention read them: a lane's 16 bytes of k are 16 dims of one
 // key, its 16 bytes of v 16 keys of one dim, and both go into MFMA operands as
-// they come. The arrays are set to zeros (codes: 0) at creation, columns past
-// the dims stay that, and every f16 in kt and vt is finite, so rows and columns
-// past the data may be read (their products are dropped or meet zeros).
+// they come. Codes and f16 are zeros at creation, columns past the dims stay that,
+// and every f16 in kt and vt is finite, so rows and columns past the data may be
+// read: their products are dropped or meet zeros.
 #pragma once
 
 #include <hip/hip_runtime.h>

@@ -30,7 +30,10 @@ namespace {
 
 using Buf = const TensorBuffer *;
 
-constexpr size_t kMaxCapacity = size_t{1} << 29;
+// A launch has fewer than 2^32 threads in a dimension: one for each token (of all
+// sequences and heads: the fold's), or 32 for each of a head's (the weights': 16
+// parts of its blocks in fours, 256 threads each).
+constexpr size_t kMaxCapacity = size_t{1} << 27, kMaxTokens = size_t{1} << 31;
 constexpr size_t kMaxBatch = 65535, kMaxHeads = 4096;
 
 int fail(char *error, size_t capacity, const char *message) {
@@ -40,14 +43,15 @@ int fail(char *error, size_t capacity, const char *message) {
 
 size_t round_up(size_t n, size_t to) { return (n + to - 1) / to * to; }
 
-// Sizes of the cache's arrays one after another, or false where they overflow.
+// Sizes of the cache's arrays one after another, or false where there are too many
+// tokens.
 struct Layout {
     size_t k, v, meta, kt, vt, length, total;
 };
 bool layout_of(size_t batch, size_t heads, size_t blocks, size_t kp, size_t vp, Layout *l) {
     const size_t pairs = batch * heads;   // below 2^28
-    if (blocks > SIZE_MAX / kv::kTokens / kv::kMaxDim / 8 / pairs) return false;
     const size_t tokens = pairs * blocks * kv::kTokens;
+    if (tokens > kMaxTokens) return false;
     l->k = 0;
     l->v = l->k + round_up(tokens * kp, 256);
     l->meta = l->v + round_up(tokens * vp, 256);
@@ -117,6 +121,7 @@ int append(TensorDType dtype, TensorKvCache *c, Buf key, Buf value, const uint32
             return 0;
         }
     }
+    if (n > INT_MAX) return fail(error, capacity, "cache append: too many tokens");
     if (n == 0) return 1;
     if (!sdk_ready(error, capacity) || !not_recording("cache append", error, capacity)) return 0;
     for (size_t first = 0; first < c->batch; first += kv::kBatchPerLaunch) {
@@ -151,6 +156,7 @@ int read(TensorDType dtype, const TensorKvCache *c, TensorBuffer *key, TensorBuf
     TensorKvCache *const held = const_cast<TensorKvCache *>(c);
     std::lock_guard<std::mutex> lock(held->mutex);
     if (rows < longest_of(c)) return fail(error, capacity, "cache read: fewer rows than the longest sequence has tokens");
+    if (rows > INT_MAX) return fail(error, capacity, "cache read: too many rows");
     if (rows == 0) return 1;
     if (!sdk_ready(error, capacity)) return 0;
     // a recorded call is replayed on later lengths: those the outputs have room for
@@ -215,12 +221,12 @@ int tensor_kv_cache_create(size_t batch, size_t kv_heads, size_t capacity, size_
     if (result == nullptr || batch == 0 || batch > kMaxBatch || kv_heads == 0 || kv_heads > kMaxHeads || capacity == 0 ||
         capacity > kMaxCapacity || head_dim == 0 || head_dim > kv::kMaxDim || value_dim == 0 || value_dim > kv::kMaxDim)
         return fail(error, error_capacity, "cache requires a result pointer, 1 to 65535 sequences, 1 to 4096 heads, 1 to "
-                    "2^29 tokens, and head and value dimensions of 1 to 256");
+                    "2^27 tokens, and head and value dimensions of 1 to 256");
     const size_t blocks = (capacity + kv::kTokens - 1) / kv::kTokens;
     const size_t kp = round_up(head_dim, 16), vp = round_up(value_dim, 16);
     Layout l;
     if (!layout_of(batch, kv_heads, blocks, kp, vp, &l))
-        return fail(error, error_capacity, "cache exceeds addressable size");
+        return fail(error, error_capacity, "cache requires at most 2^31 tokens (in whole blocks) of all sequences and heads together");
     if (!sdk_ready(error, error_capacity)) return 0;
     if (sdk_recording() != Recording::kNo)
         return fail(error, error_capacity, "a cache cannot be created while a graph is recorded");
@@ -232,13 +238,16 @@ int tensor_kv_cache_create(size_t batch, size_t kv_heads, size_t capacity, size_
         return fail(error, error_capacity, "out of memory creating cache");
     }
     char *memory = nullptr;
-    // zeros: a row or column past the data is finite wherever a kernel reads it
     if (!hip_ok(hipMalloc(reinterpret_cast<void **>(&memory), l.total), "cache: hipMalloc", error, error_capacity)) {
         delete c;
         std::free(length);
         return 0;
     }
-    if (!hip_ok(hipMemsetAsync(memory, 0, l.total, sdk_stream()), "cache: hipMemsetAsync", error, error_capacity)) {
+    // columns past the dims are codes of 0 and zeros: they count in no block's largest
+    // value, and meet a zero of q as what they are
+    if (!hip_ok(hipMemsetAsync(memory, 128, l.meta, sdk_stream()), "cache: hipMemsetAsync", error, error_capacity) ||
+        !hip_ok(hipMemsetAsync(memory + l.meta, 0, l.total - l.meta, sdk_stream()), "cache: hipMemsetAsync", error,
+                error_capacity)) {
         (void)hipFree(memory);
         delete c;
         std::free(length);

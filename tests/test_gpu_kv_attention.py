@@ -111,6 +111,15 @@ def test_tiles(sdk, shape, causal):
 
 
 @pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("shape", TILES[:3] + TILES[4:8] + TILES[9:], ids=str)
+def test_tiles_without_weights(sdk, shape, causal):
+    kv, heads, length, n, dim, vdim = shape
+    pair = Pair(sdk, 1, kv, length, dim, vdim, n + 1)
+    pair.append(length)
+    run(pair, "f16", heads, n, causal=causal, what="f16")
+
+
+@pytest.mark.parametrize("causal", [True, False])
 @pytest.mark.parametrize("shape", [(1, 2, 30000, 1001, 128, 128), (1, 2, 40010, 1000, 80, 96), (2, 2, 50000, 1150, 64, 60),
                                    (1, 4, 64000, 1000, 30, 17), (64, 64, 1700, 1024, 32, 32)], ids=str)
 def test_tiles_f32(sdk, shape, causal):
@@ -262,6 +271,22 @@ def test_scores_that_overflow(sdk):
     q[0, 0, 1] = 1e-3
     got, _ = attend(sdk, pair.cache, q, 1e6, False, vdim=16)
     assert (got[0, 0, 0] == 0).all() and np.isfinite(got).all() and got[0, 0, 1].any()
+
+
+@pytest.mark.parametrize("n", [1, 20])
+@pytest.mark.parametrize("dims", [(72, 72), (40, 24), (100, 33)], ids=str)
+def test_the_largest_keys_cut(sdk, dims, n):
+    """A cut block goes on in f16: columns past the dims stay zeros at any scale."""
+    pair = Pair(sdk, 1, 2, 200, *dims, seed=5)
+    k = pair.rng.uniform(-65504, 65504, (1, 2, 130, dims[0])).astype(np.float16)
+    k[0, :, 3, 0] = 65504
+    k[0, :, 70, 1] = -65504
+    v = pair.rng.uniform(-65504, 65504, (1, 2, 130, dims[1])).astype(np.float16)
+    v[0, :, 70, 0] = 65504
+    pair.append(130, key=k, value=v)
+    pair.truncate([100])
+    run(pair, "f32", 4, n, scale=1e-5, weighted=True)
+    run(pair, "f16", 4, n, scale=1e-5, weighted=True)
 
 
 def test_long_cache(sdk):

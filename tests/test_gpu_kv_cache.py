@@ -211,6 +211,32 @@ def test_evict(sdk, case, dims):
     check_read(sdk, target, model, "target cut")
 
 
+@pytest.mark.parametrize("dims", [(8, 8), (72, 72), (24, 120), (200, 136), (136, 64)], ids=str)
+def test_evict_of_odd_groups(sdk, dims):
+    """Rows of whole groups of 8 but not of 16: what is held past them is no value."""
+    pair = Pair(sdk, 2, 2, 500, *dims, seed=31)
+    pair.append(400, counts=[400, 333])
+    w = np.exp(pair.rng.standard_normal((2, 2, 400))).astype(np.float32)
+    target = sdk.kv_cache(2, 2, 200, *dims)
+    sdk.call("tensor_kv_cache_evict", pair.cache, sdk.from_numpy(w), 3, 20, 200, target, None, None)
+    pair.model, _ = pair.model.evict(w, 3, 20, 200)
+    pair.cache = target
+    pair.check(str(dims))
+    pair.truncate([150, 100])
+    pair.append(30)
+    pair.check("cut and appended to")
+
+
+def test_more_rows_than_an_int_are_refused(sdk):
+    cache = sdk.kv_cache(1, 1, 10, 1)
+    rows = sdk.tensor("f16", (1, 1, 2 ** 31, 1))
+    ok, message = sdk.try_call("tensor_kv_cache_append_f16", cache, rows, rows, u32s([1]))
+    assert ok == 0 and message == "cache append: too many tokens"
+    ok, message = sdk.try_call("tensor_kv_cache_read_f16", cache, rows, None)
+    assert ok == 0 and message == "cache read: too many rows"
+    rows.free()
+
+
 @pytest.mark.parametrize("length", [32768, 32769, 70001])
 def test_evict_of_long_sequences(sdk, length):
     """Around the length up to which the weights stay in registers."""

@@ -54,3 +54,12 @@ def test_a_missing_cache_is_refused(lib):
     assert lib.tensor_kv_cache_capacity(None) == 0
     assert lib.tensor_kv_cache_byte_length(None) == 0
     lib.tensor_kv_cache_free(None)
+
+
+@pytest.mark.parametrize("sizes", [(1, 1, 2 ** 27 + 1, 1, 1), (1, 17, 2 ** 27, 1, 1), (65535, 4096, 64, 1, 1),
+                                   (65535, 513, 1, 256, 256)])
+def test_create_refuses_too_many_tokens(lib, sizes):
+    ok, handle, message = create(lib, *sizes)
+    assert ok == 0 and handle is None
+    assert message.startswith("cache requires a result pointer" if sizes[2] > 2 ** 27 else
+                              "cache requires at most 2^31 tokens")
