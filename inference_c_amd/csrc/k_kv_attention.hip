@@ -79,9 +79,9 @@ template <typename S, uint32_t P> struct Query {
 #pragma unroll
             for (uint32_t s = 0; s < kSteps; ++s) {
                 const uint32_t d = step_dim<P>(s, g);
+                load8(row, dim, d, x[s]);
 #pragma unroll
                 for (uint32_t e = 0; e < 8; ++e) {
-                    x[s][e] = d + e < dim ? row[d + e] : 0.0f;
                     big = fmaxf(big, fabsf(x[s][e]));
                     finite = finite && __builtin_isfinite(x[s][e]);
                 }

@@ -61,11 +61,12 @@ template <typename S, uint32_t P> struct TileQuery {
             float x[kSteps][8], big = 0.0f;
             bool finite = true;
 #pragma unroll
+            for (uint32_t c = 0; c < kSteps; ++c) load8(row, dim, 16 * c + 8 * half, x[c]);
+#pragma unroll
             for (uint32_t c = 0; c < kSteps; ++c)
 #pragma unroll
                 for (uint32_t e = 0; e < 8; ++e) {
-                    const uint32_t d = 16 * c + 8 * half + e;
-                    x[c][e] = d < dim ? row[d] * sign : 0.0f;
+                    x[c][e] *= sign;
                     big = fmaxf(big, fabsf(x[c][e]));
                     finite = finite && __builtin_isfinite(x[c][e]);
                 }

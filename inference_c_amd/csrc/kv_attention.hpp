@@ -86,6 +86,23 @@ __device__ inline void pieces_of(float x, half8 &p0, half8 &p1, half8 &p2, uint3
     p0[e] = (_Float16)(rest - (float)p1[e]);
 }
 
+// Elements d .. d + 7 of an f32 row, zeros past its end (rows of whole fours are
+// asked for without a test).
+__device__ inline void load8(const float *row, uint32_t dim, uint32_t d, float (&x)[8]) {
+    if (dim % 4 == 0) {
+#pragma unroll
+        for (uint32_t i = 0; i < 8; i += 4) {
+            f32x4 v = *reinterpret_cast<const f32x4 *>(row + (d + i < dim ? d + i : 0));
+            if (d + i >= dim) v = f32x4{0, 0, 0, 0};
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) x[i + e] = v[e];
+        }
+    } else {
+#pragma unroll
+        for (uint32_t e = 0; e < 8; ++e) x[e] = d + e < dim ? row[d + e] : 0.0f;
+    }
+}
+
 // How many keys packed row r sees (0 or fewer: none); padded rows and rows past
 // the head see all.
 __device__ inline int seen_by(uint32_t i, bool live, uint32_t length, uint32_t count, int causal) {
