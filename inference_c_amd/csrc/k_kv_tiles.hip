@@ -276,6 +276,17 @@ __global__ __launch_bounds__(kThreads, tiles_twice(sizeof(S) == 4, P) ? 2 : 1) v
         float16v &to = kPair ? fresh[kPair ? i % VT : 0] : o[i % VT];
         to = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, x, to, 0, 0, 0);
     };
+    // f16: the sum of P as the product has it, beside that product
+    float add[4], inverse_ratio = 1.0f;
+    auto clear_add = [&] { add[0] = add[1] = add[2] = add[3] = 0.0f; };
+    auto add_p = [&](uint32_t i) {
+        if constexpr (!kPair)
+#pragma unroll
+            for (uint32_t e = i * 16 / NO; e < (i + 1) * 16 / NO; ++e) {
+                const half2_t two = {ph[e / 4][e % 4 * 2], ph[e / 4][e % 4 * 2 + 1]};
+                add[e % 4] = __builtin_amdgcn_fdot2(two, half2_t{(_Float16)1.0f, (_Float16)1.0f}, add[e % 4], false);
+            }
+    };
     auto clear_fresh = [&] {
         if constexpr (kPair)
 #pragma unroll
@@ -354,6 +365,7 @@ __global__ __launch_bounds__(kThreads, tiles_twice(sizeof(S) == 4, P) ? 2 : 1) v
         const float factor = f2.x * q.factor;
         float part_max[4] = {neg_inf, neg_inf, neg_inf, neg_inf};
         clear_fresh();
+        clear_add();
         steps<NO>([&](uint32_t i) { return value_operand((s + 1) & 1, i); }, [&](uint32_t i, half8 v) { output(i, v); },
                   [&](uint32_t i) {
 #pragma unroll
@@ -361,8 +373,10 @@ __global__ __launch_bounds__(kThreads, tiles_twice(sizeof(S) == 4, P) ? 2 : 1) v
 #pragma unroll
                       for (uint32_t e = i * 32 / NO; e < (i + 1) * 32 / NO; ++e)
                           part_max[e % 4] = fmaxf(part_max[e % 4], now[e / 16][e % 16]);
+                      add_p(i);
                   });
         add_fresh();
+        if constexpr (!kPair) sum += ((add[0] + add[1]) + (add[2] + add[3])) * inverse_ratio;
         const float raw = fmaxf(fmaxf(part_max[0], part_max[1]), fmaxf(part_max[2], part_max[3]));
         next_meta = take_meta(s + 1);
         fetch_meta(s + 2);
@@ -394,7 +408,8 @@ __global__ __launch_bounds__(kThreads, tiles_twice(sizeof(S) == 4, P) ? 2 : 1) v
         const float base = (big == neg_inf ? 0.0f : big - kHeadroom<S>) -
                            (kInExponent ? __builtin_amdgcn_logf(ratio) : 0.0f);
         const float to_p = ratio * kPairScale<S>;
-        float add[4] = {0.0f, 0.0f, 0.0f, 0.0f}, add_exact = 0.0f;
+        float add_exact = 0.0f;
+        clear_add();
         clear(ahead);
         // (after the last tile: the scores of an old one, not used)
         steps<NS>([&](uint32_t i) { return key_operand((s + 1) & 1, i); }, [&](uint32_t i, half8 k) { score(ahead, i, k); },
@@ -414,12 +429,6 @@ __global__ __launch_bounds__(kThreads, tiles_twice(sizeof(S) == 4, P) ? 2 : 1) v
                           if constexpr (kPair) asm volatile("" : "+v"(y));   // (one f32 for both its f16s)
                           ph[e / 8][e % 8] = (_Float16)y;
                           if constexpr (kPair) pl[e / 8][e % 8] = (_Float16)(y - (float)ph[e / 8][e % 8]);
-                          if (!kPair && e % 2 == 1) {   // the sum of P as the product has it
-                              const half2_t ones = {(_Float16)1.0f, (_Float16)1.0f};
-                              float &to = add[kExact ? 0 : e / 2 % 4];   // (registers are short)
-                              to = __builtin_amdgcn_fdot2(half2_t{ph[e / 8][e % 8 - 1], ph[e / 8][e % 8]}, ones,
-                                                          to, false);
-                          }
                           // (taken here, not moved to where it is used)
                           if (e % 8 == 7) {
                               asm volatile("" : "+v"(ph[e / 8]));
@@ -428,7 +437,8 @@ __global__ __launch_bounds__(kThreads, tiles_twice(sizeof(S) == 4, P) ? 2 : 1) v
                           }
                       }
                   });
-        sum += ((add[0] + add[1]) + (add[2] + add[3])) * (kPair ? 1.0f : fast_rcp(ratio));
+        if constexpr (kPair) sum += (add[0] + add[1]) + (add[2] + add[3]);
+        else inverse_ratio = fast_rcp(ratio);
         if constexpr (kExact) exact += add_exact;
     };
     float16v other[2];
@@ -446,9 +456,11 @@ __global__ __launch_bounds__(kThreads, tiles_twice(sizeof(S) == 4, P) ? 2 : 1) v
     }
     __syncthreads();
     clear_fresh();
+    clear_add();
     steps<NO>([&](uint32_t i) { return value_operand((tiles + 1) & 1, i); }, [&](uint32_t i, half8 v) { output(i, v); },
-              [](uint32_t) {});
+              add_p);
     add_fresh();
+    if constexpr (!kPair) sum += ((add[0] + add[1]) + (add[2] + add[3])) * inverse_ratio;
     sum = flash::pair_sum(sum);
     exact = kExact ? flash::pair_sum(exact) : sum;
     big -= kHeadroom<S>;
