@@ -148,8 +148,11 @@ __global__ __launch_bounds__(kThreads, tiles_twice(sizeof(S) == 4, P) ? 2 : 1) v
     constexpr uint32_t KROW = P + 8, VROW = kTokens + 8;   // LDS rows, halves
     constexpr uint32_t KTILE = kTokens * KROW, VTILE = VT * 32 * VROW;
     constexpr uint32_t KPER = (kTokens * P / 16 + kThreads - 1) / kThreads;   // 16-byte pieces of codes per thread
+    // Of a row's groups of 8 the even ones lie in its first half and the odd ones
+    // in its second, so that a wave's lanes write 16 bytes side by side.
+    constexpr uint32_t KHALF = P / 2, VHALF = kTokens / 2;
     // (each tile with a spare place, for pieces past the end)
-    __shared__ __attribute__((aligned(16))) _Float16 ks[2][KTILE + 16], vs[2][VTILE + 16];
+    __shared__ __attribute__((aligned(16))) _Float16 ks[2][KTILE + KHALF + 8], vs[2][VTILE + VHALF + 8];
     __shared__ int wave_most[kWaves];
     const View &c = a.c;
     const uint32_t tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
@@ -217,8 +220,8 @@ __global__ __launch_bounds__(kThreads, tiles_twice(sizeof(S) == 4, P) ? 2 : 1) v
 #pragma unroll
     for (uint32_t u = 0; u < KPER; ++u) {
         const uint32_t p = tid + u * kThreads;
-        kto[u] = p < kpieces ? p * 16 / c.kp * KROW + p * 16 % c.kp : KTILE;
-        vto[u] = p < vpieces ? p / 4 * VROW + p % 4 * 16 : VTILE;
+        kto[u] = p < kpieces ? p * 16 / c.kp * KROW + p * 16 % c.kp / 2 : KTILE;
+        vto[u] = p < vpieces ? p / 4 * VROW + p % 4 * 8 : VTILE;
     }
     u32x4 kreg[KPER], vreg[KPER];
     // (asked for without a test, past the end some block again: the count of loads
@@ -233,14 +236,14 @@ __global__ __launch_bounds__(kThreads, tiles_twice(sizeof(S) == 4, P) ? 2 : 1) v
 #pragma unroll
         for (uint32_t u = 0; u < KPER; ++u) vreg[u] = from[min(tid + u * kThreads, vpieces - 1)];
     };
-    auto put = [&](_Float16 *to, half8 lo, half8 hi) {
+    auto put = [&](_Float16 *to, uint32_t far, half8 lo, half8 hi) {
         *reinterpret_cast<half8 *>(to) = lo;
-        *reinterpret_cast<half8 *>(to + 8) = hi;
+        *reinterpret_cast<half8 *>(to + far) = hi;
     };
     auto stash_k = [&](uint32_t buf) {
 #pragma unroll
         for (uint32_t u = 0; u < KPER; ++u)
-            put(&ks[buf][kto[u]], codes(kreg[u].x, kreg[u].y), codes(kreg[u].z, kreg[u].w));
+            put(&ks[buf][kto[u]], KHALF, codes(kreg[u].x, kreg[u].y), codes(kreg[u].z, kreg[u].w));
     };
 
     const float neg_inf = -__builtin_inff();
@@ -261,11 +264,11 @@ __global__ __launch_bounds__(kThreads, tiles_twice(sizeof(S) == 4, P) ? 2 : 1) v
     float16v fresh[kPair ? VT : 1];   // f32: a tile's outputs
     auto key_operand = [&](uint32_t buf, uint32_t i) {
         i %= NS1;
-        return *reinterpret_cast<const half8 *>(&ks[buf][(32 * (i % 2) + swap23(col)) * KROW + 16 * (i / 2) + 8 * half]);
+        return *reinterpret_cast<const half8 *>(&ks[buf][(32 * (i % 2) + swap23(col)) * KROW + 8 * (i / 2) + KHALF * half]);
     };
     auto value_operand = [&](uint32_t buf, uint32_t i) {
         i %= NO1;
-        return *reinterpret_cast<const half8 *>(&vs[buf][(32 * (i % VT) + col) * VROW + 16 * (i / VT) + 8 * half]);
+        return *reinterpret_cast<const half8 *>(&vs[buf][(32 * (i % VT) + col) * VROW + 8 * (i / VT) + VHALF * half]);
     };
     auto score = [&](float16v (&to)[2], uint32_t i, half8 k) {
         to[i % 2] = __builtin_amdgcn_mfma_f32_32x32x16_f16(k, q.piece[i / NS1][i % NS1 / 2], to[i % 2], 0, 0, 0);
@@ -312,13 +315,13 @@ __global__ __launch_bounds__(kThreads, tiles_twice(sizeof(S) == 4, P) ? 2 : 1) v
         const u32x4 w = keys ? kreg[piece] : vreg[piece];
         const half8 x = second ? codes(w.z, w.w) : codes(w.x, w.y);
         _Float16 *const to = keys ? &ks[buf][kto[piece]] : &vs[buf][vto[piece]];
-        *reinterpret_cast<half8 *>(to + 8 * second) = x;
+        *reinterpret_cast<half8 *>(to + (keys ? KHALF : VHALF) * second) = x;
     };
 
     // columns past the padded dim meet zeros of q, and the first turn's P of no
     // tile meets these values: neither may be NaN
     for (uint32_t p = tid; p < kTokens * (P - c.kp) / 8; p += kThreads) {
-        const uint32_t per = (P - c.kp) / 8, t = p / per, d = c.kp + p % per * 8;
+        const uint32_t per = (P - c.kp) / 8, t = p / per, group = c.kp / 8 + p % per, d = group % 2 * KHALF + group / 2 * 8;
         *reinterpret_cast<half8 *>(&ks[0][t * KROW + d]) = half8{};
         *reinterpret_cast<half8 *>(&ks[1][t * KROW + d]) = half8{};
     }
@@ -332,7 +335,7 @@ __global__ __launch_bounds__(kThreads, tiles_twice(sizeof(S) == 4, P) ? 2 : 1) v
 #pragma unroll
             for (uint32_t u = 0; u < KPER; ++u) {
                 const uint32_t p = min(tid + u * kThreads, kpieces - 1);
-                put(&ks[0][kto[u]], kt[2 * p], kt[2 * p + 1]);
+                put(&ks[0][kto[u]], KHALF, kt[2 * p], kt[2 * p + 1]);
             }
         } else {
             stash_k(0);
@@ -449,7 +452,7 @@ __global__ __launch_bounds__(kThreads, tiles_twice(sizeof(S) == 4, P) ? 2 : 1) v
 #pragma unroll
             for (uint32_t u = 0; u < KPER; ++u) {
                 const uint32_t p = min(tid + u * kThreads, vpieces - 1);
-                put(&vs[0][vto[u]], vt[2 * p], vt[2 * p + 1]);
+                put(&vs[0][vto[u]], VHALF, vt[2 * p], vt[2 * p + 1]);
             }
         }
         if (s + 1 < tiles) turn(s + 1, other, st);
