@@ -109,7 +109,10 @@ template <bool kStream, typename V> __device__ inline V load_codes(const V *p) {
 
 // One workgroup: 16 packed rows of one (sequence, kv head) and one part of its
 // blocks; wave w takes blocks w, w + 4, ... of the part and the waves' results
-// meet in LDS.
+// meet in LDS. Bound by the codes' way from memory: 8 x 8 heads x 4096 tokens of D 128
+// (67 MB) 14 us, 4.7 TB/s, and the fold 3; one sequence of 131000 tokens (268 MB) 47 us,
+// 5.7 TB/s (a copy of 1 GiB: 5.1). Two workgroups for every CU: three or four make more
+// parts to fold (8 x 4096 18 -> 22 us).
 // What the first loads wait for comes as leading arguments, which are in scalar
 // registers when a wave starts: the struct behind them takes a microsecond to
 // arrive. (8 x 4096 tokens, from the wave's start to its first loads' issue: 2 us
@@ -408,7 +411,9 @@ __device__ inline f32x2 fold_ml(const f32x2 *ml, const float *exact, uint32_t pa
 // Merges the parts of rows, kRowWaves waves for each: the waves take the parts in
 // turn, a lane four output elements. The workgroups after `folds` do a token per
 // thread of one (sequence, head): their weights from the stored scores. Bound by
-// its chain of memory latencies: up to 4 parts one wave per row, up to 16 four.
+// its chain of memory latencies: up to 4 parts one wave per row, up to 16 four. 3 to 6
+// us. (The last workgroup of a row folding in the rows kernel instead: 60 us more, for
+// the fences that order its parts.)
 template <typename S, uint32_t kFoldWaves, uint32_t kRowWaves>
 __global__ __launch_bounds__(kFoldWaves *kWave) void kv_fold_kernel(const float *part_o, const f32x2 *part_ml, size_t rows,
                                                                   uint32_t parts, uint32_t n, uint32_t in_head,
