@@ -273,6 +273,15 @@ def test_scores_that_overflow(sdk):
     assert (got[0, 0, 0] == 0).all() and np.isfinite(got).all() and got[0, 0, 1].any()
 
 
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_weights_of_a_long_causal_prompt(sdk, dtype):
+    """Blocks enough to fill the chip, and the first seen by many more rows than the
+    last: their rows are shared by more workgroups than that takes."""
+    pair = Pair(sdk, 1, 40, 1600, 16, 24, 12)
+    pair.append(1600)
+    run(pair, dtype, 80, 1600, weighted=True)
+
+
 @pytest.mark.parametrize("n", [1, 20])
 @pytest.mark.parametrize("dims", [(72, 72), (40, 24), (100, 33)], ids=str)
 def test_the_largest_keys_cut(sdk, dims, n):
