@@ -520,6 +520,8 @@ uint32_t widest_of(const View &c) { return c.kp > c.vp ? c.kp : c.vp; }
 // (2.0e9) 44 and 52, 8 x 512 x 8000 (4.1e9) 72 and 74, 32 x 512 x 8000 226 and 201.
 constexpr double kTileProducts = 2.6e9, kTileProductsF32 = 3.5e9;
 constexpr uint32_t kWorkgroups = 512;   // two for every CU
+// Whether a CU holds two workgroups of the rows kernel (their registers decide).
+constexpr bool rows_twice(bool f32, uint32_t widest) { return widest <= (f32 ? 128u : 192u); }
 
 Plan plan_of(bool f32, const View &c, const AttentionShape &a) {
     Plan p{};
@@ -532,11 +534,13 @@ Plan plan_of(bool f32, const View &c, const AttentionShape &a) {
     p.tiles = products >= (f32 ? kTileProductsF32 : kTileProducts) && tiles_fit(f32, widest_of(c));
     const uint32_t rows_each = p.tiles ? kTileRows : kRows;
     p.row_groups = (in_head + rows_each - 1) / rows_each;
-    // parts: workgroups for every CU twice over (tiles of which a CU holds one: once;
-    // f32 D 128, 8 heads x 512 rows x 8000 keys 74 us, twice over 87), with a block for
-    // each wave (tiles: four blocks) at least
+    // parts: workgroups for every CU twice over (once for those of which a CU holds one:
+    // tiles, f32 D 128, 8 heads x 512 rows x 8000 keys 74 us, twice over 87; rows, f16 D
+    // 256, 8 x 8 heads x 4096 keys 30 us, twice over 35), with a block for each wave
+    // (tiles: four blocks) at least
     const uint64_t base = pairs * p.row_groups;
-    const uint32_t fill = p.tiles && !tiles_twice(f32, widest_of(c)) ? kWorkgroups / 2 : kWorkgroups;
+    const bool twice = p.tiles ? tiles_twice(f32, widest_of(c)) : rows_twice(f32, widest_of(c));
+    const uint32_t fill = twice ? kWorkgroups : kWorkgroups / 2;
     uint64_t parts = base >= fill ? 1 : fill / base;
     const uint32_t most = (blocks + kWaves - 1) / kWaves;
     parts = parts < most ? parts : most;
