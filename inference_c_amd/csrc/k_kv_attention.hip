@@ -500,7 +500,7 @@ __global__ __launch_bounds__(kFoldWaves *kWave) void kv_fold_kernel(const float 
 
 struct Plan {
     bool tiles;    // many rows: k_kv_tiles.hip
-    bool scores;   // the weights come from scores that the rows kernel stores
+    bool scores;   // the weights come from scores that the rows kernel stores (never with tiles)
     uint32_t row_groups, parts, row_parts;
     size_t rows, score_stride;
     size_t o_bytes, ml_bytes, exact_bytes, row_bytes, score_bytes, partial_bytes;
@@ -531,7 +531,9 @@ Plan plan_of(bool f32, const View &c, const AttentionShape &a) {
     // keys that a row sees on average
     const double keys = a.longest - (a.causal ? 0.5 * (a.n < a.longest ? a.n : a.longest) : 0.0);
     const double products = (double)pairs * in_head * keys * widest_of(c);
-    p.tiles = products >= (f32 ? kTileProductsF32 : kTileProducts) && tiles_fit(f32, widest_of(c));
+    // (never for a packed tile of the rows kernel or less: of those the weights come
+    // from scores, which only the rows kernel stores)
+    p.tiles = in_head > kRows && products >= (f32 ? kTileProductsF32 : kTileProducts) && tiles_fit(f32, widest_of(c));
     const uint32_t rows_each = p.tiles ? kTileRows : kRows;
     p.row_groups = (in_head + rows_each - 1) / rows_each;
     // parts: workgroups for every CU twice over (once for those of which a CU holds one:

@@ -1,0 +1,90 @@
+"""Attention over the 8-bit key/value cache at the limits of its range: few query
+rows over very many keys."""
+import ctypes
+
+import numpy as np
+import pytest
+
+from tests.kv_model import u32s
+from tests.test_gpu_kv_attention import attend, compare, run
+from tests.test_gpu_kv_cache import DTYPES, Pair
+
+pytestmark = pytest.mark.gpu
+
+
+def one_long(sdk, batch, kv, length, dim, vdim, seed):
+    """A batch whose first sequence has `length` tokens (its keys and values come
+    four times) and whose others have a few: as many keys to plan for as if all
+    were long."""
+    pair = Pair(sdk, batch, kv, length, dim, vdim, seed)
+    n = length // 4
+    k, v = np.zeros((batch, kv, n, dim), np.float16), np.zeros((batch, kv, n, vdim), np.float16)
+    short = [(7 * b) % 23 + 1 for b in range(batch)]
+    few = max(short)
+    for x in (k, v):
+        x[0] = pair.rng.standard_normal(x[0].shape)
+        x[1:, :, :few] = pair.rng.standard_normal(x[1:, :, :few].shape)
+    tk, tv = sdk.from_numpy(k), sdk.from_numpy(v)
+    for turn in range(4):
+        counts = [n] + [m if turn == 2 else 0 for m in short[1:]]
+        sdk.call("tensor_kv_cache_append_f16", pair.cache, tk, tv, u32s(counts))
+        pair.model.append(k[:, :, :max(counts)], v[:, :, :max(counts)], counts)
+    return pair
+
+
+# batch, kv heads, query heads, rows, tokens of the longest, dim, value dim: at most
+# 16 packed rows per kv head, and more products (sequences x kv heads x rows x tokens
+# x the wider dim) than the tile kernel is used from for prompts; key parts (few
+# sequences and heads) and none (many)
+FEW = [("f16", 64, 4, 16, 1, 10400, 16, 256), ("f16", 64, 4, 64, 1, 2600, 16, 256), ("f16", 32, 8, 64, 2, 2600, 256, 16),
+       ("f16", 16, 2, 32, 1, 20800, 16, 256), ("f32", 64, 4, 64, 1, 6800, 16, 128), ("f32", 16, 2, 16, 2, 54400, 16, 128)]
+
+
+@pytest.mark.parametrize("shape", FEW, ids=str)
+def test_weights_of_few_rows_over_many_keys(sdk, shape):
+    dtype, batch, kv, heads, n, length, dim, vdim = shape
+    pair = one_long(sdk, batch, kv, length, dim, vdim, n)
+    run(pair, dtype, heads, n, weighted=True, what="causal")
+    run(pair, dtype, heads, n, causal=False, weighted=True, what="all seen")
+    run(pair, dtype, heads, n, what="no weights")
+
+
+# capacity instead of tokens: what a recorded call is planned for
+CAPACITIES = [("f16", 4, 2, 8, 1, 330000, 16, 256), ("f16", 64, 4, 16, 1, 10400, 16, 256), ("f16", 2, 2, 8, 4, 165000, 256, 16),
+              ("f32", 64, 4, 64, 1, 6800, 16, 128), ("f32", 4, 2, 8, 3, 290000, 16, 128)]
+
+
+@pytest.mark.parametrize("shape", CAPACITIES, ids=str)
+def test_recorded_weights_of_few_rows_in_a_large_cache(sdk, shape):
+    dtype, batch, kv, heads, n, capacity, dim, vdim = shape
+    hip = sdk.lib
+    hip.tensor_device_hip_stream.restype = ctypes.c_void_p
+    stream = ctypes.c_void_p(hip.tensor_device_hip_stream())
+    pair = Pair(sdk, batch, kv, capacity, dim, vdim, 41)
+    pair.append(100, counts=[100 - b % 90 for b in range(batch)])
+    q = pair.rng.standard_normal((batch, heads, n, dim)).astype(DTYPES[dtype])
+    tq, out = sdk.from_numpy(q), sdk.tensor(dtype, (batch, heads, n, vdim))
+    w = sdk.tensor("f32", (batch, kv, 400))
+    call = (f"tensor_kv_cache_attention_{dtype}", pair.cache, tq, None, 0.25, 1, w, out)
+    sdk.call(*call)
+    sdk.synchronize()
+    graph, exe = ctypes.c_void_p(), ctypes.c_void_p()
+    assert hip.hipStreamBeginCapture(stream, 2) == 0
+    try:
+        sdk.call(*call)
+    finally:
+        assert hip.hipStreamEndCapture(stream, ctypes.byref(graph)) == 0
+    assert hip.hipGraphInstantiate(ctypes.byref(exe), graph, None, None, ctypes.c_size_t(0)) == 0
+    for change in (None, "append", "eager", "append"):
+        if change == "append":
+            pair.append(130, counts=[130 - b % 3 for b in range(batch)])
+        elif change == "eager":
+            attend(sdk, pair.cache, q, 0.3, False, vdim=vdim)
+        w0 = pair.rng.random(w.shape).astype(np.float32)
+        w.upload(w0)
+        out.upload(np.full(out.shape, 99, DTYPES[dtype]))
+        sdk.synchronize()
+        assert hip.hipGraphLaunch(exe, stream) == 0
+        compare(pair.model, q, 0.25, True, None, out.download(), w0, w.download(), str(change))
+    assert hip.hipGraphExecDestroy(exe) == 0
+    assert hip.hipGraphDestroy(graph) == 0
