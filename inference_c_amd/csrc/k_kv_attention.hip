@@ -519,6 +519,15 @@ uint32_t widest_of(const View &c) { return c.kp > c.vp ? c.kp : c.vp; }
 // (2.3e9) 58 and 63, 32 x 1024 x 2000 (3.9e9) 102 and 87; D 128, 32 x 256 x 2000
 // (2.0e9) 44 and 52, 8 x 512 x 8000 (4.1e9) 72 and 74, 32 x 512 x 8000 226 and 201.
 constexpr double kTileProducts = 2.6e9, kTileProductsF32 = 3.5e9;
+// ... where it takes less than the rows kernel's workgroups of 16 rows do: it multiplies
+// 128 rows whatever is there, in the time of two of those at f16, of four at dims up to 32
+// and of five at f32. Measured at 64 heads x 8000 keys, from 2.6e9 products on (us, rows
+// kernel and tiles): f16 D 128, 32 rows 48 and 47, 48 rows 69 and 50, 96 rows 125 and 57; D
+// 256, 32 rows 94 and 103, 48 rows 149 and 109; 64 x 32000, D 128, 16 rows 93 and 168; D 64,
+// 32 rows 90 and 99, 48 rows 137 and 107; D 32, 64 rows 84 and 88, 96 rows 144 and 91; f32
+// D 128, 64 rows 349 and 378, 96 rows 589 and 399; D 64, 64 rows 211 and 255, 96 rows 339
+// and 254; 64 x 8000, 160 rows 112 and 129, 256 rows 148 and 134.
+constexpr uint32_t rows_for_tile(bool f32, uint32_t widest) { return kRows * (f32 ? 5 : widest <= 32 ? 4 : 2); }
 constexpr uint32_t kWorkgroups = 512;   // two for every CU
 // Whether a CU holds two workgroups of the rows kernel (their registers decide).
 constexpr bool rows_twice(bool f32, uint32_t widest) { return widest <= (f32 ? 128u : 192u); }
@@ -531,9 +540,10 @@ Plan plan_of(bool f32, const View &c, const AttentionShape &a) {
     // keys that a row sees on average
     const double keys = a.longest - (a.causal ? 0.5 * (a.n < a.longest ? a.n : a.longest) : 0.0);
     const double products = (double)pairs * in_head * keys * widest_of(c);
-    // (never for a packed tile of the rows kernel or less: of those the weights come
-    // from scores, which only the rows kernel stores)
-    p.tiles = in_head > kRows && products >= (f32 ? kTileProductsF32 : kTileProducts) && tiles_fit(f32, widest_of(c));
+    const uint32_t whole_rows = (in_head + kRows - 1) / kRows * kRows;
+    const uint32_t row_tiles = (in_head + kTileRows - 1) / kTileRows;
+    p.tiles = whole_rows > (uint64_t)row_tiles * rows_for_tile(f32, widest_of(c)) &&
+              products >= (f32 ? kTileProductsF32 : kTileProducts) && tiles_fit(f32, widest_of(c));
     const uint32_t rows_each = p.tiles ? kTileRows : kRows;
     p.row_groups = (in_head + rows_each - 1) / rows_each;
     // parts: workgroups for every CU twice over (once for those of which a CU holds one:
@@ -550,7 +560,8 @@ Plan plan_of(bool f32, const View &c, const AttentionShape &a) {
     p.rows = (size_t)a.batch * a.q_heads * a.n;
     p.o_bytes = p.parts > 1 ? whole256(p.parts * p.rows * c.vdim * 4) : 0;
     // a token's scores, 4 bytes per row written and read again, against its key
-    // again: for up to a tile of rows the scores
+    // again: for up to 16 rows the scores (which the rows kernel, that these
+    // always take, stores)
     p.scores = a.weights != nullptr && in_head <= kRows;
     p.score_stride = (size_t)blocks * kTokens;
     p.ml_bytes = p.parts > 1 || p.scores ? whole256(p.parts * p.rows * sizeof(f32x2)) : 0;

@@ -49,6 +49,20 @@ def test_weights_of_few_rows_over_many_keys(sdk, shape):
     run(pair, dtype, heads, n, what="no weights")
 
 
+# around the packed rows from which so many products go to the tile kernel
+MORE = [("f16", 64, 4, 68, 1, 2600, 16, 256), ("f16", 64, 4, 32, 4, 2600, 256, 16), ("f16", 64, 4, 44, 3, 1600, 16, 256),
+        ("f16", 64, 8, 128, 4, 5200, 16, 32), ("f16", 64, 8, 104, 5, 5200, 16, 32), ("f32", 64, 4, 64, 3, 2400, 16, 128),
+        ("f32", 64, 4, 128, 2, 1720, 16, 128), ("f32", 64, 4, 52, 5, 1720, 16, 128), ("f32", 64, 4, 68, 2, 3600, 16, 200)]
+
+
+@pytest.mark.parametrize("shape", MORE, ids=str)
+def test_some_rows_over_many_keys(sdk, shape):
+    dtype, batch, kv, heads, n, length, dim, vdim = shape
+    pair = one_long(sdk, batch, kv, length, dim, vdim, heads)
+    run(pair, dtype, heads, n, weighted=True, what="causal")
+    run(pair, dtype, heads, n, causal=False, what="no weights")
+
+
 # capacity instead of tokens: what a recorded call is planned for
 CAPACITIES = [("f16", 4, 2, 8, 1, 330000, 16, 256), ("f16", 64, 4, 16, 1, 10400, 16, 256), ("f16", 2, 2, 8, 4, 165000, 256, 16),
               ("f32", 64, 4, 64, 1, 6800, 16, 128), ("f32", 4, 2, 8, 3, 290000, 16, 128)]
