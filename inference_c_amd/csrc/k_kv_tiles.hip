@@ -31,10 +31,9 @@ template <typename S, uint32_t P> struct TileQuery {
     static constexpr uint32_t kSteps = P / 16;
     static constexpr bool kPair = sizeof(S) == 4;
     half8 piece[kPieces<S>][kSteps];
-    float factor;   // the power of two that a f32 row was divided by
+    int shift = 0;   // an f32 row was divided by 2^shift
 
     __device__ inline void load(const S *row, uint32_t dim, uint32_t half, float sign) {
-        factor = 1.0f;
         if constexpr (!kPair) {
             const _Float16 s = (_Float16)sign;
             if (dim % 8 == 0) {
@@ -73,28 +72,30 @@ template <typename S, uint32_t P> struct TileQuery {
             big = flash::pair_max(finite ? big : __builtin_inff());
             const bool usable = big > 0.0f && __builtin_isfinite(big);
             const int exponent = usable ? __builtin_amdgcn_frexp_expf(big) : 14;
-            factor = __builtin_isfinite(big) ? __builtin_ldexpf(1.0f, exponent - 14) : __builtin_nanf("");
+            shift = exponent - 14;
+            const float none = big > 0.0f ? __builtin_nanf("") : 0.0f;   // (not finite: no score is)
 #pragma unroll
             for (uint32_t c = 0; c < kSteps; ++c)
 #pragma unroll
                 for (uint32_t e = 0; e < 8; ++e) {
-                    const float y = usable ? __builtin_ldexpf(x[c][e], 14 - exponent) : 0.0f;
+                    const float y = usable ? __builtin_ldexpf(x[c][e], -shift) : none;
                     pieces_of(y, piece[0][c], piece[1][c], piece[2][c], e);
                 }
         }
     }
 };
 
-// A block's factor of raw products, positive (queries carry the scale's sign), and,
-// for f32, what rounding took off it. A block of zero keys has raw products 0: any
-// factor.
-template <typename S, bool kExact> __device__ inline f32x2 block_factor(float k_scale, double scale2) {
+// A block's factor of raw products, for f32 times the query row's 2^shift, and what
+// rounding took off it. Positive (queries carry the scale's sign) and finite: masked
+// products are -inf before it. Below kTiny products come to nothing either way. A block
+// of zero keys has raw products 0: any factor.
+template <typename S, bool kExact> __device__ inline f32x2 block_factor(float k_scale, double scale2, int shift) {
     const float k = k_scale == 0.0f ? 1.0f : k_scale;
     const double scale = scale2 == 0.0 ? 1.0 : fabs(scale2);
     if constexpr (sizeof(S) == 2 && !kExact) {
         return f32x2{fminf(fmaxf(k * (float)scale, kTiny), kHuge), 0.0f};
     } else {
-        const double f = (double)k * scale;
+        const double f = sizeof(S) == 4 ? __builtin_ldexp((double)k * scale, shift) : (double)k * scale;
         const float hi = fminf(fmaxf((float)f, kTiny), kHuge);
         return f32x2{hi, (float)(f - (double)hi)};
     }
@@ -371,8 +372,8 @@ __global__ __launch_bounds__(kThreads, tiles_twice(sizeof(S) == 4, P) ? 2 : 1) v
                 now[e / 16][e % 16] = (int)key >= last ? neg_inf : x;
             }
         }
-        const f32x2 f2 = block_factor<S, kExact>(m.k_scale, a.scale2);
-        const float factor = f2.x * q.factor;
+        const f32x2 f2 = block_factor<S, kExact>(m.k_scale, a.scale2, q.shift);
+        const float factor = f2.x;
         float part_max[4] = {neg_inf, neg_inf, neg_inf, neg_inf};
         clear_fresh();
         clear_add();
@@ -429,7 +430,7 @@ __global__ __launch_bounds__(kThreads, tiles_twice(sizeof(S) == 4, P) ? 2 : 1) v
                           const float raw_score = now[e / 16][e % 16];
                           float x = __builtin_fmaf(raw_score, factor, -base);
                           if constexpr (kPair) {
-                              const float off = raw_score * (f2.y * q.factor);
+                              const float off = raw_score * f2.y;
                               x += fabsf(off) < 1.0f ? off : 0.0f;   // (not for -inf)
                           }
                           x = __builtin_amdgcn_exp2f(x);
@@ -509,7 +510,7 @@ __global__ __launch_bounds__(kThreads, P <= 64 ? 3 : P <= 128 ? 2 : 1) void kv_w
     constexpr uint32_t KC = P / 16, QROW = P + 8, kStep = 32;
     constexpr uint32_t G = (P / 8 + 7) / 8;   // groups of 8 dims of a thread: 8 threads stage a row
     __shared__ __attribute__((aligned(16))) _Float16 qs[2][kPieces<S>][kStep * QROW];
-    __shared__ f32x4 terms[2][kStep];         // of a row: maximum, 1 / sum (0: adds nothing), factor
+    __shared__ f32x4 terms[2][kStep];         // of a row: maximum, 1 / sum (0: adds nothing), shift
     const View &c = a.c;
     const uint32_t tid = threadIdx.x, lane = tid & 63, col = lane & 31, half = lane >> 5;
     const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane(tid / kWave);
@@ -537,7 +538,7 @@ __global__ __launch_bounds__(kThreads, P <= 64 ? 3 : P <= 128 ? 2 : 1) void kv_w
             }
         }
     const float sign = a.scale2 > 0.0 ? 1.0f : a.scale2 < 0.0 ? -1.0f : 0.0f;
-    const float k_factor = block_factor<S, true>(open ? 1.0f : meta.k_scale, a.scale2).x;
+    const float k_scale = open ? 1.0f : meta.k_scale;
     float acc[32];
 #pragma unroll
     for (int e = 0; e < 32; ++e) acc[e] = 0.0f;
@@ -589,7 +590,7 @@ __global__ __launch_bounds__(kThreads, P <= 64 ? 3 : P <= 128 ? 2 : 1) void kv_w
 #pragma unroll
             for (uint32_t e = 0; e < 8; ++e) x[g][e] = ml.y != 0.0f && d + e < c.dim ? x[g][e] * (S)sign : (S)0.0f;
         }
-        float factor = 1.0f;
+        int shift = 0;
         if constexpr (kPair) {
             float big = 0.0f;
 #pragma unroll
@@ -598,14 +599,13 @@ __global__ __launch_bounds__(kThreads, P <= 64 ? 3 : P <= 128 ? 2 : 1) void kv_w
                 for (uint32_t e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[g][e]));
 #pragma unroll
             for (int d = 1; d < 8; d *= 2) big = fmaxf(big, __shfl_xor(big, d, kWave));
-            const int exponent = big > 0.0f ? __builtin_amdgcn_frexp_expf(big) : 14;
-            factor = __builtin_ldexpf(1.0f, exponent - 14);
+            shift = big > 0.0f ? __builtin_amdgcn_frexp_expf(big) - 14 : 0;
 #pragma unroll
             for (uint32_t g = 0; g < G; ++g) {
                 half8 piece[3];
 #pragma unroll
                 for (uint32_t e = 0; e < 8; ++e)
-                    pieces_of(__builtin_ldexpf(x[g][e], 14 - exponent), piece[0], piece[1], piece[2], e);
+                    pieces_of(__builtin_ldexpf(x[g][e], -shift), piece[0], piece[1], piece[2], e);
                 const uint32_t d = (sub + 8 * g) * 8;
                 if (d < P)
 #pragma unroll
@@ -618,7 +618,7 @@ __global__ __launch_bounds__(kThreads, P <= 64 ? 3 : P <= 128 ? 2 : 1) void kv_w
                 if (d < P) *reinterpret_cast<half8 *>(&qs[buf][0][srow * QROW + d]) = x[g];
             }
         }
-        if (sub == 0) terms[buf][srow] = f32x4{ml.x, ml.y, factor, 0.0f};
+        if (sub == 0) terms[buf][srow] = f32x4{ml.x, ml.y, (float)shift, 0.0f};
     };
     // two steps' rows are on their way while a step is computed
     Staged even, odd;
@@ -637,7 +637,7 @@ __global__ __launch_bounds__(kThreads, P <= 64 ? 3 : P <= 128 ? 2 : 1) void kv_w
         const int seen = seen_by(i, live, length, count, a.causal);
         if (wave_any(live && seen > (int)(t * kTokens))) {
             const f32x4 term = terms[buf][col];
-            const float factor = k_factor * term.z;
+            const float factor = block_factor<S, true>(k_scale, a.scale2, (int)term.z).x;
             float16v st[2];
 #pragma unroll
             for (int s = 0; s < 2; ++s)

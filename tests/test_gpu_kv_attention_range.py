@@ -1,5 +1,5 @@
 """Attention over the 8-bit key/value cache at the limits of its range: few query
-rows over very many keys."""
+rows over very many keys, queries far from 1."""
 import ctypes
 
 import numpy as np
@@ -7,7 +7,7 @@ import pytest
 
 from tests.kv_model import u32s
 from tests.test_gpu_kv_attention import attend, compare, run
-from tests.test_gpu_kv_cache import DTYPES, Pair
+from tests.test_gpu_kv_cache import DTYPES, Pair, rows_of
 
 pytestmark = pytest.mark.gpu
 
@@ -102,3 +102,24 @@ def test_recorded_weights_of_few_rows_in_a_large_cache(sdk, shape):
         compare(pair.model, q, 0.25, True, None, out.download(), w0, w.download(), str(change))
     assert hip.hipGraphExecDestroy(exe) == 0
     assert hip.hipGraphDestroy(graph) == 0
+
+
+@pytest.mark.parametrize("keys", [1.0, 2.0 ** -12])
+@pytest.mark.parametrize("size", [1e-30, 1e-37, 1e-40, 1e-44])
+def test_tiny_f32_queries(sdk, size, keys):
+    """Rows whose scores come to nothing see their tokens alike, and no others, and
+    add their weights, on every kernel."""
+    pair = Pair(sdk, 1, 2, 200, 64, 64, 42)
+    k, v = (rows_of(pair.rng, (1, 2, 150, 64), "f16", s) for s in (keys, 1.0))
+    pair.append(150, key=k, value=v)
+    for n in (1, 9, 70):
+        for scale in (0.125, -1e-4):
+            run(pair, "f32", 4, n, scale=scale, spread=size, weighted=True, what=f"{n} rows, {scale}")
+    run(pair, "f32", 4, 70, scale=0.125, spread=size, causal=False, weighted=True, what="all seen")
+
+
+def test_tiny_f32_queries_in_tiles(sdk):
+    pair = Pair(sdk, 2, 64, 1200, 64, 64, 43)
+    pair.append(1200)
+    for size in (1e-36, 1e-44):
+        run(pair, "f32", 64, 512, scale=0.125, spread=size, weighted=True, what=f"{size}")
