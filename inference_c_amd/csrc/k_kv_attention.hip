@@ -57,10 +57,9 @@ template <typename S, uint32_t P> struct Query {
     static constexpr uint32_t kSteps = P / 32;
     static constexpr bool kPair = sizeof(S) == 4;
     half8 piece[kPieces<S>][kSteps];
-    float factor;   // the power of two that a f32 row was divided by
+    int shift = 0;   // an f32 row was divided by 2^shift
 
     __device__ inline void load(const S *row, uint32_t dim, uint32_t g) {
-        factor = 1.0f;
         if constexpr (!kPair) {
 #pragma unroll
             for (uint32_t s = 0; s < kSteps; ++s) {
@@ -91,12 +90,13 @@ template <typename S, uint32_t P> struct Query {
             // leave its maximum at -inf, and it is zeros
             const bool usable = big > 0.0f && __builtin_isfinite(big);
             const int exponent = usable ? __builtin_amdgcn_frexp_expf(big) : 14;   // big in [2^(e-1), 2^e)
-            factor = __builtin_isfinite(big) ? __builtin_ldexpf(1.0f, exponent - 14) : __builtin_nanf("");
+            shift = exponent - 14;
+            const float none = big > 0.0f ? __builtin_nanf("") : 0.0f;
 #pragma unroll
             for (uint32_t s = 0; s < kSteps; ++s)
 #pragma unroll
                 for (uint32_t e = 0; e < 8; ++e) {
-                    const float y = usable ? __builtin_ldexpf(x[s][e], 14 - exponent) : 0.0f;
+                    const float y = usable ? __builtin_ldexpf(x[s][e], -shift) : none;
                     pieces_of(y, piece[0][s], piece[1][s], piece[2][s], e);
                 }
         }
@@ -200,14 +200,15 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(const uint8_t *keys, 
 
     // one block: kf(u, s) and vf(j, s) give the A operands
     auto step = [&](uint32_t t, Meta meta, auto kf, auto vf, auto keys_done) {
-        // f32: what rounding takes off the factor and the scores is added back in
-        // the exponent (scores of 10 would be off by 1e-6 of their weight)
-        const double whole_factor = (double)meta.k_scale * a.scale2;
-        float factor = (float)whole_factor, factor_rest = 0.0f;
-        if constexpr (kPair) {
-            factor_rest = (float)(whole_factor - (double)factor) * q.factor;
-            factor *= q.factor;
-        }
+        // The factor of raw products, for f32 times the row's 2^shift, is kept finite:
+        // a product of 0 is a score of 0 at any scale. f32: what rounding takes off the
+        // factor and the scores is added back in the exponent (scores of 10 would be
+        // off by 1e-6 of their weight)
+        double whole_factor = (double)meta.k_scale * a.scale2;
+        if constexpr (kPair) whole_factor = __builtin_ldexp(whole_factor, q.shift);
+        const float factor = fminf(fmaxf((float)whole_factor, -kHuge), kHuge);
+        float factor_rest = 0.0f;
+        if constexpr (kPair) factor_rest = fabsf(factor) < kHuge ? (float)(whole_factor - (double)factor) : 0.0f;
         float p[16], rest[kPair ? 16 : 1];
 #pragma unroll
         for (uint32_t u = 0; u < 4; ++u) {

@@ -23,8 +23,6 @@ namespace {
 
 typedef float float16v __attribute__((ext_vector_type(16)));
 
-constexpr float kTiny = 1.1754944e-38f, kHuge = 3.0e38f;
-
 // 32 query rows as B operands, one per 16 dims and piece, times `sign`
 // (the scale's; 0 where the scale is).
 template <typename S, uint32_t P> struct TileQuery {

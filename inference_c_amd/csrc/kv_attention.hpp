@@ -19,6 +19,7 @@ constexpr uint32_t kThreads = 256;
 constexpr uint32_t kWaves = 4;
 constexpr uint32_t kRows = 16;         // packed rows of a wave
 constexpr double kLog2e = 1.4426950408889634;
+constexpr float kTiny = 1.1754944e-38f, kHuge = 3.0e38f;   // what a factor of raw products is kept between
 constexpr float kUnitRange = 8.0f;     // a value scale further from the unit moves it
 // f16: P of a row whose maximum is M is 2^(s - M + kHeadroom): as far up as the unit's
 // range and the lazy rescale of the maximum (by more than 2^kLazy) leave room for, 2^15

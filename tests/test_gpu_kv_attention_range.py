@@ -123,3 +123,26 @@ def test_tiny_f32_queries_in_tiles(sdk):
     pair.append(1200)
     for size in (1e-36, 1e-44):
         run(pair, "f32", 64, 512, scale=0.125, spread=size, weighted=True, what=f"{size}")
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_zero_queries_at_any_scale(sdk, dtype):
+    """Products of 0 are scores of 0, also where scale and keys together pass f32."""
+    pair = Pair(sdk, 1, 2, 200, 64, 64, 44)
+    k, v = (rows_of(pair.rng, (1, 2, 150, 64), "f16", s) for s in (1000.0, 1.0))
+    k[0, 1, 64:128] = 0
+    pair.append(150, key=k, value=v)
+    for n in (1, 9, 70):
+        for scale in (3e38, -3e38):
+            run(pair, dtype, 4, n, scale=scale, spread=0.0, weighted=True, what=f"{n} rows, {scale}")
+
+
+def test_tiny_f32_queries_at_large_scales(sdk):
+    """Rows below the smallest power of two whose reciprocal f32 holds, with scales
+    that bring their scores back."""
+    pair = Pair(sdk, 1, 2, 200, 64, 64, 45)
+    k, v = (rows_of(pair.rng, (1, 2, 150, 64), "f16", s) for s in (30.0, 1.0))
+    pair.append(150, key=k, value=v)
+    for size, scale in ((1e-37, 1e35), (1e-40, 1e38), (1e-42, 3e38)):
+        for n in (1, 9, 70):
+            run(pair, "f32", 4, n, scale=scale, spread=size, weighted=True, what=f"{size}: {n} rows")
