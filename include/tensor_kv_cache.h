@@ -23,7 +23,10 @@
  *   - tensor operands are device tensors; calls enqueue on the SDK stream and
  *     return;
  *   - lengths are kept on the host too, so every check is made before any work
- *     is queued, and a call that fails leaves the cache as it was;
+ *     is queued, and a call that is refused leaves the cache as it was. Should
+ *     the runtime fail to launch a kernel, the sequences of the launches before
+ *     it (256 in each) are done and the others as they were, and the lengths
+ *     say which; of an eviction the target is as it was;
  *   - `counts`, where a call takes it, is a host array of `batch` numbers: of
  *     sequence b only the first counts[b] tokens (or query rows) are there and
  *     the rest of its rows is padding, neither read nor written. NULL: all are
