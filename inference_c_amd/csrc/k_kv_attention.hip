@@ -29,7 +29,8 @@
 //
 // f16: the output is divided by the sum of P as rounded to f16, so that a row with one
 // large weight has its value exactly; accumulated token weights, which are f32, go by the
-// sum before that rounding.
+// sum before that rounding. Token weights of either type go by scores in one f32, off by
+// 2^-24 of the score: sums of many rows' weights, for which 32 bits are enough.
 #include "kv_attention.hpp"
 
 namespace icsdk {

@@ -19,7 +19,6 @@ namespace icsdk {
 namespace kv {
 namespace {
 
-typedef uint16_t u16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 
 constexpr uint32_t kThreads = 256;
