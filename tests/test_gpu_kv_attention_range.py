@@ -1,5 +1,5 @@
 """Attention over the 8-bit key/value cache at the limits of its range: few query
-rows over very many keys, queries far from 1."""
+rows over very many keys, queries far from 1, and how large errors typically are."""
 import ctypes
 
 import numpy as np
@@ -146,3 +146,52 @@ def test_tiny_f32_queries_at_large_scales(sdk):
     for size, scale in ((1e-37, 1e35), (1e-40, 1e38), (1e-42, 3e38)):
         for n in (1, 9, 70):
             run(pair, "f32", 4, n, scale=scale, spread=size, weighted=True, what=f"{size}: {n} rows")
+
+
+def leaning(pair, heads, n, dtype, lean):
+    """Causal query rows that each give one token they see about the weight `lean`
+    (0: none in particular)."""
+    batch, kv, dim, _ = pair.model.shape
+    q = pair.rng.standard_normal((batch, heads, n, dim)) * 0.5
+    for b, j in np.ndindex(batch, heads):
+        k = pair.model.k[b][j // (heads // kv)].held()
+        seen = len(k) - n + 1 + np.arange(n)
+        if lean:
+            to = k[(pair.rng.random(n) * seen).astype(np.int64)]
+            score = np.log(seen * lean / (1 - lean))
+            q[b, j] += to * (score * dim ** 0.5 / (to * to).sum(-1))[:, None]
+    return q.astype(DTYPES[dtype])
+
+
+@pytest.mark.parametrize("lean", [0.0, 0.9])
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("shape", [(1, 2, 4, 5), (1, 2, 4, 70), (2, 64, 64, 512)], ids=["rows", "more rows", "tiles"])
+def test_typical_errors(sdk, shape, dtype, lean):
+    """Root mean squares of the errors, relative to those of what they are errors of;
+    the bounds of the other tests are worst cases, and grow with the keys.
+
+    f32 outputs, in units of u = 2^-24, 1200 keys of 64 dims. Scores (13 in log2 units
+    where a row leans on a token) add up in four steps or so, each off by u of them:
+    36 u of that token's weight, which comes to 0.9 * 0.1 of that in the output, 3 u.
+    19 blocks' sums and outputs are added one by one: 19^0.5 u / 2, 2 u each. A block's
+    products add up in eight steps, each off by u of the largest: 3 u. P is a pair, and
+    its exponential is off by u. Together (3^2 + 2^2 + 2^2 + 3^2 + 1 + 1)^0.5, 5 u: less
+    than 16.
+    Weights: 36 u of the scores at most, and of those again 0.1 in their sum; the
+    factor's rounding 9 u, likewise; at most 22 additions in a row, 3 u: less than 32.
+    f16 outputs: P and the output rounded, each off by 2^-11 / 3^0.5 at most: 2^-11."""
+    batch, kv, heads, n = shape
+    pair = Pair(sdk, batch, kv, 1200, 64, 64, 46)
+    pair.append(1200)
+    q = leaning(pair, heads, n, dtype, lean)
+    got, got_w = attend(sdk, pair.cache, q, 0.125, True, None, np.zeros((batch, kv, 1200), np.float32), 64)
+    want, _, want_w, _ = pair.model.attention(q, 0.125, True)
+    plain, _ = attend(sdk, pair.cache, q, 0.125, True, None, None, 64)
+
+    def error(x, y):
+        return float(np.sqrt(np.square(x.astype(np.float64) - y).mean() / np.square(y).mean()))
+
+    most = 2.0 ** -11 if dtype == "f16" else 2.0 ** -20
+    assert error(got, want) < most and error(plain, want) < most, (error(got, want), error(plain, want))
+    assert error(got_w, want_w) < 2.0 ** -19, error(got_w, want_w)
+    print(f"{shape} {dtype} {lean}: outputs {error(got, want):.2e}, weights {error(got_w, want_w):.2e}")
