@@ -380,3 +380,39 @@ def test_offsets_past_32_bits(sdk):
     target = sdk.kv_cache(2, 12, 100, 256, 256)
     sdk.call("tensor_kv_cache_evict", pair.cache, None, 4, 10, 90, target, None, None)
     check_read(sdk, target, pair.model.evict(None, 4, 10, 90)[0])
+
+
+@pytest.mark.parametrize("shape", [(65535, 1), (1, 4096), (300, 257)], ids=str)
+def test_the_most_sequences_and_heads(sdk, shape):
+    """Every entry point at the largest batch and head count, over three tokens."""
+    batch, kv, dim = *shape, 8
+    rng = np.random.default_rng(47)
+    k, v = (rng.standard_normal((batch, kv, 3, dim)).astype(np.float16) for _ in range(2))
+    cache, target = sdk.kv_cache(batch, kv, 64, dim), sdk.kv_cache(batch, kv, 64, dim)
+    tk, tv = sdk.from_numpy(k), sdk.from_numpy(v)
+    sdk.call("tensor_kv_cache_append_f16", cache, tk, tv, None)
+    sdk.call("tensor_kv_cache_append_f16", cache, tk, tv, None)
+    sdk.call("tensor_kv_cache_truncate", cache, u32s([3] * batch))
+    out_k, out_v = sdk.tensor("f16", k.shape), sdk.tensor("f16", v.shape)
+    sdk.call("tensor_kv_cache_read_f16", cache, out_k, out_v)
+    assert_bits_equal(out_k.download(), k, "keys")
+    assert_bits_equal(out_v.download(), v, "values")
+    q = rng.standard_normal((batch, kv, 1, dim)).astype(np.float32)
+    s = np.einsum("bhqd,bhtd->bht", q.astype(np.float64), k.astype(np.float64))
+    p = np.exp(s - s.max(-1, keepdims=True))
+    p /= p.sum(-1, keepdims=True)
+    w, out = sdk.from_numpy(np.zeros((batch, kv, 3), np.float32)), sdk.tensor("f32", q.shape)
+    sdk.call("tensor_kv_cache_attention_f32", cache, sdk.from_numpy(q), None, 1.0, 1, w, out)
+    # scores of 8 products of up to 25 or so, and a few roundings of what is no larger than 5
+    assert np.abs(out.download()[:, :, 0] - np.einsum("bht,bhtd->bhd", p, v.astype(np.float64))).max() < 2.0 ** -15
+    got_w = w.download()
+    assert np.abs(got_w - p).max() < 2.0 ** -17
+    kept = sdk.tensor("u32", (batch, kv, 2))
+    sdk.call("tensor_kv_cache_evict", cache, w, 0, 0, 2, target, None, kept)
+    index = np.sort(np.argsort(-got_w.astype(np.float64), axis=-1, kind="stable")[..., :2], axis=-1)
+    assert np.array_equal(kept.download(), index)
+    out_k, out_v = sdk.tensor("f16", (batch, kv, 2, dim)), sdk.tensor("f16", (batch, kv, 2, dim))
+    sdk.call("tensor_kv_cache_read_f16", target, out_k, out_v)
+    assert_bits_equal(out_k.download(), np.take_along_axis(k, index[..., None], 2), "kept keys")
+    assert_bits_equal(out_v.download(), np.take_along_axis(v, index[..., None], 2), "kept values")
+    assert target.lengths == [2] * batch
