@@ -109,9 +109,9 @@ int tensor_kv_cache_read_f16(const TensorKvCache *cache, TensorBuffer *key,
    weights, F32 [batch, kv_heads, tokens] with tokens at least the longest
    length, or NULL: weights[b, h, t] += the softmax weight that token t got,
    summed over the rows and query heads of kv head h (rows whose output is not
-   finite, and padded ones, add nothing). They go by scores
-   rounded to f32, each weight off by 2^-24 of its score; f32 outputs go by
-   what that rounding takes off as well. */
+   finite, and padded ones, add nothing). They go by scores rounded to f32,
+   each weight off by 2^-24 of its score; f32 outputs go by what that rounding
+   takes off as well. */
 int tensor_kv_cache_attention_f32(const TensorKvCache *cache,
                                   const TensorBuffer *query,
                                   const uint32_t *counts, float scale,

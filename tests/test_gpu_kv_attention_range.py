@@ -70,6 +70,19 @@ CAPACITIES = [("f16", 4, 2, 8, 1, 330000, 16, 256), ("f16", 64, 4, 16, 1, 10400,
 
 @pytest.mark.parametrize("shape", CAPACITIES, ids=str)
 def test_recorded_weights_of_few_rows_in_a_large_cache(sdk, shape):
+    check_replays(sdk, shape)
+
+
+# as many rows and so large a capacity that the tile kernel is recorded, in key parts
+# that the cache does not reach and in one
+@pytest.mark.parametrize("shape", [("f16", 4, 2, 8, 20, 40000, 16, 256), ("f32", 4, 2, 8, 30, 40000, 16, 128),
+                                   ("f16", 64, 4, 8, 150, 2600, 32, 32), ("f16", 2, 2, 4, 200, 60000, 64, 64)], ids=str)
+def test_recorded_tiles_in_a_large_cache(sdk, shape):
+    check_replays(sdk, shape)
+
+
+def check_replays(sdk, shape):
+    """A call recorded at a hundred tokens, replayed as the cache grows."""
     dtype, batch, kv, heads, n, capacity, dim, vdim = shape
     hip = sdk.lib
     hip.tensor_device_hip_stream.restype = ctypes.c_void_p
