@@ -26,14 +26,15 @@
  *     is queued, and a call that is refused leaves the cache as it was. Should
  *     the runtime fail to launch a kernel, the sequences of the launches before
  *     it (256 in each) are done and the others as they were, and the lengths
- *     say which; of an eviction the target is as it was;
+ *     say which; of an eviction the target is as it was, of a
+ *     reorder the cache;
  *   - `counts`, where a call takes it, is a host array of `batch` numbers: of
  *     sequence b only the first counts[b] tokens (or query rows) are there and
  *     the rest of its rows is padding, neither read nor written. NULL: all are
  *     there;
- *   - append, truncate and evict change lengths and are refused while the SDK
- *     stream records a graph. Attention and read may be recorded: a replay
- *     works on what the cache then holds;
+ *   - append, truncate, evict and copy change lengths and are refused while the
+ *     SDK stream records a graph. Attention, read and reorder may be recorded: a
+ *     replay works on what the cache then holds;
  *   - calls from several host threads are safe; a cache is freed, and replayed
  *     graphs that use it are destroyed, when no call uses it.
  */
@@ -143,6 +144,54 @@ int tensor_kv_cache_evict(const TensorKvCache *cache,
                           size_t recent, size_t keep, TensorKvCache *target,
                           TensorBuffer *target_weights, TensorBuffer *kept,
                           char *error, size_t error_capacity);
+
+/* ---- several continuations of one prompt ---------------------------------- */
+
+/* An entry of `source` that leaves its sequence of the target as it is. */
+#define TENSOR_KV_CACHE_KEEP UINT32_MAX
+
+/* Sequence b of `target` becomes a copy, as it is held, of sequence source[b] of
+   `cache` (a host array of the target's batch; an entry may be repeated):
+   a prompt into its beams or a free slot, a batch closed up. The target has the
+   cache's heads and dims, room for what it gets, and any batch and capacity. It
+   may be the cache itself, where no sequence that is copied is replaced. Changes
+   lengths: not recorded into a graph. */
+int tensor_kv_cache_copy(const TensorKvCache *cache, const uint32_t *source,
+                         TensorKvCache *target, char *error,
+                         size_t error_capacity);
+
+/* Beams follow their choice (tensor_beam_select, tensor_ops_ext.h), in place: with
+   parents U32 [groups, beams], groups * beams the cache's batch, sequence
+   g * beams + i becomes what sequence g * beams + parents[g, i] was. 1 to 64
+   beams. The parents are on the device: the call does not wait for them, and an
+   index not below `beams` leaves its sequence as it is. The sequences of a group
+   are of one length, at each replay of a recorded call too. */
+int tensor_kv_cache_reorder(TensorKvCache *cache, const TensorBuffer *parents,
+                            char *error, size_t error_capacity);
+
+/* tensor_kv_cache_attention of sequences whose tokens follow a prefix that
+   several of them share: the first members[0] sequences of `cache` continue
+   sequence 0 of `prefix`, the next members[1] sequence 1, and so on (host
+   array of the prefix's batch, zeros allowed, in all the cache's batch; NULL:
+   equal groups). Each query row sees every token of its prefix and, of its
+   sequence's own tokens in `cache`, those that tensor_kv_cache_attention lets it
+   see; one softmax goes over both. A prefix's tokens are read once for all of its
+   sequences, or once for many. The caches have the same heads and dims. Query
+   rows of all sequences and heads together: at most 2^26. */
+int tensor_kv_cache_attention_shared_f32(const TensorKvCache *prefix,
+                                         const TensorKvCache *cache,
+                                         const TensorBuffer *query,
+                                         const uint32_t *members,
+                                         const uint32_t *counts, float scale,
+                                         int causal, TensorBuffer *output,
+                                         char *error, size_t error_capacity);
+int tensor_kv_cache_attention_shared_f16(const TensorKvCache *prefix,
+                                         const TensorKvCache *cache,
+                                         const TensorBuffer *query,
+                                         const uint32_t *members,
+                                         const uint32_t *counts, float scale,
+                                         int causal, TensorBuffer *output,
+                                         char *error, size_t error_capacity);
 
 #ifdef __cplusplus
 }

@@ -187,6 +187,39 @@ int tensor_argmax_f32(const TensorBuffer *input, TensorBuffer *index_output,
 int tensor_argmax_f16(const TensorBuffer *input, TensorBuffer *index_output,
                       char *error, size_t error_capacity);
 
+/* ---- beam search ---------------------------------------------------------- */
+
+/* One step's choice over beams and vocabulary. Of each group the `keep`
+   candidates (beam b, token v) of largest score
+       scores[b] + logits[b, v] - log(sum_v exp(logits[b, v])),
+   in that order, compared in 64 bits (of equal ones the lower beam, then the larger
+   logit, then the lower token): parents[j] = b, tokens[j] = v, new_scores[j]
+   the score rounded to f32, and new_ended[j] = (v == end_token).
+   logits [groups, beams, vocab], scores F32 [groups, beams], ended U32 [groups,
+   beams] or NULL, parents and tokens U32 and new_scores F32 [groups, keep],
+   new_ended U32 [groups, keep] or NULL. 1 to 64 beams, keep 1 to 64, vocab up
+   to 2^26, groups * beams up to 2^24. new_scores may be scores, and new_ended may be
+   ended; the other outputs are tensors of their own.
+   A beam with ended[b] != 0 has one candidate: end_token, at scores[b]; its
+   logits are not looked at. Logits of -inf are no candidates, nor is a beam's any
+   where its score or one of its logits is NaN; with logits of +inf, as in
+   tensor_softmax, those share the probability. Where a group has fewer than
+   `keep` candidates (of a score above -inf), the rest is parent 0, end_token and
+   a score of -inf.
+   No reference op (closed form). */
+int tensor_beam_select_f32(const TensorBuffer *logits,
+                           const TensorBuffer *scores,
+                           const TensorBuffer *ended, uint32_t end_token,
+                           TensorBuffer *parents, TensorBuffer *tokens,
+                           TensorBuffer *new_scores, TensorBuffer *new_ended,
+                           char *error, size_t error_capacity);
+int tensor_beam_select_f16(const TensorBuffer *logits,
+                           const TensorBuffer *scores,
+                           const TensorBuffer *ended, uint32_t end_token,
+                           TensorBuffer *parents, TensorBuffer *tokens,
+                           TensorBuffer *new_scores, TensorBuffer *new_ended,
+                           char *error, size_t error_capacity);
+
 /* ---- rotary position embedding ----------------------------------------- */
 
 /* Split-half (NeoX) RoPE applied in place to query [seq, query_heads,

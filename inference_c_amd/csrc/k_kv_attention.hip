@@ -118,11 +118,13 @@ template <bool kStream, typename V> __device__ inline V load_codes(const V *p) {
 // registers when a wave starts: the struct behind them takes a microsecond to
 // arrive. (8 x 4096 tokens, from the wave's start to its first loads' issue: 2 us
 // out of 12 with the struct alone.)
-template <typename S, uint32_t P, bool kStream>
+// kShared: a pass of attention over a prefix and own tokens.
+template <typename S, uint32_t P, bool kStream, bool kShared>
 __global__ __launch_bounds__(kThreads) void kv_rows_kernel(const uint8_t *keys, const uint8_t *values,
                                                            const uint32_t *lengths, const Meta *metas, const S *queries,
                                                            uint32_t all_blocks, uint32_t heads, uint32_t parts_first,
-                                                           uint32_t pitches, uint32_t n, uint32_t group, Args<S> a) {
+                                                           uint32_t pitches, uint32_t n, uint32_t group,
+                                                           typename ArgsOf<S, kShared>::type a) {
     constexpr bool kPair = sizeof(S) == 4;
     constexpr uint32_t NC = P / 64, NV = P / 16;
     constexpr bool kOdd = P % 64 != 0;
@@ -188,7 +190,8 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(const uint8_t *keys, 
     const uint32_t end = min(begin + share, blocks), end_whole = min(end, whole);
     const uint32_t r = row0 + m, i = n == 1 ? 0 : r % n;
     const bool live = r < in_head && i < count;
-    const size_t row = head * in_head + (r < in_head ? r : in_head - 1);   // (rows past the head repeat its last)
+    size_t row = head * in_head + (r < in_head ? r : in_head - 1);   // (rows past the head repeat its last)
+    if constexpr (kShared) row = shared_row(a, r, b, h, in_head, count);
     const int seen = seen_by(i, live, length, count, a.causal);
     Query<S, P> q;
     q.load(queries + row * c.dim, c.dim, g);
@@ -364,7 +367,7 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(const uint8_t *keys, 
         total_exact += w[k] * lds_ml[k][m].z;
     }
     const bool writes = live && r < in_head;
-    if (parts == 1) {
+    if (!kShared && parts == 1) {
         S *const out = a.out + row * c.vdim;
 #pragma unroll
         for (uint32_t j = wave; j < NV; j += kWaves) {
@@ -599,55 +602,70 @@ Plan plan_of(bool f32, const View &c, const AttentionShape &a) {
 // (67 MB, found there by calls in a row): 19.5, as a stream 20.6.
 constexpr size_t kStreamBytes = size_t{192} << 20;
 
-template <typename S, uint32_t P>
-hipError_t launch_rows(const Args<S> &a, uint32_t groups, hipStream_t s) {
+template <typename S, uint32_t P, bool kShared>
+hipError_t launch_rows(const typename ArgsOf<S, kShared>::type &a, uint32_t groups, hipStream_t s) {
     const dim3 grid(groups * a.parts, a.c.heads, a.pairs / a.c.heads);
     const size_t bytes = (size_t)a.pairs * a.longest * (a.c.kp + a.c.vp);
-    const auto kernel = bytes > kStreamBytes ? kv_rows_kernel<S, P, true> : kv_rows_kernel<S, P, false>;
+    const auto kernel = bytes > kStreamBytes ? kv_rows_kernel<S, P, true, kShared> : kv_rows_kernel<S, P, false, kShared>;
     kernel<<<grid, kThreads, 0, s>>>(a.c.k, a.c.v, a.c.length, a.c.meta, a.q, a.c.blocks, a.c.heads,
                                      a.parts | a.first << 16, a.c.kp | a.c.vp << 16, a.n, a.group, a);
     return hipGetLastError();
 }
-template <typename S>
-hipError_t launch_rows(const Args<S> &a, uint32_t widest, uint32_t groups, hipStream_t s) {
-    if (widest <= 32) return launch_rows<S, 32>(a, groups, s);
-    if (widest <= 64) return launch_rows<S, 64>(a, groups, s);
-    if (widest <= 96) return launch_rows<S, 96>(a, groups, s);
-    if (widest <= 128) return launch_rows<S, 128>(a, groups, s);
-    if (widest <= 192) return launch_rows<S, 192>(a, groups, s);
-    return launch_rows<S, 256>(a, groups, s);
+template <typename S, bool kShared>
+hipError_t launch_rows(const typename ArgsOf<S, kShared>::type &a, uint32_t widest, uint32_t groups, hipStream_t s) {
+    if (widest <= 32) return launch_rows<S, 32, kShared>(a, groups, s);
+    if (widest <= 64) return launch_rows<S, 64, kShared>(a, groups, s);
+    if (widest <= 96) return launch_rows<S, 96, kShared>(a, groups, s);
+    if (widest <= 128) return launch_rows<S, 128, kShared>(a, groups, s);
+    if (widest <= 192) return launch_rows<S, 192, kShared>(a, groups, s);
+    return launch_rows<S, 256, kShared>(a, groups, s);
 }
 
-template <typename S>
-hipError_t launch(Args<S> a, const Plan &p, uint32_t batch, uint32_t longest, float *partial, hipStream_t s) {
-    const uint32_t blocks = (longest + kTokens - 1) / kTokens, widest = widest_of(a.c);
+// The rows' (or tiles') launches of a plan.
+template <typename S, bool kShared>
+hipError_t launch_pass(typename ArgsOf<S, kShared>::type a, const Plan &p, hipStream_t s) {
+    const uint32_t widest = widest_of(a.c);
     // (a launch holds fewer than 2^32 threads)
     const uint32_t most = (1u << 23) / (a.pairs * p.parts) < 1 ? 1 : (1u << 23) / (a.pairs * p.parts);
     for (uint32_t g0 = 0; g0 < p.row_groups; g0 += most) {
         a.row_group0 = g0;
         const uint32_t groups = p.row_groups - g0 < most ? p.row_groups - g0 : most;
-        const hipError_t status = p.tiles ? launch_tiles(a, widest, groups, s) : launch_rows(a, widest, groups, s);
+        const hipError_t status = p.tiles ? launch_tiles<S, kShared>(a, widest, groups, s)
+                                          : launch_rows<S, kShared>(a, widest, groups, s);
         if (status != hipSuccess) return status;
     }
-    if (p.parts > 1 || p.scores) {
-        // (at most 512 row groups where there are parts)
-        const uint32_t folds = p.parts > 1 ? a.pairs * a.group * a.n : 0;
-        const uint32_t threads = p.parts > 16 ? 16 * kWave : kThreads;
-        const uint32_t token_groups = p.scores ? (blocks * kTokens + threads - 1) / threads : 0;
-        const uint32_t workgroups = p.parts <= kWaves ? (folds + kWaves - 1) / kWaves : folds;
-        const uint32_t grid = workgroups + a.pairs * token_groups;
-        if (grid == 0) return hipSuccess;
-        auto fold = [&](auto kernel) {
-            kernel<<<grid, threads, 0, s>>>(a.part_o, a.part_ml, a.rows, p.parts, a.n, a.group * a.n, a.c.vdim, workgroups,
-                                            a.first * a.c.heads * a.group * a.n, token_groups, folds, a);
-        };
-        if (p.parts <= kWaves) fold(kv_fold_kernel<S, kWaves, 1>);
-        else if (threads == kThreads) fold(kv_fold_kernel<S, kWaves, kWaves>);
-        else fold(kv_fold_kernel<S, 16, 16>);
-        const hipError_t status = hipGetLastError();
-        if (status != hipSuccess) return status;
-    }
-    if (a.row_ml != nullptr && blocks > 0) return launch_weights(a, widest, batch, blocks, p.row_parts, partial, s);
+    return hipSuccess;
+}
+
+// Joins `parts` parts of the rows of a launch's sequences; its workgroups after those
+// take weights from the stored scores, if there are any.
+template <typename S>
+hipError_t launch_fold(const Args<S> &a, uint32_t parts, bool scores, uint32_t longest, hipStream_t s) {
+    const uint32_t blocks = (longest + kTokens - 1) / kTokens;
+    // (at most 512 row groups where there are parts)
+    const uint32_t folds = parts > 1 ? a.pairs * a.group * a.n : 0;
+    const uint32_t threads = parts > 16 ? 16 * kWave : kThreads;
+    const uint32_t token_groups = scores ? (blocks * kTokens + threads - 1) / threads : 0;
+    const uint32_t workgroups = parts <= kWaves ? (folds + kWaves - 1) / kWaves : folds;
+    const uint32_t grid = workgroups + a.pairs * token_groups;
+    if (grid == 0) return hipSuccess;
+    auto fold = [&](auto kernel) {
+        kernel<<<grid, threads, 0, s>>>(a.part_o, a.part_ml, a.rows, parts, a.n, a.group * a.n, a.c.vdim, workgroups,
+                                        a.first * a.c.heads * a.group * a.n, token_groups, folds, a);
+    };
+    if (parts <= kWaves) fold(kv_fold_kernel<S, kWaves, 1>);
+    else if (threads == kThreads) fold(kv_fold_kernel<S, kWaves, kWaves>);
+    else fold(kv_fold_kernel<S, 16, 16>);
+    return hipGetLastError();
+}
+
+template <typename S>
+hipError_t launch(const Args<S> &a, const Plan &p, uint32_t batch, uint32_t longest, float *partial, hipStream_t s) {
+    const uint32_t blocks = (longest + kTokens - 1) / kTokens;
+    hipError_t status = launch_pass<S, false>(a, p, s);
+    if (status == hipSuccess && (p.parts > 1 || p.scores)) status = launch_fold(a, p.parts, p.scores, longest, s);
+    if (status != hipSuccess) return status;
+    if (a.row_ml != nullptr && blocks > 0) return launch_weights(a, widest_of(a.c), batch, blocks, p.row_parts, partial, s);
     return hipSuccess;
 }
 
@@ -694,6 +712,92 @@ hipError_t run(const View &c, const AttentionShape &sh, const void *query, void 
     return hipSuccess;
 }
 
+// ---- a prefix and own tokens ---------------------------------------------------------
+
+// Attention of sequences whose tokens follow a prefix that several of them share, in
+// two passes into the same rows' parts: over the prefix the rows of a group's sequences
+// are packed as one head's rows, so that its codes are read once for all of them, then
+// over each sequence's own tokens. A softmax over both is their parts' join.
+struct SharedPlan {
+    AttentionShape over;   // of the pass over the prefix
+    Plan prefix, own;
+    size_t rows, o_bytes, ml_bytes;
+};
+
+SharedPlan plan_of(bool f32, const View &prefix, const PrefixShape &ps, const View &c, const AttentionShape &a) {
+    SharedPlan p;
+    p.over = AttentionShape{ps.batch, prefix.heads, ps.most * (a.q_heads / c.heads) * a.n, ps.longest, a.scale, false,
+                            nullptr, nullptr, 0, 0};
+    p.prefix = plan_of(f32, prefix, p.over);
+    p.own = plan_of(f32, c, a);
+    p.rows = p.own.rows;
+    const size_t parts = p.prefix.parts + p.own.parts;
+    p.o_bytes = whole256(parts * p.rows * c.vdim * 4);
+    p.ml_bytes = whole256(parts * p.rows * sizeof(f32x2));
+    return p;
+}
+
+template <typename S>
+hipError_t run_shared(const View &prefix, const PrefixShape &ps, const View &c, const AttentionShape &sh,
+                      const void *query, void *output, void *workspace, hipStream_t s) {
+    const SharedPlan p = plan_of(sizeof(S) == 4, prefix, ps, c, sh);
+    const uint32_t group = sh.q_heads / c.heads;
+    SharedArgs<S> a{};
+    a.q = static_cast<const S *>(query);
+    a.out = static_cast<S *>(output);
+    a.part_o = static_cast<float *>(workspace);
+    a.part_ml = reinterpret_cast<f32x2 *>(static_cast<char *>(workspace) + p.o_bytes);
+    a.rows = p.rows;
+    a.scale2 = (double)sh.scale * kLog2e;
+    a.own_rows = group * sh.n;
+    // a group's rows are one head's rows here, all of them there
+    a.c = prefix;
+    a.group = 1;
+    a.n = p.over.n;
+    a.parts = p.prefix.parts;
+    a.longest = ps.longest;
+    a.row_groups = p.prefix.row_groups;
+    uint32_t sequence = 0;
+    for (uint32_t first = 0; first < ps.batch; first += kBatchPerLaunch) {
+        const uint32_t batch = ps.batch - first < kBatchPerLaunch ? ps.batch - first : kBatchPerLaunch;
+        for (uint32_t b = 0; b < batch; ++b) {
+            a.member.n[b] = ps.members[first + b] != 0 ? sequence : 0;   // (of none, a row that is there)
+            a.count.n[b] = ps.members[first + b] * a.own_rows;
+            sequence += ps.members[first + b];
+        }
+        a.first = first;
+        a.pairs = batch * c.heads;
+        const hipError_t status = launch_pass<S, true>(a, p.prefix, s);
+        if (status != hipSuccess) return status;
+    }
+    a.c = c;
+    a.group = group;
+    a.n = sh.n;
+    a.parts = p.own.parts;
+    a.longest = sh.longest;
+    a.row_groups = p.own.row_groups;
+    a.causal = sh.causal;
+    float *const part_o = a.part_o;
+    f32x2 *const part_ml = a.part_ml;
+    for (uint32_t first = 0; first < sh.batch; first += kBatchPerLaunch) {
+        const uint32_t batch = sh.batch - first < kBatchPerLaunch ? sh.batch - first : kBatchPerLaunch;
+        for (uint32_t b = 0; b < batch; ++b) {
+            a.member.n[b] = first + b;
+            a.count.n[b] = sh.counts ? sh.counts[first + b] : sh.n;
+        }
+        a.first = first;
+        a.pairs = batch * c.heads;
+        a.part_o = part_o + (size_t)p.prefix.parts * p.rows * c.vdim;
+        a.part_ml = part_ml + (size_t)p.prefix.parts * p.rows;
+        hipError_t status = launch_pass<S, true>(a, p.own, s);
+        a.part_o = part_o;
+        a.part_ml = part_ml;
+        if (status == hipSuccess) status = launch_fold<S>(a, p.prefix.parts + p.own.parts, false, 0, s);
+        if (status != hipSuccess) return status;
+    }
+    return hipSuccess;
+}
+
 }  // namespace
 
 size_t attention_workspace(bool f32, const View &c, const AttentionShape &a) { return plan_of(f32, c, a).bytes(); }
@@ -701,6 +805,18 @@ size_t attention_workspace(bool f32, const View &c, const AttentionShape &a) { r
 hipError_t attention(bool f32, const View &c, const AttentionShape &a, const void *query, void *output,
                      void *workspace, hipStream_t s) {
     return f32 ? run<float>(c, a, query, output, workspace, s) : run<_Float16>(c, a, query, output, workspace, s);
+}
+
+size_t attention_shared_workspace(bool f32, const View &prefix, const PrefixShape &p, const View &c,
+                                  const AttentionShape &a) {
+    const SharedPlan plan = plan_of(f32, prefix, p, c, a);
+    return plan.o_bytes + plan.ml_bytes;
+}
+
+hipError_t attention_shared(bool f32, const View &prefix, const PrefixShape &p, const View &c, const AttentionShape &a,
+                            const void *query, void *output, void *workspace, hipStream_t s) {
+    return f32 ? run_shared<float>(prefix, p, c, a, query, output, workspace, s)
+               : run_shared<_Float16>(prefix, p, c, a, query, output, workspace, s);
 }
 
 }  // namespace kv

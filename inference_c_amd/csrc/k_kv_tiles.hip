@@ -146,8 +146,10 @@ __device__ inline void steps(R operand, M product, W work) {
 // workgroups), two groups of four waves a phase apart (332 us), first operands of a
 // phase asked for in the one before (1%).
 // kExact: with the sum of P before its rounding to f16 too, for the weights.
-template <typename S, uint32_t P, bool kExact>
-__global__ __launch_bounds__(kThreads, tiles_twice(sizeof(S) == 4, P) ? 2 : 1) void kv_tiles_kernel(Args<S> a) {
+// kShared: a pass of attention over a prefix and own tokens.
+template <typename S, uint32_t P, bool kExact, bool kShared>
+__global__ __launch_bounds__(kThreads, tiles_twice(sizeof(S) == 4, P) ? 2 : 1) void kv_tiles_kernel(
+    typename ArgsOf<S, kShared>::type a) {
     constexpr bool kPair = sizeof(S) == 4;
     static_assert(!kPair || !kExact);   // (its sum is exact by itself)
     constexpr uint32_t KC = P / 16, VT = (P + 31) / 32;
@@ -173,7 +175,8 @@ __global__ __launch_bounds__(kThreads, tiles_twice(sizeof(S) == 4, P) ? 2 : 1) v
     const uint32_t length = c.length[seq], count = a.count.n[b];
     const uint32_t r = row_block * kTileRows + wave * 32 + col, i = r % a.n;
     const bool live = r < in_head && i < count;
-    const size_t row = head * in_head + min(r, in_head - 1);
+    size_t row = head * in_head + min(r, in_head - 1);
+    if constexpr (kShared) row = shared_row(a, r, b, h, in_head, count);
     const int seen = seen_by(i, live, length, count, a.causal);
     // keys that some row of the workgroup, and that every row of the wave, sees
     int most = live ? seen : 0, least = live ? seen : (int)length;
@@ -474,7 +477,7 @@ __global__ __launch_bounds__(kThreads, tiles_twice(sizeof(S) == 4, P) ? 2 : 1) v
     exact = kExact ? flash::pair_sum(exact) : sum;
     big -= kHeadroom<S>;
     if (!live) return;
-    const bool direct = a.parts == 1;
+    const bool direct = !kShared && a.parts == 1;
 #pragma unroll
     for (uint32_t v = 0; v < VT; ++v)
 #pragma unroll
@@ -705,16 +708,16 @@ __global__ __launch_bounds__(kThreads) void kv_weights_add_kernel(Args<S> a, uin
     a.weights[((size_t)seq * c.heads + h) * a.weight_stride + t] += total;
 }
 
-template <typename S, uint32_t P>
-hipError_t tiles(const Args<S> &a, uint32_t groups, hipStream_t s) {
+template <typename S, uint32_t P, bool kShared>
+hipError_t tiles(const typename ArgsOf<S, kShared>::type &a, uint32_t groups, hipStream_t s) {
     const dim3 grid(groups * a.pairs * a.parts);
-    if constexpr (sizeof(S) == 2) {
+    if constexpr (sizeof(S) == 2 && !kShared) {
         if (a.weights != nullptr) {
-            kv_tiles_kernel<S, P, true><<<grid, kThreads, 0, s>>>(a);
+            kv_tiles_kernel<S, P, true, false><<<grid, kThreads, 0, s>>>(a);
             return hipGetLastError();
         }
     }
-    kv_tiles_kernel<S, P, false><<<grid, kThreads, 0, s>>>(a);
+    kv_tiles_kernel<S, P, false, kShared><<<grid, kThreads, 0, s>>>(a);
     return hipGetLastError();
 }
 
@@ -733,15 +736,15 @@ hipError_t weights(const Args<S> &a, uint32_t batch, uint32_t blocks, uint32_t r
 
 bool tiles_fit(bool f32, uint32_t widest) { return !f32 || widest <= 128; }
 
-template <typename S>
-hipError_t launch_tiles(const Args<S> &a, uint32_t widest, uint32_t groups, hipStream_t s) {
-    if (widest <= 32) return tiles<S, 32>(a, groups, s);
-    if (widest <= 64) return tiles<S, 64>(a, groups, s);
-    if (widest <= 96) return tiles<S, 96>(a, groups, s);
-    if (widest <= 128) return tiles<S, 128>(a, groups, s);
+template <typename S, bool kShared>
+hipError_t launch_tiles(const typename ArgsOf<S, kShared>::type &a, uint32_t widest, uint32_t groups, hipStream_t s) {
+    if (widest <= 32) return tiles<S, 32, kShared>(a, groups, s);
+    if (widest <= 64) return tiles<S, 64, kShared>(a, groups, s);
+    if (widest <= 96) return tiles<S, 96, kShared>(a, groups, s);
+    if (widest <= 128) return tiles<S, 128, kShared>(a, groups, s);
     if constexpr (sizeof(S) == 2) {
-        if (widest <= 192) return tiles<S, 192>(a, groups, s);
-        return tiles<S, 256>(a, groups, s);
+        if (widest <= 192) return tiles<S, 192, kShared>(a, groups, s);
+        return tiles<S, 256, kShared>(a, groups, s);
     }
     return hipErrorInvalidValue;
 }
@@ -757,8 +760,10 @@ hipError_t launch_weights(const Args<S> &a, uint32_t widest, uint32_t batch, uin
     return weights<S, 256>(a, batch, blocks, row_parts, partial, s);
 }
 
-template hipError_t launch_tiles<float>(const Args<float> &, uint32_t, uint32_t, hipStream_t);
-template hipError_t launch_tiles<_Float16>(const Args<_Float16> &, uint32_t, uint32_t, hipStream_t);
+template hipError_t launch_tiles<float, false>(const Args<float> &, uint32_t, uint32_t, hipStream_t);
+template hipError_t launch_tiles<_Float16, false>(const Args<_Float16> &, uint32_t, uint32_t, hipStream_t);
+template hipError_t launch_tiles<float, true>(const SharedArgs<float> &, uint32_t, uint32_t, hipStream_t);
+template hipError_t launch_tiles<_Float16, true>(const SharedArgs<_Float16> &, uint32_t, uint32_t, hipStream_t);
 template hipError_t launch_weights<float>(const Args<float> &, uint32_t, uint32_t, uint32_t, uint32_t, float *, hipStream_t);
 template hipError_t launch_weights<_Float16>(const Args<_Float16> &, uint32_t, uint32_t, uint32_t, uint32_t, float *,
                                              hipStream_t);

@@ -88,6 +88,18 @@ hipError_t argmax_f32(const float *x, size_t n, uint32_t *index_out, void *parti
 hipError_t argmax_f16(const uint16_t *x, size_t n, uint32_t *index_out, void *partials,
                       hipStream_t s);
 
+// Beam search's choice (k_beam.hip): logits [groups, beams, vocab], scores and ended
+// (may be null) [groups, beams], outputs [groups, keep] (new_ended may be null).
+// At least one group; `workspace`: beam_select_workspace bytes of device scratch.
+constexpr uint32_t kBeamMax = 64, kBeamMaxKeep = 64;
+struct BeamShape {
+    size_t groups, beams, vocab, keep;
+};
+size_t beam_select_workspace(const BeamShape &b, bool f32);
+hipError_t beam_select(bool f32, const BeamShape &b, const void *logits, const float *scores, const uint32_t *ended,
+                       uint32_t end_token, uint32_t *parents, uint32_t *tokens, float *new_scores, uint32_t *new_ended,
+                       void *workspace, hipStream_t s);
+
 // In-place split-half RoPE on q [seq, qh, dim] and k [seq, kh, dim].
 // Shapes whose half row is a multiple of the 16-byte vector (<= 128 pairs,
 // aligned tensors) need no scratch; others need `table`, device scratch of

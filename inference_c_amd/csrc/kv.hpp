@@ -1,6 +1,6 @@
 // The 8-bit key/value cache in device memory, and the launchers of its kernels
-// (k_kv_cache.hip: append, read, truncate, evict; k_kv_attention.hip:
-// attention).
+// (k_kv_cache.hip: append, read, truncate, evict; k_kv_copy.hip: copy, reorder;
+// k_kv_attention.hip: attention).
 //
 // Of each (sequence, kv head), in blocks of 64 tokens:
 //   k     [block][token][kp]   codes + 128 as bytes, kp = head dim in whole 16s
@@ -69,6 +69,18 @@ struct EvictArgs {
 };
 hipError_t evict(const View &from, const View &to, uint32_t batch, const EvictArgs &a, hipStream_t s);
 
+// Sequences first .. first + batch - 1 of `to` become copies of sequences source[b] of
+// `from` (kKeep: stay as they are); `longest` bounds the sources' lengths. `to` may be
+// `from` where no sequence is both read and written.
+constexpr uint32_t kKeep = 0xffffffffu;
+hipError_t copy(const View &from, const View &to, uint32_t first, uint32_t batch, const Counts &source, uint32_t longest,
+                hipStream_t s);
+// In each group of `beams` sequences (of one length, at most `longest`), sequence i
+// becomes what sequence parents[i] was.
+constexpr uint32_t kMaxBeams = 64;
+hipError_t reorder(const View &c, uint32_t groups, uint32_t beams, const uint32_t *parents, uint32_t longest,
+                   hipStream_t s);
+
 struct AttentionShape {
     uint32_t batch, q_heads, n;   // n query rows per head
     uint32_t longest;             // bound of the lengths, for the plan
@@ -83,6 +95,18 @@ struct AttentionShape {
 size_t attention_workspace(bool f32, const View &c, const AttentionShape &a);
 hipError_t attention(bool f32, const View &c, const AttentionShape &a, const void *query, void *output,
                      void *workspace, hipStream_t s);
+
+// The same with the tokens of `prefix` before each sequence's own: sequences of `c`
+// lie in groups, one per sequence of the prefix, of members[p] each (host; `most`: the
+// largest). No weights.
+struct PrefixShape {
+    uint32_t batch, most, longest;
+    const uint32_t *members;
+};
+size_t attention_shared_workspace(bool f32, const View &prefix, const PrefixShape &p, const View &c,
+                                  const AttentionShape &a);
+hipError_t attention_shared(bool f32, const View &prefix, const PrefixShape &p, const View &c, const AttentionShape &a,
+                            const void *query, void *output, void *workspace, hipStream_t s);
 
 }  // namespace kv
 }  // namespace icsdk

@@ -52,6 +52,27 @@ template <typename S> struct Args {
     Counts count;
 };
 
+// Of a pass that goes with another one into the same rows' parts: attention over a
+// prefix and over the sequences' own tokens (k_kv_attention.hip). A packed row of
+// (sequence, head) of the pass's cache is row r % own_rows of that head of sequence
+// member.n[b] + r / own_rows of q and the parts. Outputs are parts, however few.
+template <typename S> struct SharedArgs : Args<S> {
+    uint32_t own_rows;
+    Counts member;
+};
+template <typename S, bool kShared> struct ArgsOf { typedef Args<S> type; };
+template <typename S> struct ArgsOf<S, true> { typedef SharedArgs<S> type; };
+
+// The row of q, the parts and the output that packed row r of sequence first + b and
+// head h is (rows that are not there repeat the last that is).
+template <typename S>
+__device__ inline size_t shared_row(const SharedArgs<S> &a, uint32_t r, uint32_t b, uint32_t h, uint32_t in_head,
+                                    uint32_t count) {
+    r = min(r, in_head - a.n + max(count, 1u) - 1);
+    const uint32_t m = r / a.own_rows;
+    return ((size_t)(a.member.n[b] + m) * a.c.heads + h) * a.own_rows + (r - m * a.own_rows);
+}
+
 // A block's Meta through the scalar cache (no kernel writes it while one that
 // reads it runs): a vector load would wait in line with the codes asked for ahead.
 __device__ inline Meta scalar_meta(const Meta *at) {
@@ -141,8 +162,8 @@ constexpr uint32_t kTileRows = 128;
 bool tiles_fit(bool f32, uint32_t widest);
 // Whether a CU holds two of its workgroups (their registers decide).
 constexpr bool tiles_twice(bool f32, uint32_t widest) { return !f32 && widest <= 128; }
-template <typename S>
-hipError_t launch_tiles(const Args<S> &a, uint32_t widest, uint32_t groups, hipStream_t s);
+template <typename S, bool kShared>
+hipError_t launch_tiles(const typename ArgsOf<S, kShared>::type &a, uint32_t widest, uint32_t groups, hipStream_t s);
 // Weights from the rows' maxima and sums; row_parts > 1: `partial` holds row_parts
 // sums for each token of every (sequence, head).
 template <typename S>

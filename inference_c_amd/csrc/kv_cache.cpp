@@ -5,41 +5,22 @@
 // and on the device, where the kernels that change a cache set it and the
 // others read it (so that a recorded read or attention works on what the cache
 // holds when it is replayed).
-#include "kv.hpp"
-#include "sdk.hpp"
-
-#include "tensor_kv_cache.h"
+#include "kv_handle.hpp"
 
 #include <climits>
 #include <cmath>
 #include <cstdlib>
-#include <mutex>
 #include <new>
 
 using namespace icsdk;
 
-struct TensorKvCache {
-    std::mutex mutex;
-    size_t batch, capacity, bytes;
-    kv::View view;
-    void *memory;
-    uint32_t *length;   // [batch]
-};
-
 namespace {
-
-using Buf = const TensorBuffer *;
 
 // A launch has fewer than 2^32 threads in a dimension: one for each token (of all
 // sequences and heads: the fold's), or 32 for each of a head's (the weights': 16
 // parts of its blocks in fours, 256 threads each).
 constexpr size_t kMaxCapacity = size_t{1} << 27, kMaxTokens = size_t{1} << 31;
 constexpr size_t kMaxBatch = 65535, kMaxHeads = 4096;
-
-int fail(char *error, size_t capacity, const char *message) {
-    set_error(error, capacity, "%s", message);
-    return 0;
-}
 
 size_t round_up(size_t n, size_t to) { return (n + to - 1) / to * to; }
 
@@ -59,43 +40,6 @@ bool layout_of(size_t batch, size_t heads, size_t blocks, size_t kp, size_t vp, 
     l->vt = l->kt + round_up(pairs * kv::kTokens * kp * 2, 256);
     l->length = l->vt + round_up(pairs * kv::kTokens * vp * 2, 256);
     l->total = l->length + round_up(batch * 4, 256);
-    return true;
-}
-
-bool device_tensor(Buf t, TensorDType dtype, size_t rank) {
-    return t != nullptr && tensor_buffer_dtype(t) == dtype && tensor_buffer_rank(t) == rank &&
-           tensor_buffer_storage(t) == TENSOR_BUFFER_STORAGE_DEVICE;
-}
-
-bool shaped(Buf t, size_t a, size_t b, size_t c) {
-    const uint64_t *s = tensor_buffer_shape(t);
-    return s[0] == a && s[1] == b && s[2] == c;
-}
-
-bool shaped(Buf t, size_t a, size_t b, size_t c, size_t d) {
-    return shaped(t, a, b, c) && tensor_buffer_shape(t)[3] == d;
-}
-
-void *dev(Buf t) { return t ? tensor_buffer_device_handle_internal(t) : nullptr; }
-
-// A call that changes lengths cannot be replayed: the host's lengths would not
-// follow.
-bool not_recording(const char *what, char *error, size_t capacity) {
-    if (sdk_recording() == Recording::kNo) return true;
-    set_error(error, capacity, "%s changes the cache's lengths and cannot be recorded into a graph", what);
-    return false;
-}
-
-uint32_t longest_of(const TensorKvCache *c) {
-    uint32_t n = 0;
-    for (size_t b = 0; b < c->batch; ++b) n = c->length[b] > n ? c->length[b] : n;
-    return n;
-}
-
-// counts[b] <= n for every sequence
-bool counts_fit(const TensorKvCache *c, const uint32_t *counts, size_t n) {
-    for (size_t b = 0; counts != nullptr && b < c->batch; ++b)
-        if (counts[b] > n) return false;
     return true;
 }
 

@@ -30,7 +30,7 @@ NUMPY_DTYPES = {
 HOST, DEVICE = 0, 1
 
 _P, _F, _D = ctypes.c_void_p, ctypes.c_float, ctypes.c_double
-_Z, _I, _U64 = ctypes.c_size_t, ctypes.c_int, ctypes.c_uint64
+_Z, _I, _U32, _U64 = ctypes.c_size_t, ctypes.c_int, ctypes.c_uint32, ctypes.c_uint64
 
 # Operation signatures, without the trailing (char *error, size_t capacity).
 OP_ARGTYPES = {
@@ -65,6 +65,11 @@ OP_ARGTYPES = {
     "tensor_kv_cache_attention_f32": [_P, _P, _P, _F, _I, _P, _P],
     "tensor_kv_cache_attention_f16": [_P, _P, _P, _F, _I, _P, _P],
     "tensor_kv_cache_evict": [_P, _P, _Z, _Z, _Z, _P, _P, _P],
+    "tensor_kv_cache_copy": [_P, _P, _P], "tensor_kv_cache_reorder": [_P, _P],
+    "tensor_kv_cache_attention_shared_f32": [_P, _P, _P, _P, _P, _F, _I, _P],
+    "tensor_kv_cache_attention_shared_f16": [_P, _P, _P, _P, _P, _F, _I, _P],
+    "tensor_beam_select_f32": [_P, _P, _P, _U32, _P, _P, _P, _P],
+    "tensor_beam_select_f16": [_P, _P, _P, _U32, _P, _P, _P, _P],
     "tensor_device_synchronize": [],
 }
 
@@ -245,8 +250,8 @@ class Tensor:
 
 class KvCache:
     """Owns one TensorKvCache: keys and values of one layer held in 8 bits.
-    Passed to Sdk.call like a Tensor; host arrays of counts or lengths are
-    ctypes arrays of c_uint32, one number per sequence."""
+    Passed to Sdk.call like a Tensor; host arrays of counts, lengths, sources or
+    members are ctypes arrays of c_uint32, one number per sequence."""
 
     def __init__(self, sdk: "Sdk", batch: int, kv_heads: int, capacity: int, head_dim: int,
                  value_dim: Optional[int] = None):
