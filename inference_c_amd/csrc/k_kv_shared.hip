@@ -1,0 +1,270 @@
+// Attention over the 8-bit cache of sequences whose tokens follow a prefix that
+// several of them share.
+//
+// Two passes into the same rows' parts: over the prefix the rows of a group's sequences
+// are packed as one head's rows, so that its codes are read once for 16 or 128 of them,
+// and over each sequence's own tokens as in attention without a prefix. A softmax over
+// both is their parts' join (kv_fold_kernel). The passes are one launch: neither waits
+// for the other, and where the prefix is bound by its products (tiles) and the own
+// tokens by memory (rows), a CU has one of each.
+#include "kv_rows.hpp"
+#include "kv_tiles.hpp"
+
+namespace icsdk {
+namespace kv {
+namespace {
+
+template <typename S> struct Both {
+    SharedArgs<S> pass[2];   // the prefix, own tokens
+    uint32_t first;          // workgroups of the first pass; those behind are the second's
+};
+
+// Workgroup i of a pass by the rows kernel.
+template <typename S, uint32_t P, bool kStream>
+__device__ __forceinline__ void rows_of(RowsOut<P> &lds_o, RowsMl &lds_ml, Constant<SharedArgs<S>> &a, uint32_t i) {
+    const uint32_t x = i % a.columns, pair = i / a.columns, h = pair % a.c.heads, b = pair / a.c.heads;
+    rows_of<S, P, kStream>(lds_o, lds_ml, a.c.k, a.c.v, a.c.length, a.c.meta, a.q, a.c.blocks, a.c.heads,
+                           a.parts | a.first << 16, a.c.kp | a.c.vp << 16, a.n, a.group, a, x, h, b);
+}
+
+template <typename S, uint32_t P, bool kStream>
+__global__ __launch_bounds__(kThreads) void kv_shared_rows_kernel(Both<S>) {
+    __shared__ RowsOut<P> lds_o;
+    __shared__ RowsMl lds_ml;
+    auto &both = kernel_arguments<Both<S>>(0);
+    const uint32_t second = blockIdx.x >= both.first ? 1 : 0;
+    rows_of<S, P, kStream>(lds_o, lds_ml, both.pass[second], blockIdx.x - (second ? both.first : 0));
+}
+
+template <typename S, uint32_t P>
+__global__ __launch_bounds__(kThreads, tiles_twice(sizeof(S) == 4, P) ? 2 : 1) void kv_shared_tiles_kernel(Both<S>) {
+    __shared__ __attribute__((aligned(16))) typename TilesLds<P>::Keys ks;
+    __shared__ __attribute__((aligned(16))) typename TilesLds<P>::Values vs;
+    __shared__ typename TilesLds<P>::Most wave_most;
+    auto &both = kernel_arguments<Both<S>>(0);
+    const uint32_t second = blockIdx.x >= both.first ? 1 : 0;
+    tiles_of<S, P, false>(ks, vs, wave_most, both.pass[second], blockIdx.x - (second ? both.first : 0));
+}
+
+// Tiles over the prefix, rows over own tokens.
+template <typename S, uint32_t P>
+__global__ __launch_bounds__(kThreads, 2) void kv_shared_mixed_kernel(Both<S>) {
+    static_assert(tiles_twice(sizeof(S) == 4, P) && sizeof(RowsOut<P>) + sizeof(RowsMl) <= sizeof(typename TilesLds<P>::Keys));
+    __shared__ __attribute__((aligned(16))) typename TilesLds<P>::Keys ks;
+    __shared__ __attribute__((aligned(16))) typename TilesLds<P>::Values vs;
+    __shared__ typename TilesLds<P>::Most wave_most;
+    auto &both = kernel_arguments<Both<S>>(0);
+    if (blockIdx.x < both.first) {
+        tiles_of<S, P, false>(ks, vs, wave_most, both.pass[0], blockIdx.x);
+    } else {
+        char *const lds = reinterpret_cast<char *>(ks);
+        rows_of<S, P, false>(*reinterpret_cast<RowsOut<P> *>(lds), *reinterpret_cast<RowsMl *>(lds + sizeof(RowsOut<P>)),
+                             both.pass[1], blockIdx.x - both.first);
+    }
+}
+
+// Rows up to which 16 waves join a row's parts: above, four do. Measured at 33 parts of
+// 2048 rows: 18 us by 16 waves, 10 by four.
+constexpr size_t kWideRows = 512;
+
+// ---- plan --------------------------------------------------------------------------------
+
+// A pass: its kernel and its workgroups.
+struct Pass {
+    bool tiles;
+    uint32_t batch, row_groups, parts;
+};
+struct SharedPlan {
+    Pass prefix, own;
+    bool together;   // in one launch
+    uint32_t n;      // rows of a prefix's head
+    size_t rows, o_bytes, ml_bytes;
+};
+
+Pass pass_of(const View &c, bool tiles, uint32_t batch, uint32_t in_head, uint32_t longest, uint64_t workgroups) {
+    Pass p{tiles, batch, 0, 1};
+    const uint32_t rows = tiles ? kTileRows : kRows, blocks = (longest + kTokens - 1) / kTokens;
+    p.row_groups = (in_head + rows - 1) / rows;
+    const uint64_t base = (uint64_t)batch * c.heads * p.row_groups, most = (blocks + kWaves - 1) / kWaves;
+    uint64_t parts = base == 0 ? 1 : workgroups / base;
+    parts = parts < most ? parts : most;
+    p.parts = parts < 1 ? 1 : (uint32_t)parts;
+    return p;
+}
+
+uint64_t workgroups_of(const View &c, const Pass &p) { return (uint64_t)p.batch * c.heads * p.row_groups * p.parts; }
+
+SharedPlan plan_of(bool f32, const View &prefix, const PrefixShape &ps, const View &c, const AttentionShape &a) {
+    SharedPlan p;
+    const uint32_t widest = widest_of(c), own_rows = a.q_heads / c.heads * a.n;
+    p.n = ps.most * own_rows;
+    const Plan over = icsdk::kv::plan_of(f32, prefix, AttentionShape{ps.batch, prefix.heads, p.n, ps.longest, a.scale, false,
+                                                                     nullptr, nullptr, 0, 0});
+    const Plan own = icsdk::kv::plan_of(f32, c, a);
+    // beside a pass by tiles another one by tiles needs no products enough to fill the chip
+    const bool own_tiles = own.tiles || (over.tiles && own.many), prefix_tiles = over.tiles || (own_tiles && over.many);
+    const bool mixed = prefix_tiles && !own_tiles;
+    p.together = prefix_tiles == own_tiles || (mixed && tiles_twice(f32, widest));
+    const bool twice = prefix_tiles || own_tiles ? tiles_twice(f32, widest) : rows_twice(f32, widest);
+    const uint32_t fill = twice ? kWorkgroups : kWorkgroups / 2;
+    p.own = pass_of(c, own_tiles, a.batch, own_rows, a.longest, fill);
+    // the prefix has what the own tokens leave of the chip, half at least
+    const uint64_t taken = p.together ? workgroups_of(c, p.own) : 0;
+    p.prefix = pass_of(prefix, prefix_tiles, ps.batch, p.n, ps.longest, fill - (taken < fill / 2 ? taken : fill / 2));
+    p.rows = (size_t)a.batch * a.q_heads * a.n;
+    const size_t parts = p.prefix.parts + p.own.parts;
+    p.o_bytes = whole256(parts * p.rows * c.vdim * 4);
+    p.ml_bytes = whole256(parts * p.rows * sizeof(f32x2));
+    return p;
+}
+
+// ---- launch --------------------------------------------------------------------------------
+
+// The launches that a pass is in: 256 sequences and 2^22 workgroups each.
+template <typename S> struct Cursor {
+    const View &c;
+    const Pass &pass;
+    uint32_t first = 0, group = 0;
+
+    bool done() const { return first >= pass.batch; }
+    // Sequences, row groups and workgroups of the next launch.
+    uint32_t batch() const { return pass.batch - first < kBatchPerLaunch ? pass.batch - first : kBatchPerLaunch; }
+    uint32_t next(SharedArgs<S> &a) {
+        a.first = first;
+        a.pairs = batch() * c.heads;
+        a.row_group0 = group;
+        const uint32_t fit = (1u << 22) / (a.pairs * pass.parts), most = fit < 1 ? 1 : fit;
+        const uint32_t groups = pass.row_groups - group < most ? pass.row_groups - group : most;
+        a.columns = groups * pass.parts;
+        group += groups;
+        if (group == pass.row_groups) {
+            first += batch();
+            group = 0;
+        }
+        return a.columns * a.pairs;
+    }
+};
+
+template <typename S, uint32_t P> hipError_t launch(const Both<S> &both, uint32_t grid, bool tiles0, bool tiles1, bool stream, hipStream_t s) {
+    if constexpr (tiles_twice(sizeof(S) == 4, P)) {
+        if (tiles0 && !tiles1) {
+            kv_shared_mixed_kernel<S, P><<<grid, kThreads, 0, s>>>(both);
+            return hipGetLastError();
+        }
+    }
+    if constexpr (sizeof(S) == 2 || P <= 128) {
+        if (tiles0 && tiles1) {
+            kv_shared_tiles_kernel<S, P><<<grid, kThreads, 0, s>>>(both);
+            return hipGetLastError();
+        }
+    }
+    if (tiles0 || tiles1) return hipErrorInvalidValue;
+    if (stream) kv_shared_rows_kernel<S, P, true><<<grid, kThreads, 0, s>>>(both);
+    else kv_shared_rows_kernel<S, P, false><<<grid, kThreads, 0, s>>>(both);
+    return hipGetLastError();
+}
+template <typename S> hipError_t launch(const Both<S> &both, uint32_t widest, uint32_t grid, bool tiles0, bool tiles1, bool stream, hipStream_t s) {
+    if (widest <= 32) return launch<S, 32>(both, grid, tiles0, tiles1, stream, s);
+    if (widest <= 64) return launch<S, 64>(both, grid, tiles0, tiles1, stream, s);
+    if (widest <= 96) return launch<S, 96>(both, grid, tiles0, tiles1, stream, s);
+    if (widest <= 128) return launch<S, 128>(both, grid, tiles0, tiles1, stream, s);
+    if (widest <= 192) return launch<S, 192>(both, grid, tiles0, tiles1, stream, s);
+    return launch<S, 256>(both, grid, tiles0, tiles1, stream, s);
+}
+
+template <typename S>
+hipError_t run(const View &prefix, const PrefixShape &ps, const View &c, const AttentionShape &sh, const void *query,
+               void *output, void *workspace, hipStream_t s) {
+    const SharedPlan p = plan_of(sizeof(S) == 4, prefix, ps, c, sh);
+    const uint32_t group = sh.q_heads / c.heads;
+    Both<S> both{};
+    SharedArgs<S> &over = both.pass[0], &own = both.pass[1];
+    own.q = static_cast<const S *>(query);
+    own.out = static_cast<S *>(output);
+    own.part_o = static_cast<float *>(workspace);
+    own.part_ml = reinterpret_cast<f32x2 *>(static_cast<char *>(workspace) + p.o_bytes);
+    own.rows = p.rows;
+    own.scale2 = (double)sh.scale * kLog2e;
+    over = own;
+    over.c = prefix;
+    over.group = 1;   // a group's rows are one head's rows there
+    over.n = p.n;
+    over.own_rows = group * sh.n;
+    over.parts = p.prefix.parts;
+    over.longest = ps.longest;
+    over.row_groups = p.prefix.row_groups;
+    own.c = c;
+    own.group = group;
+    own.n = sh.n;
+    own.parts = p.own.parts;
+    own.longest = sh.longest;
+    own.row_groups = p.own.row_groups;
+    own.causal = sh.causal;
+    own.part_o += (size_t)p.prefix.parts * p.rows * c.vdim;
+    own.part_ml += (size_t)p.prefix.parts * p.rows;
+    const size_t held = (size_t)(ps.batch * (uint64_t)ps.longest + sh.batch * (uint64_t)sh.longest) * c.heads * (c.kp + c.vp);
+    auto go = [&](uint32_t grid, bool tiles0, bool tiles1) {
+        return launch(both, widest_of(c), grid, tiles0, tiles1, held > kStreamBytes, s);
+    };
+
+    Cursor<S> of_prefix{prefix, p.prefix}, of_own{c, p.own};
+    uint32_t sequence = 0;   // where the next group starts
+    while (!of_prefix.done() || !of_own.done()) {
+        both.first = 0;
+        uint32_t grid = 0;
+        if (!of_prefix.done()) {
+            if (of_prefix.group == 0) {   // the next prefixes
+                for (uint32_t b = 0; b < of_prefix.batch(); ++b) {
+                    over.count.n[b] = sequence;
+                    sequence += ps.members[of_prefix.first + b];
+                }
+                over.last = sequence;
+            }
+            both.first = grid = of_prefix.next(over);
+        }
+        if (grid != 0 && !p.together) {
+            const hipError_t status = go(grid, p.prefix.tiles, p.prefix.tiles);
+            if (status != hipSuccess) return status;
+            both.first = grid = 0;
+        }
+        if (!of_own.done()) {
+            for (uint32_t b = 0; b < of_own.batch(); ++b)
+                own.count.n[b] = sh.counts ? sh.counts[of_own.first + b] : sh.n;
+            grid += of_own.next(own);
+        }
+        if (grid == 0) continue;
+        const hipError_t status = go(grid, p.together ? p.prefix.tiles : p.own.tiles, p.own.tiles);
+        if (status != hipSuccess) return status;
+    }
+
+    // the parts' join, for 256 sequences each
+    const uint32_t parts = p.prefix.parts + p.own.parts;
+    own.part_o = over.part_o;
+    own.part_ml = over.part_ml;
+    for (uint32_t first = 0; first < sh.batch; first += kBatchPerLaunch) {
+        const uint32_t batch = sh.batch - first < kBatchPerLaunch ? sh.batch - first : kBatchPerLaunch;
+        for (uint32_t b = 0; b < batch; ++b) own.count.n[b] = sh.counts ? sh.counts[first + b] : sh.n;
+        own.first = first;
+        own.pairs = batch * c.heads;
+        const hipError_t status = launch_fold<S>(own, parts, false, 0, parts > 16 && p.rows <= kWideRows, s);
+        if (status != hipSuccess) return status;
+    }
+    return hipSuccess;
+}
+
+}  // namespace
+
+size_t attention_shared_workspace(bool f32, const View &prefix, const PrefixShape &p, const View &c,
+                                  const AttentionShape &a) {
+    const SharedPlan plan = plan_of(f32, prefix, p, c, a);
+    return plan.o_bytes + plan.ml_bytes;
+}
+
+hipError_t attention_shared(bool f32, const View &prefix, const PrefixShape &p, const View &c, const AttentionShape &a,
+                            const void *query, void *output, void *workspace, hipStream_t s) {
+    return f32 ? run<float>(prefix, p, c, a, query, output, workspace, s)
+               : run<_Float16>(prefix, p, c, a, query, output, workspace, s);
+}
+
+}  // namespace kv
+}  // namespace icsdk

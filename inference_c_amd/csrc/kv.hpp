@@ -1,6 +1,6 @@
 // The 8-bit key/value cache in device memory, and the launchers of its kernels
 // (k_kv_cache.hip: append, read, truncate, evict; k_kv_copy.hip: copy, reorder;
-// k_kv_attention.hip: attention).
+// k_kv_attention.hip: attention; k_kv_shared.hip: attention over a shared prefix).
 //
 // Of each (sequence, kv head), in blocks of 64 tokens:
 //   k     [block][token][kp]   codes + 128 as bytes, kp = head dim in whole 16s

@@ -1,6 +1,6 @@
 // What the kernels of attention over the 8-bit cache share: arguments, the codes
-// as f16, and the rules of rows, outputs and weights (k_kv_attention.hip describes
-// them; k_kv_tiles.hip has the kernels for many rows).
+// as f16, the rules of rows, outputs and weights (kv_rows.hpp describes them;
+// kv_tiles.hpp has the kernel for many rows), and the plan.
 #pragma once
 
 #include "kern_common.hpp"
@@ -52,25 +52,41 @@ template <typename S> struct Args {
     Counts count;
 };
 
-// Of a pass that goes with another one into the same rows' parts: attention over a
-// prefix and over the sequences' own tokens (k_kv_attention.hip). A packed row of
-// (sequence, head) of the pass's cache is row r % own_rows of that head of sequence
-// member.n[b] + r / own_rows of q and the parts. Outputs are parts, however few.
+// Of a pass of attention over a prefix and own tokens (k_kv_shared.hip), whose rows'
+// parts meet another pass's. Over a prefix, a packed row of (sequence first + b, head) of
+// the pass's cache is row r % own_rows of that head of sequence count.n[b] + r / own_rows
+// of q and the parts: `count` has where the groups start. Over own tokens, own_rows is 0
+// and all is as in Args. Outputs are parts, however few.
 template <typename S> struct SharedArgs : Args<S> {
-    uint32_t own_rows;
-    Counts member;
+    uint32_t own_rows;   // packed rows of a sequence and head
+    uint32_t last;       // where the last group of the launch ends
+    uint32_t columns;    // of a head, workgroups of the rows kernel
 };
-template <typename S, bool kShared> struct ArgsOf { typedef Args<S> type; };
-template <typename S> struct ArgsOf<S, true> { typedef SharedArgs<S> type; };
+// Arguments where a kernel finds them: memory that nothing writes.
+template <typename A> using Constant = const __attribute__((address_space(4))) A;
+template <typename A> __device__ inline Constant<A> &kernel_arguments(uint32_t offset) {
+    return *(Constant<A> *)((const __attribute__((address_space(4))) char *)__builtin_amdgcn_kernarg_segment_ptr() + offset);
+}
+template <typename A> constexpr bool kIsShared = false;
+template <typename S> constexpr bool kIsShared<Constant<SharedArgs<S>>> = true;
 
-// The row of q, the parts and the output that packed row r of sequence first + b and
-// head h is (rows that are not there repeat the last that is).
+// How many of a query head's rows are there.
+template <typename S> __device__ inline uint32_t rows_there(Constant<Args<S>> &a, uint32_t b) { return a.count.n[b]; }
+template <typename S> __device__ inline uint32_t rows_there(Constant<SharedArgs<S>> &a, uint32_t b) {
+    if (a.own_rows == 0) return a.count.n[b];
+    // (over a prefix `count` has where the groups start)
+    const uint32_t end = (b + 1) * a.c.heads < a.pairs ? a.count.n[b + 1] : a.last;
+    return (end - a.count.n[b]) * a.own_rows;
+}
+// The row of q, the parts and the output that packed row r is (rows that are not there
+// repeat the last that is, or the first of all).
 template <typename S>
-__device__ inline size_t shared_row(const SharedArgs<S> &a, uint32_t r, uint32_t b, uint32_t h, uint32_t in_head,
+__device__ inline size_t shared_row(Constant<SharedArgs<S>> &a, uint32_t r, uint32_t b, uint32_t h, uint32_t in_head,
                                     uint32_t count) {
     r = min(r, in_head - a.n + max(count, 1u) - 1);
-    const uint32_t m = r / a.own_rows;
-    return ((size_t)(a.member.n[b] + m) * a.c.heads + h) * a.own_rows + (r - m * a.own_rows);
+    if (a.own_rows == 0) return ((size_t)(a.first + b) * a.c.heads + h) * in_head + r;
+    const uint32_t m = r / a.own_rows, sequence = count != 0 ? a.count.n[b] + m : 0;
+    return ((size_t)sequence * a.c.heads + h) * a.own_rows + (r - m * a.own_rows);
 }
 
 // A block's Meta through the scalar cache (no kernel writes it while one that
@@ -162,13 +178,40 @@ constexpr uint32_t kTileRows = 128;
 bool tiles_fit(bool f32, uint32_t widest);
 // Whether a CU holds two of its workgroups (their registers decide).
 constexpr bool tiles_twice(bool f32, uint32_t widest) { return !f32 && widest <= 128; }
-template <typename S, bool kShared>
-hipError_t launch_tiles(const typename ArgsOf<S, kShared>::type &a, uint32_t widest, uint32_t groups, hipStream_t s);
+template <typename S>
+hipError_t launch_tiles(const Args<S> &a, uint32_t widest, uint32_t groups, hipStream_t s);
 // Weights from the rows' maxima and sums; row_parts > 1: `partial` holds row_parts
 // sums for each token of every (sequence, head).
 template <typename S>
 hipError_t launch_weights(const Args<S> &a, uint32_t widest, uint32_t batch, uint32_t blocks, uint32_t row_parts,
                           float *partial, hipStream_t s);
+
+// Joins `parts` parts of the rows of a launch's sequences, by wide workgroups or not;
+// its workgroups after those take token weights from the stored scores, if there are any.
+template <typename S>
+hipError_t launch_fold(const Args<S> &a, uint32_t parts, bool scores, uint32_t longest, bool wide, hipStream_t s);
+
+struct Plan {
+    bool many;     // rows enough for a tile to take less time than workgroups of 16 rows
+    bool tiles;    // and products enough: k_kv_tiles.hip
+    bool scores;   // the weights come from scores that the rows kernel stores (never with tiles)
+    uint32_t row_groups, parts, row_parts;
+    size_t rows, score_stride;
+    size_t o_bytes, ml_bytes, exact_bytes, row_bytes, score_bytes, partial_bytes;
+    size_t bytes() const { return o_bytes + ml_bytes + exact_bytes + row_bytes + score_bytes + partial_bytes; }
+};
+
+inline size_t whole256(size_t bytes) { return (bytes + 255) / 256 * 256; }
+inline uint32_t widest_of(const View &c) { return c.kp > c.vp ? c.kp : c.vp; }
+constexpr uint32_t kWorkgroups = 512;   // two for every CU
+// Whether a CU holds two workgroups of the rows kernel (their registers decide).
+constexpr bool rows_twice(bool f32, uint32_t widest) { return widest <= (f32 ? 128u : 192u); }
+Plan plan_of(bool f32, const View &c, const AttentionShape &a);
+
+// Codes past what the 256 MB cache behind the L2s holds to the next call are read
+// as a stream. One sequence of 131000 tokens (268 MB): 62.5 -> 56.6 us; 8 x 4096
+// (67 MB, found there by calls in a row): 19.5, as a stream 20.6.
+constexpr size_t kStreamBytes = size_t{192} << 20;
 
 }  // namespace kv
 }  // namespace icsdk

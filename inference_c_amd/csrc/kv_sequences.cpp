@@ -1,7 +1,7 @@
 // The key/value cache's entry points for several continuations of one prompt
 // (include/tensor_kv_cache.h): sequences copied and reordered as they are held
 // (k_kv_copy.hip), and attention over a prefix that sequences share
-// (k_kv_attention.hip).
+// (k_kv_shared.hip).
 #include "kv_handle.hpp"
 
 #include <climits>
