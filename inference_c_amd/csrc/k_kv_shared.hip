@@ -63,8 +63,70 @@ __global__ __launch_bounds__(kThreads, 2) void kv_shared_mixed_kernel(Both<S>) {
     }
 }
 
-// Rows up to which 16 waves join a row's parts: above, four do. Measured at 33 parts of
-// 2048 rows: 18 us by 16 waves, 10 by four.
+// ---- the parts' join ------------------------------------------------------------------------
+
+struct JoinArgs {
+    const float *part_o;
+    const f32x2 *part_ml;
+    size_t rows, first_row;    // of all sequences; where the launch's begin
+    uint32_t parts, vdim, all;   // all: rows of the launch
+    FastDiv per_row;             // threads of a row, four elements each
+    bool padded;                 // some rows are padding, by `count`
+    FastDiv n, per_sequence;     // rows of a query head, and of a sequence
+    Counts count;
+};
+
+// kHeld parts are asked for at once (past the last one that again, and not used).
+template <typename S, uint32_t kHeld> __global__ __launch_bounds__(kThreads) void kv_join_kernel(S *out, JoinArgs a) {
+    const uint32_t i = blockIdx.x * kThreads + threadIdx.x, r = fast_div(i, a.per_row), d = 4 * (i - r * a.per_row.divisor);
+    if (r >= a.all) return;
+    const size_t row = a.first_row + r;
+    if (a.padded && r - fast_div(r, a.n) * a.n.divisor >= a.count.n[fast_div(r, a.per_sequence)]) return;
+    const uint32_t last = a.parts - 1;
+    auto load = [&](uint32_t s) {
+        const float *const src = a.part_o + ((size_t)s * a.rows + row) * a.vdim + d;
+        f32x4 x;
+        if (a.vdim % 4 == 0) {
+            x = *reinterpret_cast<const f32x4 *>(src);
+        } else {
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) x[e] = d + e < a.vdim ? src[e] : 0.0f;
+        }
+        return x;
+    };
+    f32x4 v = {0, 0, 0, 0}, held[kHeld];
+    f32x2 ml[kHeld];
+#pragma unroll
+    for (uint32_t k = 0; k < kHeld; ++k) {
+        const uint32_t s = min(k, last);
+        held[k] = load(s);
+        ml[k] = a.part_ml[(size_t)s * a.rows + row];
+    }
+    float top = ml[0].x, total = 0.0f;
+#pragma unroll
+    for (uint32_t k = 1; k < kHeld; ++k) top = fmaxf(top, ml[k].x);
+#pragma unroll 8
+    for (uint32_t s = kHeld; s < a.parts; ++s) top = fmaxf(top, a.part_ml[(size_t)s * a.rows + row].x);
+    // (a part that saw nothing has weight 0, and a NaN in it stays)
+    auto weight = [&](float m) { return top == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - top); };
+#pragma unroll
+    for (uint32_t k = 0; k < kHeld; ++k)
+        if (k < a.parts) {
+            const float w = weight(ml[k].x);
+            v += held[k] * w;
+            total += ml[k].y * w;
+        }
+#pragma unroll 8
+    for (uint32_t s = kHeld; s < a.parts; ++s) {
+        const f32x2 x = a.part_ml[(size_t)s * a.rows + row];
+        const float w = weight(x.x);
+        v += load(s) * w;
+        total += x.y * w;
+    }
+    store_out(out + row * a.vdim, a.vdim, d, finish(v, top, total));
+}
+
+// Few rows of many parts are joined by 16 waves each (kv_fold_kernel).
 constexpr size_t kWideRows = 512;
 
 // ---- plan --------------------------------------------------------------------------------
@@ -244,9 +306,31 @@ hipError_t run(const View &prefix, const PrefixShape &ps, const View &c, const A
     for (uint32_t first = 0; first < sh.batch; first += kBatchPerLaunch) {
         const uint32_t batch = sh.batch - first < kBatchPerLaunch ? sh.batch - first : kBatchPerLaunch;
         for (uint32_t b = 0; b < batch; ++b) own.count.n[b] = sh.counts ? sh.counts[first + b] : sh.n;
-        own.first = first;
-        own.pairs = batch * c.heads;
-        const hipError_t status = launch_fold<S>(own, parts, false, 0, parts > 16 && p.rows <= kWideRows, s);
+        const uint32_t per_sequence = sh.q_heads * sh.n;
+        hipError_t status = hipSuccess;
+        if (parts > 16 && p.rows <= kWideRows) {
+            own.first = first;
+            own.pairs = batch * c.heads;
+            status = launch_fold<S>(own, parts, false, 0, true, s);
+        } else {
+            // (whole sequences, fewer than 2^32 threads)
+            const uint32_t threads = (c.vdim + 3) / 4, most = (1u << 31) / threads / per_sequence;
+            for (uint32_t b = 0; b < batch && status == hipSuccess;) {
+                const uint32_t now = batch - b < most ? batch - b : most < 1 ? 1 : most;
+                JoinArgs j{own.part_o, own.part_ml, p.rows, (size_t)(first + b) * per_sequence, parts, c.vdim,
+                           now * per_sequence, make_fast_div(threads), sh.counts != nullptr, make_fast_div(sh.n),
+                           make_fast_div(per_sequence), {}};
+                for (uint32_t i = 0; i < now; ++i) j.count.n[i] = own.count.n[b + i];
+                auto join = [&](auto kernel) {
+                    kernel<<<(j.all * threads + kThreads - 1) / kThreads, kThreads, 0, s>>>(static_cast<S *>(output), j);
+                };
+                if (parts <= 2) join(kv_join_kernel<S, 2>);
+                else if (parts <= 4) join(kv_join_kernel<S, 4>);
+                else join(kv_join_kernel<S, 8>);
+                status = hipGetLastError();
+                b += now;
+            }
+        }
         if (status != hipSuccess) return status;
     }
     return hipSuccess;

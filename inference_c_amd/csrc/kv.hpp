@@ -70,11 +70,11 @@ struct EvictArgs {
 hipError_t evict(const View &from, const View &to, uint32_t batch, const EvictArgs &a, hipStream_t s);
 
 // Sequences first .. first + batch - 1 of `to` become copies of sequences source[b] of
-// `from` (kKeep: stay as they are); `longest` bounds the sources' lengths. `to` may be
-// `from` where no sequence is both read and written.
+// `from` (kKeep: stay as they are); `longest` bounds the sources' lengths, `tokens` are
+// all that the call copies. `to` may be `from` where no sequence is both read and written.
 constexpr uint32_t kKeep = 0xffffffffu;
 hipError_t copy(const View &from, const View &to, uint32_t first, uint32_t batch, const Counts &source, uint32_t longest,
-                hipStream_t s);
+                size_t tokens, hipStream_t s);
 // In each group of `beams` sequences (of one length, at most `longest`), sequence i
 // becomes what sequence parents[i] was.
 constexpr uint32_t kMaxBeams = 64;

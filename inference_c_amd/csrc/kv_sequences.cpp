@@ -44,6 +44,7 @@ int copy(const TensorKvCache *from, const uint32_t *source, TensorKvCache *to, c
         return fail(error, capacity, "cache copy: the target's heads and dimensions must be the cache's");
     const Locked lock(from, to);
     uint32_t longest = 0;
+    size_t tokens = 0;
     bool any = false;
     // within one cache, a copy of itself is what a sequence is already
     auto keeps = [&](size_t b) { return source[b] == TENSOR_KV_CACHE_KEEP || (from == to && source[b] == b); };
@@ -64,6 +65,7 @@ int copy(const TensorKvCache *from, const uint32_t *source, TensorKvCache *to, c
             return 0;
         }
         longest = n > longest ? n : longest;
+        tokens += n;
         any = true;
     }
     if (!any) return 1;
@@ -78,7 +80,7 @@ int copy(const TensorKvCache *from, const uint32_t *source, TensorKvCache *to, c
             here = here || sources.n[b] != kv::kKeep;
         }
         if (!here) continue;
-        if (!hip_ok(kv::copy(from->view, to->view, (uint32_t)first, batch, sources, longest, sdk_stream()),
+        if (!hip_ok(kv::copy(from->view, to->view, (uint32_t)first, batch, sources, longest, tokens, sdk_stream()),
                     "cache copy: kernel launch", error, capacity))
             return 0;
         for (uint32_t b = 0; b < batch; ++b)

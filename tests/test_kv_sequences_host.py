@@ -22,7 +22,8 @@ static icsdk::kv::Counts told;       // the last copy's sources
 static uint32_t told_batch, told_longest, told_most;
 namespace icsdk {
 namespace kv {
-hipError_t copy(const View &, const View &, uint32_t, uint32_t batch, const Counts &source, uint32_t longest, hipStream_t) {
+hipError_t copy(const View &, const View &, uint32_t, uint32_t batch, const Counts &source, uint32_t longest, size_t,
+                hipStream_t) {
     told = source, told_batch = batch, told_longest = longest;
     return launch();
 }
