@@ -19,12 +19,17 @@ template <typename S> struct Both {
     uint32_t first;          // workgroups of the first pass; those behind are the second's
 };
 
-// Workgroup i of a pass by the rows kernel.
-template <typename S, uint32_t P, bool kStream>
+// Workgroup i of a pass by the rows kernel; kSolo: each wave does what a workgroup
+// would, the waves of four of them.
+template <typename S, uint32_t P, bool kStream, bool kSolo>
 __device__ __forceinline__ void rows_of(RowsOut<P> &lds_o, RowsMl &lds_ml, Constant<SharedArgs<S>> &a, uint32_t i) {
-    const uint32_t x = i % a.columns, pair = i / a.columns, h = pair % a.c.heads, b = pair / a.c.heads;
-    rows_of<S, P, kStream>(lds_o, lds_ml, a.c.k, a.c.v, a.c.length, a.c.meta, a.q, a.c.blocks, a.c.heads,
-                           a.parts | a.first << 16, a.c.kp | a.c.vp << 16, a.n, a.group, a, x, h, b);
+    if constexpr (kSolo) {
+        i = i * kWaves + (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+        if (i >= a.columns * a.pairs) return;
+    }
+    const uint32_t pair = i % a.pairs, x = i / a.pairs, h = pair % a.c.heads, b = pair / a.c.heads;
+    rows_of<S, P, kStream, kSolo>(lds_o, lds_ml, a.c.k, a.c.v, a.c.length, a.c.meta, a.q, a.c.blocks, a.c.heads,
+                                  a.parts | a.first << 16, a.c.kp | a.c.vp << 16, a.n, a.group, a, x, h, b);
 }
 
 template <typename S, uint32_t P, bool kStream>
@@ -33,7 +38,17 @@ __global__ __launch_bounds__(kThreads) void kv_shared_rows_kernel(Both<S>) {
     __shared__ RowsMl lds_ml;
     auto &both = kernel_arguments<Both<S>>(0);
     const uint32_t second = blockIdx.x >= both.first ? 1 : 0;
-    rows_of<S, P, kStream>(lds_o, lds_ml, both.pass[second], blockIdx.x - (second ? both.first : 0));
+    rows_of<S, P, kStream, false>(lds_o, lds_ml, both.pass[second], blockIdx.x - (second ? both.first : 0));
+}
+
+// Own tokens by waves alone.
+template <typename S, uint32_t P>
+__global__ __launch_bounds__(kThreads) void kv_shared_solo_kernel(Both<S>) {
+    __shared__ RowsOut<P> lds_o;
+    __shared__ RowsMl lds_ml;
+    auto &both = kernel_arguments<Both<S>>(0);
+    if (blockIdx.x < both.first) rows_of<S, P, false, false>(lds_o, lds_ml, both.pass[0], blockIdx.x);
+    else rows_of<S, P, false, true>(lds_o, lds_ml, both.pass[1], blockIdx.x - both.first);
 }
 
 template <typename S, uint32_t P>
@@ -58,8 +73,9 @@ __global__ __launch_bounds__(kThreads, 2) void kv_shared_mixed_kernel(Both<S>) {
         tiles_of<S, P, false>(ks, vs, wave_most, both.pass[0], blockIdx.x);
     } else {
         char *const lds = reinterpret_cast<char *>(ks);
-        rows_of<S, P, false>(*reinterpret_cast<RowsOut<P> *>(lds), *reinterpret_cast<RowsMl *>(lds + sizeof(RowsOut<P>)),
-                             both.pass[1], blockIdx.x - both.first);
+        rows_of<S, P, false, false>(*reinterpret_cast<RowsOut<P> *>(lds),
+                                    *reinterpret_cast<RowsMl *>(lds + sizeof(RowsOut<P>)), both.pass[1],
+                                    blockIdx.x - both.first);
     }
 }
 
@@ -131,9 +147,15 @@ constexpr size_t kWideRows = 512;
 
 // ---- plan --------------------------------------------------------------------------------
 
+// Measured (us, the call, four waves and solo; f16, one query row): 8 prefixes of 2000 x 8
+// sequences, 8 heads of 128, own tokens of 2 blocks 24.5 and 20.9, of 8 37.9 and 34.9, of 12
+// 45.7 and 43.1, of 16 50.3 and 51.3; 5 heads of 64, 8 x 8 sequences of 15 blocks 17.8 and
+// 25.6. With f32 queries (28 for 22) or beside tiles (49 for 46) it loses.
+constexpr uint32_t kSoloBlocks = 8;
+
 // A pass: its kernel and its workgroups.
 struct Pass {
-    bool tiles;
+    bool tiles, solo;   // (solo: rows, by waves alone)
     uint32_t batch, row_groups, parts;
 };
 struct SharedPlan {
@@ -144,7 +166,7 @@ struct SharedPlan {
 };
 
 Pass pass_of(const View &c, bool tiles, uint32_t batch, uint32_t in_head, uint32_t longest, uint64_t workgroups) {
-    Pass p{tiles, batch, 0, 1};
+    Pass p{tiles, false, batch, 0, 1};
     const uint32_t rows = tiles ? kTileRows : kRows, blocks = (longest + kTokens - 1) / kTokens;
     p.row_groups = (in_head + rows - 1) / rows;
     const uint64_t base = (uint64_t)batch * c.heads * p.row_groups, most = (blocks + kWaves - 1) / kWaves;
@@ -154,7 +176,10 @@ Pass pass_of(const View &c, bool tiles, uint32_t batch, uint32_t in_head, uint32
     return p;
 }
 
-uint64_t workgroups_of(const View &c, const Pass &p) { return (uint64_t)p.batch * c.heads * p.row_groups * p.parts; }
+uint64_t workgroups_of(const View &c, const Pass &p) {
+    const uint64_t n = (uint64_t)p.batch * c.heads * p.row_groups * p.parts;
+    return p.solo ? (n + kWaves - 1) / kWaves : n;
+}
 
 SharedPlan plan_of(bool f32, const View &prefix, const PrefixShape &ps, const View &c, const AttentionShape &a) {
     SharedPlan p;
@@ -170,6 +195,10 @@ SharedPlan plan_of(bool f32, const View &prefix, const PrefixShape &ps, const Vi
     const bool twice = prefix_tiles || own_tiles ? tiles_twice(f32, widest) : rows_twice(f32, widest);
     const uint32_t fill = twice ? kWorkgroups : kWorkgroups / 2;
     p.own = pass_of(c, own_tiles, a.batch, own_rows, a.longest, fill);
+    // own tokens of few blocks, of which four waves would have one or two each, where the
+    // workgroups of their own would take the chip from the prefix
+    p.own.solo = !f32 && !prefix_tiles && !own_tiles && a.longest <= kSoloBlocks * kTokens &&
+                 workgroups_of(c, p.own) >= fill / 2;
     // the prefix has what the own tokens leave of the chip, half at least
     const uint64_t taken = p.together ? workgroups_of(c, p.own) : 0;
     p.prefix = pass_of(prefix, prefix_tiles, ps.batch, p.n, ps.longest, fill - (taken < fill / 2 ? taken : fill / 2));
@@ -203,35 +232,37 @@ template <typename S> struct Cursor {
             first += batch();
             group = 0;
         }
-        return a.columns * a.pairs;
+        const uint32_t n = a.columns * a.pairs;
+        return pass.solo ? (n + kWaves - 1) / kWaves : n;
     }
 };
 
-template <typename S, uint32_t P> hipError_t launch(const Both<S> &both, uint32_t grid, bool tiles0, bool tiles1, bool stream, hipStream_t s) {
-    if constexpr (tiles_twice(sizeof(S) == 4, P)) {
-        if (tiles0 && !tiles1) {
-            kv_shared_mixed_kernel<S, P><<<grid, kThreads, 0, s>>>(both);
-            return hipGetLastError();
-        }
-    }
-    if constexpr (sizeof(S) == 2 || P <= 128) {
-        if (tiles0 && tiles1) {
-            kv_shared_tiles_kernel<S, P><<<grid, kThreads, 0, s>>>(both);
-            return hipGetLastError();
-        }
-    }
-    if (tiles0 || tiles1) return hipErrorInvalidValue;
-    if (stream) kv_shared_rows_kernel<S, P, true><<<grid, kThreads, 0, s>>>(both);
-    else kv_shared_rows_kernel<S, P, false><<<grid, kThreads, 0, s>>>(both);
-    return hipGetLastError();
+// Which kernel a launch takes.
+struct Kernels {
+    bool tiles[2], solo, stream;
+};
+template <typename S, uint32_t P> hipError_t launch(const Both<S> &both, uint32_t grid, const Kernels &k, hipStream_t s) {
+    auto go = [&](auto kernel) {
+        kernel<<<grid, kThreads, 0, s>>>(both);
+        return hipGetLastError();
+    };
+    if constexpr (tiles_twice(sizeof(S) == 4, P))
+        if (k.tiles[0] && !k.tiles[1]) return go(kv_shared_mixed_kernel<S, P>);
+    if constexpr (sizeof(S) == 2 || P <= 128)
+        if (k.tiles[0] && k.tiles[1]) return go(kv_shared_tiles_kernel<S, P>);
+    if (k.tiles[0] || k.tiles[1]) return hipErrorInvalidValue;   // (no plan has them)
+    if constexpr (sizeof(S) == 2)
+        if (k.solo) return go(kv_shared_solo_kernel<S, P>);
+    return k.stream ? go(kv_shared_rows_kernel<S, P, true>) : go(kv_shared_rows_kernel<S, P, false>);
 }
-template <typename S> hipError_t launch(const Both<S> &both, uint32_t widest, uint32_t grid, bool tiles0, bool tiles1, bool stream, hipStream_t s) {
-    if (widest <= 32) return launch<S, 32>(both, grid, tiles0, tiles1, stream, s);
-    if (widest <= 64) return launch<S, 64>(both, grid, tiles0, tiles1, stream, s);
-    if (widest <= 96) return launch<S, 96>(both, grid, tiles0, tiles1, stream, s);
-    if (widest <= 128) return launch<S, 128>(both, grid, tiles0, tiles1, stream, s);
-    if (widest <= 192) return launch<S, 192>(both, grid, tiles0, tiles1, stream, s);
-    return launch<S, 256>(both, grid, tiles0, tiles1, stream, s);
+template <typename S>
+hipError_t launch(const Both<S> &both, uint32_t widest, uint32_t grid, const Kernels &k, hipStream_t s) {
+    if (widest <= 32) return launch<S, 32>(both, grid, k, s);
+    if (widest <= 64) return launch<S, 64>(both, grid, k, s);
+    if (widest <= 96) return launch<S, 96>(both, grid, k, s);
+    if (widest <= 128) return launch<S, 128>(both, grid, k, s);
+    if (widest <= 192) return launch<S, 192>(both, grid, k, s);
+    return launch<S, 256>(both, grid, k, s);
 }
 
 template <typename S>
@@ -266,7 +297,7 @@ hipError_t run(const View &prefix, const PrefixShape &ps, const View &c, const A
     own.part_ml += (size_t)p.prefix.parts * p.rows;
     const size_t held = (size_t)(ps.batch * (uint64_t)ps.longest + sh.batch * (uint64_t)sh.longest) * c.heads * (c.kp + c.vp);
     auto go = [&](uint32_t grid, bool tiles0, bool tiles1) {
-        return launch(both, widest_of(c), grid, tiles0, tiles1, held > kStreamBytes, s);
+        return launch(both, widest_of(c), grid, Kernels{{tiles0, tiles1}, p.own.solo, held > kStreamBytes}, s);
     };
 
     Cursor<S> of_prefix{prefix, p.prefix}, of_own{c, p.own};

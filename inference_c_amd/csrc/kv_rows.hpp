@@ -120,10 +120,11 @@ template <bool kStream, typename V> __device__ inline V load_codes(const V *p) {
 // registers when a wave starts: the struct behind them takes a microsecond to
 // arrive. (8 x 4096 tokens, from the wave's start to its first loads' issue: 2 us
 // out of 12 with the struct alone.)
-// A is Args, or SharedArgs for a pass of attention over a prefix and own tokens.
+// A is Args, or SharedArgs for a pass of attention over a prefix and own tokens. kSolo
+// (of such a pass): a wave has 16 rows and a part by itself, and its own x, h and b.
 template <uint32_t P> using RowsOut = f32x4[kWaves][P / 16][kWave];
 using RowsMl = f32x4[kWaves][kRows];   // maximum, sums of P rounded and not
-template <typename S, uint32_t P, bool kStream, typename A>
+template <typename S, uint32_t P, bool kStream, bool kSolo, typename A>
 __device__ __forceinline__ void rows_of(RowsOut<P> &lds_o, RowsMl &lds_ml, const uint8_t *keys, const uint8_t *values,
                                         const uint32_t *lengths, const Meta *metas, const S *queries, uint32_t all_blocks,
                                         uint32_t heads, uint32_t parts_first, uint32_t pitches, uint32_t n,
@@ -141,9 +142,10 @@ __device__ __forceinline__ void rows_of(RowsOut<P> &lds_o, RowsMl &lds_ml, const
     const size_t head = (size_t)seq * heads + h;
     // the part's blocks, the open one (the last, in f16) among them
     const uint32_t whole = length / kTokens, held = (length + kTokens - 1) / kTokens;
-    const uint32_t share = ((held + parts - 1) / parts + kWaves - 1) / kWaves * kWaves;
+    constexpr uint32_t kEvery = kSolo ? 1 : kWaves;
+    const uint32_t share = ((held + parts - 1) / parts + kEvery - 1) / kEvery * kEvery;
     const uint32_t begin = min(part * share, held);
-    uint32_t t = begin + wave;
+    uint32_t t = begin + (kSolo ? 0 : wave);
 
     const Meta *const meta = metas + head * all_blocks;
     const uint32_t key_of = (m / 4) * 16 + m % 4;   // + 4 u: the lane's key row
@@ -318,8 +320,8 @@ __device__ __forceinline__ void rows_of(RowsOut<P> &lds_o, RowsMl &lds_ml, const
         }
     };
 
-    for (; t < end_whole; t += kWaves) {
-        const uint32_t next = t + kWaves;
+    for (; t < end_whole; t += kEvery) {
+        const uint32_t next = t + kEvery;
         Meta next_meta;
         step(
             t, now_meta,
@@ -353,6 +355,15 @@ __device__ __forceinline__ void rows_of(RowsOut<P> &lds_o, RowsMl &lds_ml, const
     sum = groups_sum(sum);
     exact = kPair ? sum : groups_sum(exact);
     big -= kHeadroom<S>;   // what P's exponents are relative to
+    if constexpr (kSolo) {
+        static_assert(kShared);
+        if (!live || r >= in_head) return;
+        float *const out = a.part_o + ((size_t)part * a.rows + row) * c.vdim;
+#pragma unroll
+        for (uint32_t j = 0; j < NV; ++j) store_out(out, c.vdim, 16 * j + 4 * g, o[j] * (unit / kPairScale<S>));
+        if (g == 0) a.part_ml[(size_t)part * a.rows + row] = f32x2{big, sum};
+        return;
+    }
     if (g == 0) lds_ml[wave][m] = f32x4{big, sum, exact, 0.0f};
 #pragma unroll
     for (uint32_t j = 0; j < NV; ++j) lds_o[wave][j][lane] = o[j] * (unit / kPairScale<S>);
