@@ -97,10 +97,14 @@ struct ReorderArgs {
 
 // Beams' cache memory in place: a thread has the same 16 bytes of every sequence of
 // its group, reads those that replace others, and then writes them, so no copy needs a
-// place in between. A workgroup does kColumns of them, one after another (one each
-// would be too many threads for a launch at the largest capacity). kBeams: at least
-// the group's.
-constexpr uint32_t kColumns = 2, kColumn = kThreads * 16;
+// place in between. kBeams: at least the group's. Bound by memory, read and written in
+// turn: 16 groups of 8 x 850 tokens on average, 8 heads of 128 + 128, of which half move
+// (116 MB read, as often as it goes to several, and written) 50 us, 4.7 TB/s of that. A
+// workgroup does kColumns of its 16 bytes' columns, kAhead of them at once. Measured (us,
+// 16 x 8 x 850 and 4 groups of 16 x 1000): one column 57 and 56, two one after another 54
+// and 59, four 53 and 49, four by twos 50 and 50, eight by twos 53 and 55; 32 groups of 4 x
+// 100 tokens 10.5 one by one, 8.7 by twos.
+constexpr uint32_t kColumns = 8, kColumn = kThreads * 16;
 template <uint32_t kBeams>
 __global__ __launch_bounds__(kThreads) void kv_reorder_kernel(ReorderArgs a) {
     const View &c = a.c;
@@ -112,30 +116,36 @@ __global__ __launch_bounds__(kThreads) void kv_reorder_kernel(ReorderArgs a) {
         const uint32_t p = i < a.beams ? a.parents[first + i] : i;
         parent[i] = p < a.beams ? p : i;   // (an index past the group: the sequence stays)
     }
-    // the thread's column of one kind: `pitch` bytes from one sequence to the next
+    // the thread's next kAhead columns of one kind: `pitch` bytes from one sequence to the next
+    constexpr uint32_t kAhead = kBeams <= 8 ? 4 : kBeams <= 16 ? 2 : 1;
     auto column = [&](void *memory, size_t pitch, size_t at, size_t bytes) {
-        if (at >= bytes) return;
-        char *const base = static_cast<char *>(memory) + ((size_t)first * c.heads + h) * pitch + at;
+        char *const base = static_cast<char *>(memory) + ((size_t)first * c.heads + h) * pitch;
         const size_t next = c.heads * pitch;
-        u32x4 x[kBeams];
+        u32x4 x[kAhead][kBeams];
 #pragma unroll
-        for (uint32_t i = 0; i < kBeams; ++i)
-            if (parent[i] != i) x[i] = *reinterpret_cast<const u32x4 *>(base + parent[i] * next);
+        for (uint32_t u = 0; u < kAhead; ++u)
 #pragma unroll
-        for (uint32_t i = 0; i < kBeams; ++i)
-            if (parent[i] != i) *reinterpret_cast<u32x4 *>(base + i * next) = x[i];
+            for (uint32_t i = 0; i < kBeams; ++i)
+                if (parent[i] != i && at + u * kColumn < bytes)
+                    x[u][i] = *reinterpret_cast<const u32x4 *>(base + at + u * kColumn + parent[i] * next);
+#pragma unroll
+        for (uint32_t u = 0; u < kAhead; ++u)
+#pragma unroll
+            for (uint32_t i = 0; i < kBeams; ++i)
+                if (parent[i] != i && at + u * kColumn < bytes)
+                    *reinterpret_cast<u32x4 *>(base + at + u * kColumn + i * next) = x[u][i];
     };
     const size_t lane = threadIdx.x * 16;
     if (piece < a.k_pieces) {
-        for (size_t u = 0; u < kColumns; ++u)
+        for (size_t u = 0; u < kColumns; u += kAhead)
             column(c.k, (size_t)c.blocks * kTokens * c.kp, (piece * kColumns + u) * kColumn + lane, held.k);
     } else if (piece < a.k_pieces + a.v_pieces) {
-        for (size_t u = 0; u < kColumns; ++u)
+        for (size_t u = 0; u < kColumns; u += kAhead)
             column(c.v, (size_t)c.blocks * kTokens * c.vp, ((piece - a.k_pieces) * kColumns + u) * kColumn + lane, held.v);
     } else {
-        for (size_t at = lane; at < held.meta; at += kColumn) column(c.meta, (size_t)c.blocks * sizeof(Meta), at, held.meta);
-        for (size_t at = lane; at < held.kt; at += kColumn) column(c.kt, (size_t)kTokens * c.kp * 2, at, held.kt);
-        for (size_t at = lane; at < held.vt; at += kColumn) column(c.vt, (size_t)kTokens * c.vp * 2, at, held.vt);
+        for (size_t at = lane; at < held.meta; at += kAhead * kColumn) column(c.meta, (size_t)c.blocks * sizeof(Meta), at, held.meta);
+        for (size_t at = lane; at < held.kt; at += kAhead * kColumn) column(c.kt, (size_t)kTokens * c.kp * 2, at, held.kt);
+        for (size_t at = lane; at < held.vt; at += kAhead * kColumn) column(c.vt, (size_t)kTokens * c.vp * 2, at, held.vt);
     }
 }
 
