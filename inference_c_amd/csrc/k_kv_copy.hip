@@ -104,7 +104,7 @@ struct ReorderArgs {
 // 16 x 8 x 850 and 4 groups of 16 x 1000): one column 57 and 56, two one after another 54
 // and 59, four 53 and 49, four by twos 50 and 50, eight by twos 53 and 55; 32 groups of 4 x
 // 100 tokens 10.5 one by one, 8.7 by twos.
-constexpr uint32_t kColumns = 8, kColumn = kThreads * 16;
+constexpr uint32_t kColumns = 4, kColumn = kThreads * 16;
 template <uint32_t kBeams>
 __global__ __launch_bounds__(kThreads) void kv_reorder_kernel(ReorderArgs a) {
     const View &c = a.c;
@@ -117,7 +117,7 @@ __global__ __launch_bounds__(kThreads) void kv_reorder_kernel(ReorderArgs a) {
         parent[i] = p < a.beams ? p : i;   // (an index past the group: the sequence stays)
     }
     // the thread's next kAhead columns of one kind: `pitch` bytes from one sequence to the next
-    constexpr uint32_t kAhead = kBeams <= 8 ? 4 : kBeams <= 16 ? 2 : 1;
+    constexpr uint32_t kAhead = kBeams <= 16 ? 2 : 1;
     auto column = [&](void *memory, size_t pitch, size_t at, size_t bytes) {
         char *const base = static_cast<char *>(memory) + ((size_t)first * c.heads + h) * pitch;
         const size_t next = c.heads * pitch;
