@@ -626,10 +626,19 @@ hipError_t beam_select(bool f32, const BeamShape &b, const void *logits, const f
     else scan(beam_scan_kernel<_Float16>, static_cast<const _Float16 *>(logits));
     const hipError_t status = hipGetLastError();
     if (status != hipSuccess) return status;
-    beam_pick_kernel<<<(uint32_t)b.groups, kPickWaves * kWave, 0, s>>>(
-        entries, sums, scores, ended, (uint32_t)b.beams, p.parts, (uint32_t)b.keep, p.pitch,
-        PickArgs{parents, tokens, new_scores, new_ended, end_token});
-    return hipGetLastError();
+    // (a launch holds fewer than 2^32 threads)
+    constexpr size_t kGroupsPerLaunch = size_t{1} << 22;
+    for (size_t first = 0; first < b.groups; first += kGroupsPerLaunch) {
+        const size_t groups = b.groups - first < kGroupsPerLaunch ? b.groups - first : kGroupsPerLaunch;
+        const size_t row = first * b.beams, list = row * p.parts, out = first * b.keep;
+        beam_pick_kernel<<<(uint32_t)groups, kPickWaves * kWave, 0, s>>>(
+            entries + list * p.pitch, sums + list, scores + row, ended == nullptr ? nullptr : ended + row, (uint32_t)b.beams,
+            p.parts, (uint32_t)b.keep, p.pitch,
+            PickArgs{parents + out, tokens + out, new_scores + out, new_ended == nullptr ? nullptr : new_ended + out, end_token});
+        const hipError_t launched = hipGetLastError();
+        if (launched != hipSuccess) return launched;
+    }
+    return hipSuccess;
 }
 
 }  // namespace k

@@ -2,6 +2,7 @@
 exactly, but where two beams' scores are closer than the log sums are known; scores
 within the roundings that tests/beam_model.py counts."""
 import ctypes
+import threading
 
 import numpy as np
 import pytest
@@ -238,3 +239,55 @@ def test_recorded(sdk):
     sdk.synchronize()
     for exe in runs:
         assert hip.hipGraphExecDestroy(exe) == 0
+
+
+def test_largest_vocabulary(sdk):
+    """2^26 tokens: the last of them, equal ones far apart, and sums of as many terms."""
+    vocab = 2 ** 26
+    logits = np.random.default_rng(18).random((1, 1, vocab), np.float32).astype(np.float16)
+    logits[0, 0, [vocab - 1, 5, vocab // 2 + 1]] = [4, 3, 3]
+    scores = np.array([[-1]], np.float32)
+    got = call_select(sdk, logits, scores, None, vocab - 1, 3)
+    assert got[0].tolist() == [[0, 0, 0]] and got[1].tolist() == [[vocab - 1, 5, vocab // 2 + 1]]
+    assert got[3].tolist() == [[1, 0, 0]]
+    total = sum(np.exp(part.astype(np.float64)).sum() for part in np.array_split(logits[0, 0], 64))
+    # as beam_model.tolerance counts for 128 parts of 512 tiles each
+    off = (3 * 4 + 2 + (8 + 6) * 2 * 513) * 2.0 ** -24
+    assert (np.abs(got[2][0] - (np.array([4, 3, 3]) - 1 - np.log(total))) <= off + 2.0 ** -24 * 20).all()
+
+
+def test_more_groups_than_one_launch_takes(sdk):
+    """Of 2^22 + 3 groups each its own choice."""
+    groups = 2 ** 22 + 3
+    rng = np.random.default_rng(19)
+    logits = rng.integers(-8, 9, (groups, 1, 3)).astype(np.float16)
+    scores = rng.integers(-9, 0, (groups, 1)).astype(np.float32)
+    ended = (rng.random((groups, 1)) < 0.1).astype(np.uint32)
+    parents, tokens, new_scores, new_ended = call_select(sdk, logits, scores, ended, 2, 1)
+    over = ended[:, 0] != 0
+    want = np.where(over, 2, logits[:, 0].argmax(-1))
+    assert (parents == 0).all() and np.array_equal(tokens[:, 0], want) and np.array_equal(new_ended[:, 0], want == 2)
+    x = logits[:, 0].astype(np.float64)
+    s = np.where(over, scores[:, 0], scores[:, 0] + x.max(-1) - np.log(np.exp(x).sum(-1)))
+    # (3 |t| + 2 + (8 + 6) * 2) units at 16 at most, and the score's rounding
+    assert (np.abs(new_scores[:, 0] - s) <= (3 * 16 + 2 + 28 + 16) * 2.0 ** -24).all()
+
+
+def test_threads(sdk):
+    errors = []
+
+    def work(seed):
+        try:
+            rng = np.random.default_rng(seed)
+            for i in range(6):
+                run(sdk, rng, 2, 4, 3001 + seed, 8, ("f16", "f32")[i % 2], ended=i % 3 == 0, device=i % 4 != 3,
+                    what=f"thread {seed}")
+        except BaseException as e:      # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(s,)) for s in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors[0]
