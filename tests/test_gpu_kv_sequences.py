@@ -2,6 +2,7 @@
 hold, bit for bit, and what goes on from there."""
 import copy
 import ctypes
+import threading
 
 import numpy as np
 import pytest
@@ -186,3 +187,53 @@ def test_refusals_leave_the_caches(sdk):
         c.check()
     a.check()
     b.check()
+
+
+def test_copy_past_the_caches(sdk):
+    """More than 96 MB of codes: what the target's sequences hold is what the sources do."""
+    a = Pair(sdk, 2, 1, 8300, 256, 256, 12)
+    a.append(8300, counts=[8300, 8211])
+    target = sdk.kv_cache(26, 1, 8320, 256, 256)
+    source = [b % 2 for b in range(25)] + [KEEP]
+    sdk.call("tensor_kv_cache_copy", a.cache, u32s(source), target)
+    assert target.lengths == [(8300, 8211)[s] if s != KEEP else 0 for s in source]
+    held = []
+    for cache, batch in ((a.cache, 2), (target, 26)):
+        k, v = (sdk.from_numpy(np.full((batch, 1, 8300, 256), 7, np.float16)) for _ in range(2))
+        sdk.call("tensor_kv_cache_read_f16", cache, k, v)
+        held.append([x.download().view(np.uint16) for x in (k, v)])
+    for of, to in zip(*held):
+        for b, s in enumerate(source[:25]):
+            assert np.array_equal(to[b], of[s]), b
+        assert (to[25].view(np.float16) == 7).all()
+
+
+def test_threads(sdk):
+    """Copies between two caches in both directions at once, reorders and reads among
+    them: all end, and of sequences alike every one stays what it is."""
+    pairs = [filled(sdk, 4, 2, 200, (64, 32), [130] * 4, 13) for _ in range(2)]
+    first = [KEEP, 0, KEEP, 0]
+    for pair in pairs:
+        sdk.call("tensor_kv_cache_copy", pair.cache, u32s([KEEP, 0, 0, 0]), pair.cache)
+        pair.model = copied(pair.model, [KEEP, 0, 0, 0], pair.model)
+    errors = []
+
+    def work(i):
+        try:
+            a, b = pairs[i % 2], pairs[1 - i % 2]
+            parents = sdk.from_numpy(np.array([[3, 2, 1, 0]], np.uint32))
+            for _ in range(40):
+                sdk.call("tensor_kv_cache_copy", a.cache, u32s(first), b.cache)
+                sdk.call("tensor_kv_cache_reorder", b.cache, parents)
+            a.check(f"thread {i}")
+        except BaseException as e:      # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors[0]
+    for pair in pairs:
+        pair.check()

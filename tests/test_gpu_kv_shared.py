@@ -2,6 +2,7 @@
 plain model's attention over both as one sequence: outputs within the roundings that
 tests/kv_model.py counts, special rows exactly."""
 import ctypes
+import threading
 
 import numpy as np
 import pytest
@@ -10,6 +11,7 @@ from tests import beam_model
 from tests.kv_model import u32s
 from tests.test_gpu_kv_attention import compare
 from tests.test_gpu_kv_cache import DTYPES, Pair, rows_of
+from tests.test_gpu_kv_sequences import copied
 
 pytestmark = pytest.mark.gpu
 
@@ -219,6 +221,84 @@ def test_recorded(sdk, dtype):
     sdk.synchronize()
     for exe, _ in runs:
         assert hip.hipGraphExecDestroy(exe) == 0
+
+
+def remembered(prefix):
+    """The prefix's model with its exact values worked out once."""
+    for heads in prefix.model.k + prefix.model.v:
+        for head in heads:
+            exact = head.held()
+            head.held = lambda exact=exact: exact
+
+
+@pytest.mark.parametrize("dims,tokens,dtype", [((128, 96), 16300, "f16"), ((64, 64), 32800, "f16"), ((200, 256), 8100, "f16"),
+                                               ((64, 128), 22000, "f32")], ids=str)
+def test_many_rows_on_a_long_prefix(sdk, dims, tokens, dtype):
+    """Products enough for tiles over the prefix beside few rows over own tokens."""
+    prefix = pair_of(sdk, 1, dims, [tokens], 34)
+    remembered(prefix)
+    own = pair_of(sdk, 1, dims, [(37 * b) % 200 for b in range(40)], 35)
+    run(prefix, own, dtype, 2, 16, causal=False, counts=[16 if b % 5 else b % 17 for b in range(40)])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("dims", [(64, 64), (40, 33)], ids=str)
+def test_few_rows_on_a_long_prefix(sdk, dims, dtype):
+    """Many parts of few rows, and of more rows."""
+    prefix = pair_of(sdk, 1, dims, [30000], 36)
+    remembered(prefix)
+    own = pair_of(sdk, 1, dims, [300, 20, 0, 64], 37)
+    run(prefix, own, dtype, 4, 1, causal=False, counts=[1, 1, 0, 1], what="few")
+    own = pair_of(sdk, 1, dims, [300 + i for i in range(20)], 38)
+    run(prefix, own, dtype, 2, 13, counts=[13 - i % 4 for i in range(20)], what="more")
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("dims", [(33, 7), (64, 64), (72, 96), (128, 128), (160, 192), (256, 256)], ids=str)
+def test_short_own_tokens_of_many(sdk, dims, dtype):
+    """Sequences enough to fill the chip, of 0 to 512 own tokens each."""
+    rng = np.random.default_rng(39)
+    prefix = pair_of(sdk, 4, dims, [100, 1, 65], 40)
+    own = pair_of(sdk, 4, dims, [0, 512] + [int(n) for n in rng.integers(0, 513, 68)], 41)
+    members = [30, 0, 40]
+    run(prefix, own, dtype, 12, 1, members, causal=False, what="one")
+    counts = [int(c) for c in rng.integers(0, 7, 70)]
+    own = pair_of(sdk, 4, dims, [int(n) for n in rng.integers(6, 513, 70)], 42)
+    run(prefix, own, dtype, 16, 6, members, counts=counts, what="six")
+
+
+def test_codes_past_the_caches(sdk):
+    """Lengths for which codes are read as a stream."""
+    dims = (128, 128)
+    some = pair_of(sdk, 1, dims, [4000, 70, 1, 64], 43)
+    own = Pair(sdk, 200, 1, 4000, *dims, seed=44)
+    source = [0] + [1 + b % 3 for b in range(199)]
+    sdk.call("tensor_kv_cache_copy", some.cache, u32s(source), own.cache)
+    own.model = copied(some.model, source, own.model)
+    prefix = pair_of(sdk, 1, dims, [150, 3], 45)
+    for dtype in ("f16", "f32"):
+        run(prefix, own, dtype, 2, 1, [150, 50], what=dtype)
+
+
+def test_threads_share_a_prefix(sdk):
+    prefix = pair_of(sdk, 2, (64, 64), [200, 90], 46)
+    errors = []
+
+    def work(seed):
+        try:
+            own = pair_of(sdk, 2, (64, 64), [60, 3, 64, 5], seed, capacity=100)
+            for i in range(5):
+                own.append(1)
+                run(prefix, own, ("f16", "f32")[i % 2], 4, 1 + i % 3, what=f"thread {seed}")
+        except BaseException as e:      # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(50 + s,)) for s in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors, errors[0]
 
 
 def test_refusals(sdk):
