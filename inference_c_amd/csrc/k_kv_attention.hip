@@ -16,7 +16,7 @@ __global__ __launch_bounds__(kThreads) void kv_rows_kernel(const uint8_t *keys, 
                                                            uint32_t all_blocks, uint32_t heads, uint32_t parts_first,
                                                            uint32_t pitches, uint32_t n, uint32_t group, Args<S> a) {
     __shared__ RowsOut<P> lds_o;
-    __shared__ RowsMl lds_ml;
+    __shared__ RowsMl<> lds_ml;
     rows_of<S, P, kStream, false>(lds_o, lds_ml, keys, values, lengths, metas, queries, all_blocks, heads, parts_first, pitches, n, group,
                            kernel_arguments<Args<S>>(kRowsArguments), blockIdx.x, blockIdx.y, blockIdx.z);
 }

@@ -1,7 +1,8 @@
 // Attention over the 8-bit cache of sequences whose tokens follow a prefix that
 // several of them share.
 //
-// Two passes into the same rows' parts: over the prefix the rows of a group's sequences
+// Of few tokens a workgroup has both, a wave some blocks of either (kv_shared_close_kernel).
+// Else two passes into the same rows' parts: over the prefix the rows of a group's sequences
 // are packed as one head's rows, so that its codes are read once for 16 or 128 of them,
 // and over each sequence's own tokens as in attention without a prefix. A softmax over
 // both is their parts' join (kv_fold_kernel). The passes are one launch: neither waits
@@ -22,7 +23,7 @@ template <typename S> struct Both {
 // Workgroup i of a pass by the rows kernel; kSolo: each wave does what a workgroup
 // would, the waves of four of them.
 template <typename S, uint32_t P, bool kStream, bool kSolo>
-__device__ __forceinline__ void rows_of(RowsOut<P> &lds_o, RowsMl &lds_ml, Constant<SharedArgs<S>> &a, uint32_t i) {
+__device__ __forceinline__ void rows_of(RowsOut<P> &lds_o, RowsMl<> &lds_ml, Constant<SharedArgs<S>> &a, uint32_t i) {
     if constexpr (kSolo) {
         i = i * kWaves + (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
         if (i >= a.columns * a.pairs) return;
@@ -35,7 +36,7 @@ __device__ __forceinline__ void rows_of(RowsOut<P> &lds_o, RowsMl &lds_ml, Const
 template <typename S, uint32_t P, bool kStream>
 __global__ __launch_bounds__(kThreads) void kv_shared_rows_kernel(Both<S>) {
     __shared__ RowsOut<P> lds_o;
-    __shared__ RowsMl lds_ml;
+    __shared__ RowsMl<> lds_ml;
     auto &both = kernel_arguments<Both<S>>(0);
     const uint32_t second = blockIdx.x >= both.first ? 1 : 0;
     rows_of<S, P, kStream, false>(lds_o, lds_ml, both.pass[second], blockIdx.x - (second ? both.first : 0));
@@ -45,7 +46,7 @@ __global__ __launch_bounds__(kThreads) void kv_shared_rows_kernel(Both<S>) {
 template <typename S, uint32_t P>
 __global__ __launch_bounds__(kThreads) void kv_shared_solo_kernel(Both<S>) {
     __shared__ RowsOut<P> lds_o;
-    __shared__ RowsMl lds_ml;
+    __shared__ RowsMl<> lds_ml;
     auto &both = kernel_arguments<Both<S>>(0);
     if (blockIdx.x < both.first) rows_of<S, P, false, false>(lds_o, lds_ml, both.pass[0], blockIdx.x);
     else rows_of<S, P, false, true>(lds_o, lds_ml, both.pass[1], blockIdx.x - both.first);
@@ -64,7 +65,7 @@ __global__ __launch_bounds__(kThreads, tiles_twice(sizeof(S) == 4, P) ? 2 : 1) v
 // Tiles over the prefix, rows over own tokens.
 template <typename S, uint32_t P>
 __global__ __launch_bounds__(kThreads, 2) void kv_shared_mixed_kernel(Both<S>) {
-    static_assert(tiles_twice(sizeof(S) == 4, P) && sizeof(RowsOut<P>) + sizeof(RowsMl) <= sizeof(typename TilesLds<P>::Keys));
+    static_assert(tiles_twice(sizeof(S) == 4, P) && sizeof(RowsOut<P>) + sizeof(RowsMl<>) <= sizeof(typename TilesLds<P>::Keys));
     __shared__ __attribute__((aligned(16))) typename TilesLds<P>::Keys ks;
     __shared__ __attribute__((aligned(16))) typename TilesLds<P>::Values vs;
     __shared__ typename TilesLds<P>::Most wave_most;
@@ -74,9 +75,26 @@ __global__ __launch_bounds__(kThreads, 2) void kv_shared_mixed_kernel(Both<S>) {
     } else {
         char *const lds = reinterpret_cast<char *>(ks);
         rows_of<S, P, false, false>(*reinterpret_cast<RowsOut<P> *>(lds),
-                                    *reinterpret_cast<RowsMl *>(lds + sizeof(RowsOut<P>)), both.pass[1],
+                                    *reinterpret_cast<RowsMl<> *>(lds + sizeof(RowsOut<P>)), both.pass[1],
                                     blockIdx.x - both.first);
     }
+}
+
+// Both by one workgroup, and no parts: of its eight waves four have the prefix and four
+// own tokens, of one sequence's rows.
+template <typename S, uint32_t P>
+__global__ __launch_bounds__(2 * kThreads) void kv_shared_close_kernel(Both<S>) {
+    constexpr uint32_t kMeet = 2 * kWaves;
+    __shared__ RowsOut<P, kMeet> lds_o;
+    __shared__ RowsMl<kMeet> lds_ml;
+    auto &both = kernel_arguments<Both<S>>(0);
+    const uint32_t second = (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x / kThreads);
+    auto &a = both.pass[second];
+    const uint32_t pair = blockIdx.x % a.pairs, x = blockIdx.x / a.pairs, h = pair % a.c.heads, b = pair / a.c.heads;
+    const uint32_t sequence = both.pass[1].first + b, of = second ? sequence : both.pass[0].count.n[b];
+    rows_of<S, P, false, false, kMeet>(lds_o, lds_ml, a.c.k, a.c.v, a.c.length, a.c.meta, a.q, a.c.blocks, a.c.heads, 1,
+                                       a.c.kp | a.c.vp << 16, a.n, a.group, a, x, h, of,
+                                       OwnRows{sequence, both.pass[1].count.n[b]});
 }
 
 // ---- the parts' join ------------------------------------------------------------------------
@@ -160,6 +178,7 @@ struct Pass {
 };
 struct SharedPlan {
     Pass prefix, own;
+    bool close;      // both by one workgroup
     bool together;   // in one launch
     uint32_t n;      // rows of a prefix's head
     size_t rows, o_bytes, ml_bytes;
@@ -181,13 +200,40 @@ uint64_t workgroups_of(const View &c, const Pass &p) {
     return p.solo ? (n + kWaves - 1) / kWaves : n;
 }
 
+// Few blocks are done by one workgroup of a sequence's rows (kv_shared_close_kernel): no
+// parts and no join, but a prefix is read for each sequence. Measured (us, the call, a
+// workgroup for both and parts; 2 prefixes, own tokens of 200, 8 heads, workgroups x tokens
+// of a prefix): f16 D 64, 64 x 250 7.7 and 11.3, 64 x 1000 9.1 and 11.1, 64 x 2000 (own 50)
+// 11.9 and 9.4, 512 x 500 11.9 and 14.7, 1024 x 500 19 and 17; D 128, 64 x 500 10.5 and 12.4,
+// 64 x 1000 14.4 and 13.1, 256 x 500 12.7 and 18.9, 512 x 250 20 and 19; D 192, 64 x 500 15.1
+// and 15.1, 256 x 500 17 and 23; f32 D 32, 64 x 1000 9.1 and 11.0, 512 x 500 10.5 and 12.1; D
+// 64, 64 x 500 8.8 and 11.2, 64 x 1000 11.7 and 11.5, 512 x 250 15.3 and 15.0; D 128, 64 x
+// 250 11.0 and 13.0, 64 x 500 14.0 and 13.8, 256 x 500 15.6 and 17.4; D 80, 64 x (500, own
+// 300) 11.8 and 10.2.
+constexpr uint32_t kCloseBlocks = 12, kCloseBlocksMore = 20, kCloseWorkgroups = 256;
+// (wider ones do not find registers for eight waves)
+constexpr bool close_built(bool f32, uint32_t widest) { return widest <= (f32 ? 128u : 192u); }
+bool close_fits(bool f32, const PrefixShape &ps, const View &c, const AttentionShape &a) {
+    const uint32_t widest = widest_of(c), in_head = a.q_heads / c.heads * a.n;
+    const uint32_t row_groups = (in_head + kRows - 1) / kRows;
+    const uint64_t blocks = ((uint64_t)ps.longest + kTokens - 1) / kTokens + ((uint64_t)a.longest + kTokens - 1) / kTokens;
+    const bool twice = widest <= (f32 ? 32u : 64u);   // two workgroups in a CU
+    return close_built(f32, widest) && blocks <= (widest <= (f32 ? 32u : 96u) ? kCloseBlocksMore : kCloseBlocks) &&
+           (uint64_t)a.batch * c.heads * row_groups <= (twice ? 2 : 1) * kCloseWorkgroups;
+}
+
 SharedPlan plan_of(bool f32, const View &prefix, const PrefixShape &ps, const View &c, const AttentionShape &a) {
-    SharedPlan p;
+    SharedPlan p{};
     const uint32_t widest = widest_of(c), own_rows = a.q_heads / c.heads * a.n;
     p.n = ps.most * own_rows;
     const Plan over = icsdk::kv::plan_of(f32, prefix, AttentionShape{ps.batch, prefix.heads, p.n, ps.longest, a.scale, false,
                                                                      nullptr, nullptr, 0, 0});
     const Plan own = icsdk::kv::plan_of(f32, c, a);
+    p.close = close_fits(f32, ps, c, a);
+    if (p.close) {
+        p.own = pass_of(c, false, a.batch, own_rows, a.longest, 1);
+        return p;
+    }
     // beside a pass by tiles another one by tiles needs no products enough to fill the chip
     const bool own_tiles = own.tiles || (over.tiles && own.many), prefix_tiles = over.tiles || (own_tiles && over.many);
     const bool mixed = prefix_tiles && !own_tiles;
@@ -255,6 +301,19 @@ template <typename S, uint32_t P> hipError_t launch(const Both<S> &both, uint32_
         if (k.solo) return go(kv_shared_solo_kernel<S, P>);
     return k.stream ? go(kv_shared_rows_kernel<S, P, true>) : go(kv_shared_rows_kernel<S, P, false>);
 }
+template <typename S> hipError_t launch_close(const Both<S> &both, uint32_t widest, uint32_t grid, hipStream_t s) {
+    auto go = [&](auto kernel) {
+        kernel<<<grid, 2 * kThreads, 0, s>>>(both);
+        return hipGetLastError();
+    };
+    if (widest <= 32) return go(kv_shared_close_kernel<S, 32>);
+    if (widest <= 64) return go(kv_shared_close_kernel<S, 64>);
+    if (widest <= 96) return go(kv_shared_close_kernel<S, 96>);
+    if (widest <= 128) return go(kv_shared_close_kernel<S, 128>);
+    if constexpr (close_built(sizeof(S) == 4, 192))
+        if (widest <= 192) return go(kv_shared_close_kernel<S, 192>);
+    return hipErrorInvalidValue;   // (no plan has them)
+}
 template <typename S>
 hipError_t launch(const Both<S> &both, uint32_t widest, uint32_t grid, const Kernels &k, hipStream_t s) {
     if (widest <= 32) return launch<S, 32>(both, grid, k, s);
@@ -278,6 +337,29 @@ hipError_t run(const View &prefix, const PrefixShape &ps, const View &c, const A
     own.part_ml = reinterpret_cast<f32x2 *>(static_cast<char *>(workspace) + p.o_bytes);
     own.rows = p.rows;
     own.scale2 = (double)sh.scale * kLog2e;
+    if (p.close) {
+        own.c = c;
+        own.group = group;
+        own.n = sh.n;
+        own.parts = 1;
+        own.row_groups = p.own.row_groups;
+        over = own;
+        over.c = prefix;
+        own.causal = sh.causal;
+        uint32_t on = 0, left = ps.members[0];
+        for (own.first = 0; own.first < sh.batch; own.first += kBatchPerLaunch) {
+            const uint32_t batch = sh.batch - own.first < kBatchPerLaunch ? sh.batch - own.first : kBatchPerLaunch;
+            for (uint32_t b = 0; b < batch; ++b, --left) {
+                while (left == 0) left = ps.members[++on];
+                over.count.n[b] = on;
+                own.count.n[b] = sh.counts ? sh.counts[own.first + b] : sh.n;
+            }
+            over.pairs = own.pairs = batch * c.heads;
+            const hipError_t status = launch_close(both, widest_of(c), own.pairs * own.row_groups, s);
+            if (status != hipSuccess) return status;
+        }
+        return hipSuccess;
+    }
     over = own;
     over.c = prefix;
     over.group = 1;   // a group's rows are one head's rows there

@@ -122,19 +122,25 @@ template <bool kStream, typename V> __device__ inline V load_codes(const V *p) {
 // out of 12 with the struct alone.)
 // A is Args, or SharedArgs for a pass of attention over a prefix and own tokens. kSolo
 // (of such a pass): a wave has 16 rows and a part by itself, and its own x, h and b.
-template <uint32_t P> using RowsOut = f32x4[kWaves][P / 16][kWave];
-using RowsMl = f32x4[kWaves][kRows];   // maximum, sums of P rounded and not
-template <typename S, uint32_t P, bool kStream, bool kSolo, typename A>
-__device__ __forceinline__ void rows_of(RowsOut<P> &lds_o, RowsMl &lds_ml, const uint8_t *keys, const uint8_t *values,
+// kMeet of 8: four waves have the prefix, where b is the sequence's one, and four its own
+// tokens; rows are those of `own`, and all eight meet.
+template <uint32_t P, uint32_t kMeet = kWaves> using RowsOut = f32x4[kMeet][P / 16][kWave];
+template <uint32_t kMeet = kWaves> using RowsMl = f32x4[kMeet][kRows];   // maximum, sums of P rounded and not
+struct OwnRows {
+    uint32_t sequence, count;
+};
+template <typename S, uint32_t P, bool kStream, bool kSolo, uint32_t kMeet = kWaves, typename A>
+__device__ __forceinline__ void rows_of(RowsOut<P, kMeet> &lds_o, RowsMl<kMeet> &lds_ml, const uint8_t *keys, const uint8_t *values,
                                         const uint32_t *lengths, const Meta *metas, const S *queries, uint32_t all_blocks,
                                         uint32_t heads, uint32_t parts_first, uint32_t pitches, uint32_t n,
-                                        uint32_t group, A &a, uint32_t x, uint32_t h, uint32_t b) {
-    constexpr bool kPair = sizeof(S) == 4, kShared = kIsShared<A>;
+                                        uint32_t group, A &a, uint32_t x, uint32_t h, uint32_t b,
+                                        OwnRows own = {}) {
+    constexpr bool kPair = sizeof(S) == 4, kShared = kIsShared<A>, kBoth = kMeet != kWaves;
     constexpr uint32_t NC = P / 64, NV = P / 16;
     constexpr bool kOdd = P % 64 != 0;
     auto &c = a.c;
     const uint32_t lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
-    const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const uint32_t place = (uint32_t)__builtin_amdgcn_readfirstlane(threadIdx.x / kWave), wave = kBoth ? place % kWaves : place;
     const uint32_t parts = parts_first & 0xffffu, kp = pitches & 0xffffu, vp = pitches >> 16;
     const uint32_t seq = (parts_first >> 16) + b;
     const uint32_t length = lengths[seq];
@@ -178,7 +184,7 @@ __device__ __forceinline__ void rows_of(RowsOut<P> &lds_o, RowsMl &lds_ml, const
         load_k(t);
         load_v(t);
     }
-    const uint32_t in_head = group * n, count = rows_there(a, b);
+    const uint32_t in_head = group * n, count = kBoth ? own.count : rows_there(a, b);
     // (the last rows, which see most keys, first)
     const uint32_t row0 = (a.row_groups - 1 - a.row_group0 - x / parts) * kRows;
     // what the rows see, from the first one's place among its query head's n
@@ -194,7 +200,8 @@ __device__ __forceinline__ void rows_of(RowsOut<P> &lds_o, RowsMl &lds_ml, const
     const uint32_t r = row0 + m, i = n == 1 ? 0 : r % n;
     const bool live = r < in_head && i < count;
     size_t row = head * in_head + (r < in_head ? r : in_head - 1);   // (rows past the head repeat its last)
-    if constexpr (kShared) row = shared_row(a, r, b, h, in_head, count);
+    if constexpr (kBoth) row = ((size_t)own.sequence * heads + h) * in_head + min(r, in_head - n + max(count, 1u) - 1);
+    else if constexpr (kShared) row = shared_row(a, r, b, h, in_head, count);
     const int seen = seen_by(i, live, length, count, a.causal);
     Query<S, P> q;
     q.load(queries + row * c.dim, c.dim, g);
@@ -364,31 +371,31 @@ __device__ __forceinline__ void rows_of(RowsOut<P> &lds_o, RowsMl &lds_ml, const
         if (g == 0) a.part_ml[(size_t)part * a.rows + row] = f32x2{big, sum};
         return;
     }
-    if (g == 0) lds_ml[wave][m] = f32x4{big, sum, exact, 0.0f};
+    if (g == 0) lds_ml[place][m] = f32x4{big, sum, exact, 0.0f};
 #pragma unroll
-    for (uint32_t j = 0; j < NV; ++j) lds_o[wave][j][lane] = o[j] * (unit / kPairScale<S>);
+    for (uint32_t j = 0; j < NV; ++j) lds_o[place][j][lane] = o[j] * (unit / kPairScale<S>);
     __syncthreads();
-    float top = neg_inf, total = 0.0f, total_exact = 0.0f, w[kWaves];
+    float top = neg_inf, total = 0.0f, total_exact = 0.0f, w[kMeet];
 #pragma unroll
-    for (uint32_t k = 0; k < kWaves; ++k) top = fmaxf(top, lds_ml[k][m].x);
+    for (uint32_t k = 0; k < kMeet; ++k) top = fmaxf(top, lds_ml[k][m].x);
 #pragma unroll
-    for (uint32_t k = 0; k < kWaves; ++k) {
+    for (uint32_t k = 0; k < kMeet; ++k) {
         // (a wave that saw nothing has weight 0, and a NaN in it stays)
         w[k] = top == neg_inf ? 1.0f : __builtin_amdgcn_exp2f(lds_ml[k][m].x - top);
         total += w[k] * lds_ml[k][m].y;
         total_exact += w[k] * lds_ml[k][m].z;
     }
     const bool writes = live && r < in_head;
-    if (!kShared && parts == 1) {
+    if (kBoth || (!kShared && parts == 1)) {
         S *const out = a.out + row * c.vdim;
 #pragma unroll
-        for (uint32_t j = wave; j < NV; j += kWaves) {
+        for (uint32_t j = place; j < NV; j += kMeet) {
             f32x4 v = {0, 0, 0, 0};
 #pragma unroll
-            for (uint32_t k = 0; k < kWaves; ++k) v += lds_o[k][j][lane] * w[k];
+            for (uint32_t k = 0; k < kMeet; ++k) v += lds_o[k][j][lane] * w[k];
             if (writes) store_out(out, c.vdim, 16 * j + 4 * g, finish(v, top, total));
         }
-        if (writes && g == 0 && wave == 0) {
+        if (writes && g == 0 && place == 0) {
             if (a.row_ml != nullptr) a.row_ml[row] = weight_terms(top, total_exact);
             if (a.scores != nullptr) {
                 a.part_ml[row] = f32x2{top, total};
@@ -398,13 +405,13 @@ __device__ __forceinline__ void rows_of(RowsOut<P> &lds_o, RowsMl &lds_ml, const
     } else {
         float *const out = a.part_o + ((size_t)part * a.rows + row) * c.vdim;
 #pragma unroll
-        for (uint32_t j = wave; j < NV; j += kWaves) {
+        for (uint32_t j = place; j < NV; j += kMeet) {
             f32x4 v = {0, 0, 0, 0};
 #pragma unroll
-            for (uint32_t k = 0; k < kWaves; ++k) v += lds_o[k][j][lane] * w[k];
+            for (uint32_t k = 0; k < kMeet; ++k) v += lds_o[k][j][lane] * w[k];
             if (writes) store_out(out, c.vdim, 16 * j + 4 * g, v);
         }
-        if (writes && g == 0 && wave == 0) {
+        if (writes && g == 0 && place == 0) {
             a.part_ml[(size_t)part * a.rows + row] = f32x2{top, total};
             if (a.part_exact != nullptr) a.part_exact[(size_t)part * a.rows + row] = total_exact;
         }

@@ -182,12 +182,35 @@ def test_many_sequences(sdk, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
-def test_recorded(sdk, dtype):
+@pytest.mark.parametrize("dims", [(1, 1), (8, 24), (33, 7), (32, 32), (72, 72), (96, 64), (100, 36), (128, 128), (64, 128),
+                                  (192, 128), (200, 250), (256, 256)], ids=str)
+def test_head_dims_on_a_longer_prefix(sdk, dims, dtype):
+    prefix = pair_of(sdk, 2, dims, [1400, 130], 60)
+    own = pair_of(sdk, 2, dims, [40, 70, 33, 128], 61)
+    run(prefix, own, dtype, 6, 1, what=f"{dims} decode")
+    run(prefix, own, dtype, 4, 19, members=[3, 1], counts=[19, 5, 0, 18], what=f"{dims} chunk")
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_many_short_sequences(sdk, dtype):
+    """More sequences than one launch takes, of few tokens, on prefixes of several and none."""
+    rng = np.random.default_rng(62)
+    prefix = pair_of(sdk, 1, (16, 32), [int(n) for n in rng.integers(0, 200, 40)], 63)
+    members = [p % 2 * 13 for p in range(40)]
+    members[7] += 30
+    own = pair_of(sdk, 1, (16, 32), [int(n) for n in rng.integers(0, 70, 290)], 64)
+    run(prefix, own, dtype, 3, 1, members, causal=False)
+    run(prefix, own, dtype, 2, 3, members, causal=False, counts=[int(c) for c in rng.integers(0, 4, 290)])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("before,room", [([900, 650], (1000, 400)), ([250, 100], (330, 300))], ids=str)
+def test_recorded(sdk, before, room, dtype):
     """Two recorded calls share nothing: replays follow the caches while eager calls
     take scratch memory in between."""
     hip, stream = sdk.lib, ctypes.c_void_p(sdk.stream())
-    prefix = pair_of(sdk, 2, (64, 64), [900, 650], 27, capacity=1000)
-    own = pair_of(sdk, 2, (64, 64), [30, 20, 64, 1], 28, capacity=400)
+    prefix = pair_of(sdk, 2, (64, 64), before, 27, capacity=room[0])
+    own = pair_of(sdk, 2, (64, 64), [30, 20, 64, 1], 28, capacity=room[1])
     rng = np.random.default_rng(29)
     qs = [rng.standard_normal((4, 4, n, 64)).astype(DTYPES[dtype]) for n in (1, 5)]
     outs, runs = [], []
