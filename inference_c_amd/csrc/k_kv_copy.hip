@@ -47,9 +47,9 @@ __device__ inline void copy_run(const void *from, void *to, size_t bytes) {
 
 // A workgroup: 16 KB of one (sequence, head)'s codes; the last one of each the rest.
 // Bound by memory: 4 sequences of 2000 tokens of 8 heads of 128 + 128 into 32 (131 MB
-// written) 24 us, 5.4 TB/s and more than a copy, the sources being found in the caches.
-// Codes past what the caches hold to the next call are written as a stream (kStream):
-// 131 MB copied and read back 129 -> 115 us; 64 MB 90, as a stream 92.
+// written, the sources being found in the caches) 24 us, 5.4 TB/s. Codes past what the caches
+// hold to the next call are written as a stream (kStream): that copy then takes 34 us, but
+// its read 87 for 104, both 115 for 129; 64 MB 90, as a stream 92.
 constexpr size_t kStreamBytes = size_t{96} << 20;
 
 template <bool kStream>

@@ -5,7 +5,7 @@
 // Else two passes into the same rows' parts: over the prefix the rows of a group's sequences
 // are packed as one head's rows, so that its codes are read once for 16 or 128 of them,
 // and over each sequence's own tokens as in attention without a prefix. A softmax over
-// both is their parts' join (kv_fold_kernel). The passes are one launch: neither waits
+// both is their parts' join (kv_join_kernel; kv_fold_kernel for many parts of few rows). The passes are one launch: neither waits
 // for the other, and where the prefix is bound by its products (tiles) and the own
 // tokens by memory (rows), a CU has one of each.
 #include "kv_rows.hpp"
@@ -33,6 +33,9 @@ __device__ __forceinline__ void rows_of(RowsOut<P> &lds_o, RowsMl<> &lds_ml, Con
                                   a.parts | a.first << 16, a.c.kp | a.c.vp << 16, a.n, a.group, a, x, h, b);
 }
 
+// Both by the rows kernel. 14 f32 sequences of 130 tokens with 4 rows of 16 heads on three
+// prefixes of 1500, D 80: 11 us, and the join 4, for 4 MB of codes: bound by a workgroup's
+// chain (arguments, lengths, queries, two or three blocks for each wave, the waves' meeting).
 template <typename S, uint32_t P, bool kStream>
 __global__ __launch_bounds__(kThreads) void kv_shared_rows_kernel(Both<S>) {
     __shared__ RowsOut<P> lds_o;
@@ -42,7 +45,10 @@ __global__ __launch_bounds__(kThreads) void kv_shared_rows_kernel(Both<S>) {
     rows_of<S, P, kStream, false>(lds_o, lds_ml, both.pass[second], blockIdx.x - (second ? both.first : 0));
 }
 
-// Own tokens by waves alone.
+// Own tokens by waves alone. 8 x 8 sequences of 100 tokens on 2000, 32/8 heads of 128: 18 us
+// for 47 MB (2.6 TB/s), bound by latency: three blocks for each wave of the prefix, one
+// after another, and registers for two workgroups in a CU. A fourth part of the prefix is a
+// second round of workgroups (the call 28 us for 21); three in a CU spill registers (27).
 template <typename S, uint32_t P>
 __global__ __launch_bounds__(kThreads) void kv_shared_solo_kernel(Both<S>) {
     __shared__ RowsOut<P> lds_o;
@@ -52,6 +58,10 @@ __global__ __launch_bounds__(kThreads) void kv_shared_solo_kernel(Both<S>) {
     else rows_of<S, P, false, true>(lds_o, lds_ml, both.pass[1], blockIdx.x - both.first);
 }
 
+// Both by tiles. Four sequences' 512 rows behind 8000 tokens, 32/8 heads of 128, f16: 320 us,
+// 865 TFLOP/s, bound as kv_tiles_kernel is. A pass over own tokens that goes on over the
+// prefix, without parts, took 344 us against 322 and the join's 16: its workgroups end all
+// at once.
 template <typename S, uint32_t P>
 __global__ __launch_bounds__(kThreads, tiles_twice(sizeof(S) == 4, P) ? 2 : 1) void kv_shared_tiles_kernel(Both<S>) {
     __shared__ __attribute__((aligned(16))) typename TilesLds<P>::Keys ks;
@@ -62,7 +72,11 @@ __global__ __launch_bounds__(kThreads, tiles_twice(sizeof(S) == 4, P) ? 2 : 1) v
     tiles_of<S, P, false>(ks, vs, wave_most, both.pass[second], blockIdx.x - (second ? both.first : 0));
 }
 
-// Tiles over the prefix, rows over own tokens.
+// Tiles over the prefix, rows over own tokens. 64 sequences of up to 500 tokens on 16000,
+// 32/8 heads of 128, f16: 40 us, where the tiles alone take 35 and the rows alone 18. Bound
+// by a tile's turn (1.8 us with one workgroup of tiles in a CU, 16 turns each). More parts
+// (24: 56 us for 48, the call), or own workgroups before some of the prefix's (58 to 75 us),
+// make the passes follow each other.
 template <typename S, uint32_t P>
 __global__ __launch_bounds__(kThreads, 2) void kv_shared_mixed_kernel(Both<S>) {
     static_assert(tiles_twice(sizeof(S) == 4, P) && sizeof(RowsOut<P>) + sizeof(RowsMl<>) <= sizeof(typename TilesLds<P>::Keys));
@@ -81,7 +95,8 @@ __global__ __launch_bounds__(kThreads, 2) void kv_shared_mixed_kernel(Both<S>) {
 }
 
 // Both by one workgroup, and no parts: of its eight waves four have the prefix and four
-// own tokens, of one sequence's rows.
+// own tokens, of one sequence's rows. Four sequences of 20 tokens on 200, 9/3 heads of 64:
+// 6.4 us (6.1 and the join's 1.8 by parts), a chain of latencies.
 template <typename S, uint32_t P>
 __global__ __launch_bounds__(2 * kThreads) void kv_shared_close_kernel(Both<S>) {
     constexpr uint32_t kMeet = 2 * kWaves;
@@ -110,7 +125,10 @@ struct JoinArgs {
     Counts count;
 };
 
-// kHeld parts are asked for at once (past the last one that again, and not used).
+// A thread has four elements of a row; kHeld parts are asked for at once. 4 x 32 heads x 512
+// rows of two parts (67 MB read, 17 written) 16 us, 5.2 TB/s; by four waves for each row 32.
+// Few rows of a few parts: 3.8 us, two latencies and the launch. (Past the
+// last part that one again, and not used.)
 template <typename S, uint32_t kHeld> __global__ __launch_bounds__(kThreads) void kv_join_kernel(S *out, JoinArgs a) {
     const uint32_t i = blockIdx.x * kThreads + threadIdx.x, r = fast_div(i, a.per_row), d = 4 * (i - r * a.per_row.divisor);
     if (r >= a.all) return;
