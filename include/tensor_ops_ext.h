@@ -194,7 +194,9 @@ int tensor_argmax_f16(const TensorBuffer *input, TensorBuffer *index_output,
        scores[b] + logits[b, v] - log(sum_v exp(logits[b, v])),
    in that order, compared in 64 bits (of equal ones the lower beam, then the larger
    logit, then the lower token): parents[j] = b, tokens[j] = v, new_scores[j]
-   the score rounded to f32, and new_ended[j] = (v == end_token).
+   the score rounded to f32, and new_ended[j] = (v == end_token). The sums are of f32
+   exponentials: a beam's log sum is known to 1e-7 or better in general and to
+   (2 log(vocab) + 6) 2^-24 in any case, and beams closer than that may change places.
    logits [groups, beams, vocab], scores F32 [groups, beams], ended U32 [groups,
    beams] or NULL, parents and tokens U32 and new_scores F32 [groups, keep],
    new_ended U32 [groups, keep] or NULL. 1 to 64 beams, keep 1 to 64, vocab up

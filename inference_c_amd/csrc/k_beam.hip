@@ -7,9 +7,12 @@
 // largest logits in order; beam_pick_kernel, a workgroup per group, joins the sums of a
 // row and takes the best of all parts' candidates by their scores.
 //
-// Scores are f64 from exact logits; of the log sums only the exponentials are f32,
-// each off by 2^-23 or so in either direction, so that a sum of many is off by far less
-// and two beams' candidates change places only where their scores are equal to 1e-8.
+// Scores are f64 from exact logits; of the log sums only the exponentials, and the sums of
+// 16 of them, are f32. An exponential of t = x - max is off by at most (2 |t| + 2) 2^-24 of
+// itself (t and its exponent rounded, and the last place), a sum of 16 by four roundings
+// more, so a log sum by (2 log vocab + 6) 2^-24 at the very most, where all terms round the
+// same way; 4e-8 is the largest seen over plateaus, steps and rows far from 0. Two beams'
+// candidates change places only where their scores are that close.
 #include "kernels.hpp"
 #include "kern_common.hpp"
 
@@ -122,9 +125,14 @@ struct ScanArgs {
 };
 
 // exp(t) for t <= 0 (and NaN): log2 e in two pieces, so that the exponent is off by
-// the rounding of one product alone.
+// one rounding alone.
 __device__ inline float exp_below(float t) {
-    return __builtin_amdgcn_exp2f(__builtin_fmaf(t, 1.925963033500001e-8f, t * 1.4426950216293335f));
+    return __builtin_amdgcn_exp2f(__builtin_fmaf(t, 1.4426950216293335f, t * 1.925963033500001e-8f));
+}
+// Pairwise: no term is rounded more than log2 N times.
+template <uint32_t N> __device__ inline float sum_of(const float *x) {
+    if constexpr (N == 1) return x[0];
+    else return sum_of<N / 2>(x) + sum_of<N / 2>(x + N / 2);
 }
 
 typedef uint32_t Vector __attribute__((ext_vector_type(4), aligned(2)));   // 16 bytes of logits from any on
@@ -170,7 +178,9 @@ __global__ __launch_bounds__(kWave) void beam_scan_kernel(const T *x, const uint
     load(ahead, begin + lane);
     if (ended != nullptr && ended[row] != 0) return;
 
-    float now[kLogits], m = neg_inf, s = 0.0f, of_set[kSets] = {neg_inf, neg_inf, neg_inf, neg_inf};
+    // m: the lane's largest logit; base: the wave's; s: the lane's sum of exp(x - base)
+    float now[kLogits], m = neg_inf, base = neg_inf, of_set[kSets] = {neg_inf, neg_inf, neg_inf, neg_inf};
+    double s = 0.0;
     float low = -3.4028234663852886e38f;   // entries are at least this (never -inf or NaN)
     uint32_t n = 0;
     auto take = [&](const Vector (&from)[U], uint32_t at, bool whole) {
@@ -232,22 +242,24 @@ __global__ __launch_bounds__(kWave) void beam_scan_kernel(const T *x, const uint
                 of_set[k] = fmaxf(of_set[k], of);
                 top = fmaxf(top, of);
             }
-            const float up = fmaxf(m, top);
-            if (wave_any(up == inf)) {
-                float add = 0.0f;
-#pragma unroll
-                for (uint32_t j = 0; j < kLogits; ++j) {
-                    const float y = now[j];
-                    add += y == inf ? 1.0f : y != y ? y : up == inf ? 0.0f : exp_below(y - (up == neg_inf ? 0.0f : up));
-                }
-                s = (m == up ? s : m == neg_inf || up == inf ? s * 0.0f : s * exp_below(m - up)) + add;
-            } else {
-                const float base = up == neg_inf ? 0.0f : up;
-                s *= exp_below(m - base);
-#pragma unroll
-                for (uint32_t j = 0; j < kLogits; ++j) s += exp_below(now[j] - base);
+            m = fmaxf(m, top);
+            if (wave_any(m > base)) {
+                const float next = wave_max(m);
+                if (base != neg_inf) s *= exp((double)base - (double)next);
+                base = next;
             }
-            m = up;
+            // A tile's terms in f32, tiles in f64: in one f32 the terms of flat rows, which
+            // all round the same way, left sums of 32003 off by 1e-5.
+            float term[kLogits];
+            if (base == inf) {
+#pragma unroll
+                for (uint32_t j = 0; j < kLogits; ++j) term[j] = now[j] == inf ? 1.0f : now[j] != now[j] ? now[j] : 0.0f;
+            } else {
+                const float from_base = base == neg_inf ? 0.0f : base;
+#pragma unroll
+                for (uint32_t j = 0; j < kLogits; ++j) term[j] = exp_below(now[j] - from_base);
+            }
+            s += (double)sum_of<kLogits>(term);
             largests[t * kWave + lane] = top;
         }
         // the bound, and the places that reach it
@@ -321,9 +333,8 @@ __global__ __launch_bounds__(kWave) void beam_scan_kernel(const T *x, const uint
     if (lane >= n) rank = lane;
     if (rank < a.pitch)
         a.entries[list * a.pitch + rank] = lane < n ? Entry{from_key((uint32_t)(mine >> 32)), ~(uint32_t)mine} : Entry{neg_inf, 0};
-    const float top = wave_max(m);
-    const double sum = wave_sum_f64((double)(s * (m == top ? 1.0f : exp_below(m - top))));
-    if (lane == 0) a.sums[list] = PartSum{sum, top, 0};
+    const double sum = wave_sum_f64(s);
+    if (lane == 0) a.sums[list] = PartSum{sum, base, 0};
 }
 
 // ---- of a group ----------------------------------------------------------------------
