@@ -140,6 +140,7 @@ typedef uint32_t Vector __attribute__((ext_vector_type(4), aligned(2)));   // 16
 constexpr uint32_t kLogits = 16, kTile = kLogits * kWave;   // of a lane and of a wave, at a time
 constexpr uint32_t kTiles = 16;                             // between two looks for candidates
 constexpr uint32_t kSets = 4;                               // of a lane's logits, each with its largest
+constexpr uint32_t kFewLanes = 8;                           // of several hits each, which a cut or two takes
 // Entries of a wave, and above how many they are cut to the best.
 constexpr uint32_t kSpare = 2 * kMaxKeep, kHeld = kSpare + kWave, kSlots = kHeld / kWave;
 
@@ -147,11 +148,13 @@ constexpr uint32_t kSpare = 2 * kMaxKeep, kHeld = kSpare + kWave, kSlots = kHeld
 // largest logit in LDS; the largest ones so far of `keep` lanes, or of sets of a lane's
 // logits, reach a bound, and only where a tile's lane reaches it are logits looked at
 // again, one lane for each such place. 256 rows of 128256 f32 (131 MB) 27 us, 4.8 TB/s,
-// where a copy of 1 GiB reaches 5.1; f16 17 us, bound by vector instructions (a quarter of
+// where a copy of 1 GiB reaches 5.1; f16 19 us, bound by vector instructions (a quarter of
 // them the exponentials, at a quarter of the rate). One tile each (16 x 8 x 32003 f16) 8.5
 // us: the chain of load, sum, bound, sort and store, 4 us of them for a wave alone. Measured
 // and left: candidates looked for in every tile (f32 31 us, f16 25), workgroups of four
-// waves (the same).
+// waves (the same). Logits that equal the bound are candidates too, the first `keep` of
+// them: all but three of 128256 at the type's lowest number 35 us (f32) and 26 (f16), where
+// each of them looked at took ten times as long.
 template <typename T>
 __global__ __launch_bounds__(kWave) void beam_scan_kernel(const T *x, const uint32_t *ended, uint32_t vocab, uint32_t per_part,
                                                           uint32_t keep, ScanArgs a) {
@@ -183,6 +186,10 @@ __global__ __launch_bounds__(kWave) void beam_scan_kernel(const T *x, const uint
     double s = 0.0;
     float low = -3.4028234663852886e38f;   // entries are at least this (never -inf or NaN)
     uint32_t n = 0;
+    // Places of earlier tiles with a logit of at least `counted`: once there are `keep`, one
+    // that equals it is behind them all.
+    uint32_t sure = 0;
+    float counted = low;
     auto take = [&](const Vector (&from)[U], uint32_t at, bool whole) {
 #pragma unroll
         for (uint32_t u = 0; u < U; ++u) {
@@ -202,6 +209,27 @@ __global__ __launch_bounds__(kWave) void beam_scan_kernel(const T *x, const uint
             for (uint32_t e = 0; e < E; ++e)
                 now[u * E + e] = v < end && v * E + e < vocab ? (float)x[v * E + e] : neg_inf;
         }
+    };
+    // Of the wave's hits that equal the bound, for each of a place's vectors, the first
+    // `keep` (places are in the order of their tokens).
+    auto first_equal = [&](uint32_t hits) {
+        uint32_t equal = 0;
+#pragma unroll
+        for (uint32_t j = 0; j < kLogits; ++j) equal |= now[j] == low ? 1u << j : 0u;
+        equal &= hits;
+#pragma unroll
+        for (uint32_t u = 0; u < U; ++u) {
+            const uint32_t its = (uint32_t)__builtin_popcount(equal >> u * E & ((1u << E) - 1));
+            uint32_t before = 0;
+#pragma unroll
+            for (uint32_t bit = 0; 1u << bit <= E; ++bit) before += lanes_below((its >> bit & 1) != 0, lane) << bit;
+#pragma unroll
+            for (uint32_t j = u * E; j < (u + 1) * E; ++j) {
+                if (before >= keep) hits &= ~(equal & 1u << j);
+                before += equal >> j & 1;
+            }
+        }
+        return hits;
     };
     // cuts the entries to the `keep` best
     auto cut = [&] {
@@ -278,12 +306,18 @@ __global__ __launch_bounds__(kWave) void beam_scan_kernel(const T *x, const uint
         const bool one = tiles == 1;   // (its logits are still in their lanes)
         uint32_t all = one ? kWave : 0;
         if (!one) {
+            if (counted != low) {
+                counted = low;
+                sure = 0;
+            }
+            const float above = from_key(key_of(low) + 1);
             wave_order();
             for (uint32_t t = 0; t < tiles; ++t) {
-                const bool reaches = largests[t * kWave + lane] >= low;
+                const bool reaches = largests[t * kWave + lane] >= (sure < keep ? low : above);
                 const uint32_t i = all + lanes_below(reaches, lane);
                 if (reaches) places[i] = (uint16_t)(t * kWave + lane);
                 all += lanes(reaches);
+                sure += lanes(reaches);
             }
             wave_order();
         }
@@ -300,6 +334,7 @@ __global__ __launch_bounds__(kWave) void beam_scan_kernel(const T *x, const uint
 #pragma unroll
             for (uint32_t j = 0; j < kLogits; ++j) hits |= now[j] >= low ? 1u << j : 0u;
             if (i + lane >= all) hits = 0;
+            if (lanes(__builtin_popcount(hits) > 2) > kFewLanes) hits = first_equal(hits);
             while (wave_any(hits != 0)) {
                 const uint32_t j = (uint32_t)__builtin_ctz(hits | 1u << (kLogits - 1));
                 // now[j], by the bits of j (chosen as conditions, the compiler makes a chain of
