@@ -84,7 +84,7 @@ __global__ __launch_bounds__(kThreads, P <= 64 ? 3 : P <= 128 ? 2 : 1) void kv_w
         vec8 (&x)[G] = to.x;
         f32x2 &ml = to.ml;
         const uint32_t r = min(step, steps - 1) * kStep + srow;
-        const size_t row = head * in_head + min(r, in_head - 1);
+        const size_t row = head * in_head + (count == a.n ? min(r, in_head - 1) : loaded_row(r, r % a.n, in_head, a.n, count));
         const S *src = a.q + row * c.dim;
         ml = a.row_ml[row];
         if (r >= in_head || r % a.n >= count) ml = f32x2{0.0f, 0.0f};

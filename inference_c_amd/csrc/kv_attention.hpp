@@ -78,14 +78,17 @@ template <typename S> __device__ inline uint32_t rows_there(Constant<SharedArgs<
     const uint32_t end = (b + 1) * a.c.heads < a.pairs ? a.count.n[b + 1] : a.last;
     return (end - a.count.n[b]) * a.own_rows;
 }
-// The row of q, the parts and the output that packed row r is (rows that are not there
-// repeat the last that is, or the first of all).
+// The packed row that a lane of row r (i of its query head) loads: of padding, and of rows
+// past the head, the last one of a query head that is there (count > 0), which is then in
+// the wave twice and changes nothing: what the padding holds is not looked at.
+__device__ inline uint32_t loaded_row(uint32_t r, uint32_t i, uint32_t in_head, uint32_t n, uint32_t count) {
+    return r < in_head ? r - i + min(i, count - 1) : in_head - n + count - 1;
+}
+// The row of q, the parts and the output that packed row r is.
 template <typename S>
-__device__ inline size_t shared_row(Constant<SharedArgs<S>> &a, uint32_t r, uint32_t b, uint32_t h, uint32_t in_head,
-                                    uint32_t count) {
-    r = min(r, in_head - a.n + max(count, 1u) - 1);
+__device__ inline size_t shared_row(Constant<SharedArgs<S>> &a, uint32_t r, uint32_t b, uint32_t h, uint32_t in_head) {
     if (a.own_rows == 0) return ((size_t)(a.first + b) * a.c.heads + h) * in_head + r;
-    const uint32_t m = r / a.own_rows, sequence = count != 0 ? a.count.n[b] + m : 0;
+    const uint32_t m = r / a.own_rows, sequence = a.count.n[b] + m;
     return ((size_t)sequence * a.c.heads + h) * a.own_rows + (r - m * a.own_rows);
 }
 
@@ -141,8 +144,8 @@ __device__ inline void load8(const float *row, uint32_t dim, uint32_t d, float (
     }
 }
 
-// How many keys packed row r sees (0 or fewer: none); padded rows and rows past
-// the head see all.
+// How many keys packed row r sees (0 or fewer: none); those that are loaded in the
+// place of padding and past the head see all, as the row that they repeat does.
 __device__ inline int seen_by(uint32_t i, bool live, uint32_t length, uint32_t count, int causal) {
     return causal && live ? (int)length - (int)count + (int)i + 1 : (int)length;
 }

@@ -199,9 +199,10 @@ __device__ __forceinline__ void rows_of(RowsOut<P, kMeet> &lds_o, RowsMl<kMeet> 
     const uint32_t end = min(begin + share, blocks), end_whole = min(end, whole);
     const uint32_t r = row0 + m, i = n == 1 ? 0 : r % n;
     const bool live = r < in_head && i < count;
-    size_t row = head * in_head + (r < in_head ? r : in_head - 1);   // (rows past the head repeat its last)
-    if constexpr (kBoth) row = ((size_t)own.sequence * heads + h) * in_head + min(r, in_head - n + max(count, 1u) - 1);
-    else if constexpr (kShared) row = shared_row(a, r, b, h, in_head, count);
+    const uint32_t loaded = loaded_row(r, i, in_head, n, count);
+    size_t row = head * in_head + loaded;
+    if constexpr (kBoth) row = ((size_t)own.sequence * heads + h) * in_head + loaded;
+    else if constexpr (kShared) row = shared_row(a, loaded, b, h, in_head);
     const int seen = seen_by(i, live, length, count, a.causal);
     Query<S, P> q;
     q.load(queries + row * c.dim, c.dim, g);

@@ -182,10 +182,12 @@ __device__ __forceinline__ void tiles_of(typename TilesLds<P>::Keys &ks, typenam
     const uint32_t b = pair / c.heads, h = pair % c.heads, seq = a.first + b;
     const size_t head = (size_t)seq * c.heads + h;
     const uint32_t length = c.length[seq], count = rows_there(a, b);
+    if (count == 0) return;
     const uint32_t r = row_block * kTileRows + wave * 32 + col, i = r % a.n;
     const bool live = r < in_head && i < count;
-    size_t row = head * in_head + min(r, in_head - 1);
-    if constexpr (kShared) row = shared_row(a, r, b, h, in_head, count);
+    const uint32_t loaded = loaded_row(r, i, in_head, a.n, count);
+    size_t row = head * in_head + loaded;
+    if constexpr (kShared) row = shared_row(a, loaded, b, h, in_head);
     const int seen = seen_by(i, live, length, count, a.causal);
     // keys that some row of the workgroup, and that every row of the wave, sees
     int most = live ? seen : 0, least = live ? seen : (int)length;
