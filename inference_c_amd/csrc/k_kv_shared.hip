@@ -7,7 +7,10 @@
 // and over each sequence's own tokens as in attention without a prefix. A softmax over
 // both is their parts' join (kv_join_kernel; kv_fold_kernel for many parts of few rows). The passes are one launch: neither waits
 // for the other, and where the prefix is bound by its products (tiles) and the own
-// tokens by memory (rows), a CU has one of each.
+// tokens by memory (rows), a CU has one of each. Padded rows lie among a group's packed
+// ones; they are not loaded, and a workgroup that has no others ends at once (4 x 512
+// rows on 8000 tokens 300 us, of which 512, 400, 300 and 1 are there 247, one each of three
+// 221).
 #include "kv_rows.hpp"
 #include "kv_tiles.hpp"
 
@@ -112,6 +115,11 @@ __global__ __launch_bounds__(2 * kThreads) void kv_shared_close_kernel(Both<S>) 
                                        OwnRows{sequence, both.pass[1].count.n[b]});
 }
 
+// Counts of sequences where the kernels of a call of more than a launch's find them.
+__global__ __launch_bounds__(kBatchPerLaunch) void kv_counts_kernel(uint32_t *counts, uint32_t batch, Counts of) {
+    if (threadIdx.x < batch) counts[threadIdx.x] = of.n[threadIdx.x];
+}
+
 // ---- the parts' join ------------------------------------------------------------------------
 
 struct JoinArgs {
@@ -199,7 +207,7 @@ struct SharedPlan {
     bool close;      // both by one workgroup
     bool together;   // in one launch
     uint32_t n;      // rows of a prefix's head
-    size_t rows, o_bytes, ml_bytes;
+    size_t rows, o_bytes, ml_bytes, counts_bytes;
 };
 
 Pass pass_of(const View &c, bool tiles, uint32_t batch, uint32_t in_head, uint32_t longest, uint64_t workgroups) {
@@ -240,6 +248,12 @@ bool close_fits(bool f32, const PrefixShape &ps, const View &c, const AttentionS
            (uint64_t)a.batch * c.heads * row_groups <= (twice ? 2 : 1) * kCloseWorkgroups;
 }
 
+bool padded(const AttentionShape &a) {
+    for (uint32_t b = 0; a.counts != nullptr && b < a.batch; ++b)
+        if (a.counts[b] < a.n) return true;
+    return false;
+}
+
 SharedPlan plan_of(bool f32, const View &prefix, const PrefixShape &ps, const View &c, const AttentionShape &a) {
     SharedPlan p{};
     const uint32_t widest = widest_of(c), own_rows = a.q_heads / c.heads * a.n;
@@ -270,6 +284,7 @@ SharedPlan plan_of(bool f32, const View &prefix, const PrefixShape &ps, const Vi
     const size_t parts = p.prefix.parts + p.own.parts;
     p.o_bytes = whole256(parts * p.rows * c.vdim * 4);
     p.ml_bytes = whole256(parts * p.rows * sizeof(f32x2));
+    p.counts_bytes = padded(a) && a.batch > kBatchPerLaunch ? whole256(a.batch * sizeof(uint32_t)) : 0;
     return p;
 }
 
@@ -400,6 +415,23 @@ hipError_t run(const View &prefix, const PrefixShape &ps, const View &c, const A
         return launch(both, widest_of(c), grid, Kernels{{tiles0, tiles1}, p.own.solo, held > kStreamBytes}, s);
     };
 
+    auto batch_from = [&](uint32_t first) { return sh.batch - first < kBatchPerLaunch ? sh.batch - first : kBatchPerLaunch; };
+    auto take_counts = [&](uint32_t first) {
+        for (uint32_t b = 0; b < batch_from(first); ++b) own.count.n[b] = sh.counts ? sh.counts[first + b] : sh.n;
+    };
+    take_counts(0);
+    over.padded = padded(sh) ? sh.n : 0;
+    if (p.counts_bytes != 0) {
+        uint32_t *const counts = reinterpret_cast<uint32_t *>(static_cast<char *>(workspace) + p.o_bytes + p.ml_bytes);
+        for (uint32_t first = 0; first < sh.batch; first += kBatchPerLaunch) {
+            take_counts(first);
+            kv_counts_kernel<<<1, kBatchPerLaunch, 0, s>>>(counts + first, batch_from(first), own.count);
+            const hipError_t status = hipGetLastError();
+            if (status != hipSuccess) return status;
+        }
+        over.counts = counts;
+    }
+
     Cursor<S> of_prefix{prefix, p.prefix}, of_own{c, p.own};
     uint32_t sequence = 0;   // where the next group starts
     while (!of_prefix.done() || !of_own.done()) {
@@ -421,8 +453,7 @@ hipError_t run(const View &prefix, const PrefixShape &ps, const View &c, const A
             both.first = grid = 0;
         }
         if (!of_own.done()) {
-            for (uint32_t b = 0; b < of_own.batch(); ++b)
-                own.count.n[b] = sh.counts ? sh.counts[of_own.first + b] : sh.n;
+            take_counts(of_own.first);
             grid += of_own.next(own);
         }
         if (grid == 0) continue;
@@ -435,8 +466,8 @@ hipError_t run(const View &prefix, const PrefixShape &ps, const View &c, const A
     own.part_o = over.part_o;
     own.part_ml = over.part_ml;
     for (uint32_t first = 0; first < sh.batch; first += kBatchPerLaunch) {
-        const uint32_t batch = sh.batch - first < kBatchPerLaunch ? sh.batch - first : kBatchPerLaunch;
-        for (uint32_t b = 0; b < batch; ++b) own.count.n[b] = sh.counts ? sh.counts[first + b] : sh.n;
+        const uint32_t batch = batch_from(first);
+        take_counts(first);
         const uint32_t per_sequence = sh.q_heads * sh.n;
         hipError_t status = hipSuccess;
         if (parts > 16 && p.rows <= kWideRows) {
@@ -472,7 +503,7 @@ hipError_t run(const View &prefix, const PrefixShape &ps, const View &c, const A
 size_t attention_shared_workspace(bool f32, const View &prefix, const PrefixShape &p, const View &c,
                                   const AttentionShape &a) {
     const SharedPlan plan = plan_of(f32, prefix, p, c, a);
-    return plan.o_bytes + plan.ml_bytes;
+    return plan.o_bytes + plan.ml_bytes + plan.counts_bytes;
 }
 
 hipError_t attention_shared(bool f32, const View &prefix, const PrefixShape &p, const View &c, const AttentionShape &a,

@@ -61,6 +61,10 @@ template <typename S> struct SharedArgs : Args<S> {
     uint32_t own_rows;   // packed rows of a sequence and head
     uint32_t last;       // where the last group of the launch ends
     uint32_t columns;    // of a head, workgroups of the rows kernel
+    // Over a prefix, where some of the query heads' n rows are padding: n (else 0), and
+    // every sequence's count (null: the other pass's `count`, which follows, has them).
+    uint32_t padded;
+    const uint32_t *counts;
 };
 // Arguments where a kernel finds them: memory that nothing writes.
 template <typename A> using Constant = const __attribute__((address_space(4))) A;
@@ -90,6 +94,18 @@ __device__ inline size_t shared_row(Constant<SharedArgs<S>> &a, uint32_t r, uint
     if (a.own_rows == 0) return ((size_t)(a.first + b) * a.c.heads + h) * in_head + r;
     const uint32_t m = r / a.own_rows, sequence = a.count.n[b] + m;
     return ((size_t)sequence * a.c.heads + h) * a.own_rows + (r - m * a.own_rows);
+}
+
+// Whether packed row r over a prefix is no padding.
+template <typename S> __device__ inline bool no_padding(Constant<SharedArgs<S>> &a, uint32_t r, uint32_t b) {
+    const uint32_t m = r / a.own_rows, sequence = a.count.n[b] + m, i = (r - m * a.own_rows) % a.padded;
+    return i < (a.counts != nullptr ? a.counts[sequence] : (&a)[1].count.n[sequence]);
+}
+// The row of one of the lanes in `some`.
+__device__ inline size_t row_among(size_t row, uint64_t some) {
+    const int lane = __builtin_ctzll(some);
+    return (size_t)(uint32_t)__builtin_amdgcn_readlane((int)(row >> 32), lane) << 32 |
+           (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)row, lane);
 }
 
 // A block's Meta through the scalar cache (no kernel writes it while one that

@@ -198,11 +198,19 @@ __device__ __forceinline__ void rows_of(RowsOut<P, kMeet> &lds_o, RowsMl<kMeet> 
     const uint32_t blocks = ((uint32_t)max(most, 0) + kTokens - 1) / kTokens;
     const uint32_t end = min(begin + share, blocks), end_whole = min(end, whole);
     const uint32_t r = row0 + m, i = n == 1 ? 0 : r % n;
-    const bool live = r < in_head && i < count;
+    bool live = r < in_head && i < count;
     const uint32_t loaded = loaded_row(r, i, in_head, n, count);
     size_t row = head * in_head + loaded;
     if constexpr (kBoth) row = ((size_t)own.sequence * heads + h) * in_head + loaded;
-    else if constexpr (kShared) row = shared_row(a, loaded, b, h, in_head);
+    else if constexpr (kShared) {
+        row = shared_row(a, loaded, b, h, in_head);
+        if (a.padded != 0) {   // (all of the workgroup's waves have the same rows)
+            live = live && no_padding(a, loaded, b);
+            const uint64_t some = __builtin_amdgcn_ballot_w64(live);
+            if (some == 0) return;
+            row = live ? row : row_among(row, some);
+        }
+    }
     const int seen = seen_by(i, live, length, count, a.causal);
     Query<S, P> q;
     q.load(queries + row * c.dim, c.dim, g);

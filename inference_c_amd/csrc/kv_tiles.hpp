@@ -184,13 +184,22 @@ __device__ __forceinline__ void tiles_of(typename TilesLds<P>::Keys &ks, typenam
     const uint32_t length = c.length[seq], count = rows_there(a, b);
     if (count == 0) return;
     const uint32_t r = row_block * kTileRows + wave * 32 + col, i = r % a.n;
-    const bool live = r < in_head && i < count;
+    bool live = r < in_head && i < count;
     const uint32_t loaded = loaded_row(r, i, in_head, a.n, count);
     size_t row = head * in_head + loaded;
-    if constexpr (kShared) row = shared_row(a, loaded, b, h, in_head);
+    bool loads = true;   // (a wave of padding alone does not)
+    if constexpr (kShared) {
+        row = shared_row(a, loaded, b, h, in_head);
+        if (a.padded != 0) {
+            live = live && no_padding(a, loaded, b);
+            const uint64_t some = __builtin_amdgcn_ballot_w64(live);
+            loads = some != 0;
+            if (loads && !live) row = row_among(row, some);
+        }
+    }
     const int seen = seen_by(i, live, length, count, a.causal);
     // keys that some row of the workgroup, and that every row of the wave, sees
-    int most = live ? seen : 0, least = live ? seen : (int)length;
+    int most = live ? max(seen, 0) : kShared ? -1 : 0, least = live ? seen : (int)length;
 #pragma unroll
     for (int d = 1; d < 32; d *= 2) {
         most = max(most, __shfl_xor(most, d, kWave));
@@ -203,6 +212,7 @@ __device__ __forceinline__ void tiles_of(typename TilesLds<P>::Keys &ks, typenam
 #pragma unroll
     for (uint32_t w = 1; w < kWaves; ++w) most = max(most, wave_most[w]);
     most = __builtin_amdgcn_readfirstlane(most);
+    if (kShared && most < 0) return;   // padding alone
     const uint32_t blocks = ((uint32_t)max(most, 0) + kTokens - 1) / kTokens, whole = length / kTokens;
     const uint32_t share = (blocks + a.parts - 1) / a.parts;
     const uint32_t begin = min(part * share, blocks), end = min(begin + share, blocks), tiles = end - begin;
@@ -210,8 +220,8 @@ __device__ __forceinline__ void tiles_of(typename TilesLds<P>::Keys &ks, typenam
     const uint32_t open_first = end > whole ? 1 : 0;
     auto block_of = [&](uint32_t s) { return open_first && s == 0 ? whole : min(begin + s - open_first, c.blocks - 1); };
 
-    TileQuery<S, P> q;
-    q.load(a.q + row * c.dim, c.dim, half, a.scale2 > 0.0 ? 1.0f : a.scale2 < 0.0 ? -1.0f : 0.0f);
+    TileQuery<S, P> q{};
+    if (loads) q.load(a.q + row * c.dim, c.dim, half, a.scale2 > 0.0 ? 1.0f : a.scale2 < 0.0 ? -1.0f : 0.0f);
     const Meta *const meta = c.meta + head * c.blocks;
     const uint8_t *const kcodes = c.k + head * c.blocks * kTokens * c.kp;
     const uint8_t *const vcodes = c.v + head * c.blocks * kTokens * c.vp;

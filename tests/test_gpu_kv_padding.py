@@ -1,11 +1,11 @@
-"""Padded query rows of attention over the cache: what they hold has no effect on any
-bit of the rows that are there, nor on the weights."""
+"""Padded query rows of attention over the cache and over a shared prefix: what they
+hold has no effect on any bit of the rows that are there, nor on the weights."""
 import numpy as np
 import pytest
 
 from tests.test_gpu_kv_attention import attend as attend_plain
 from tests.test_gpu_kv_cache import DTYPES
-from tests.test_gpu_kv_shared import pair_of
+from tests.test_gpu_kv_shared import attend, pair_of, run
 
 pytestmark = pytest.mark.gpu
 
@@ -26,6 +26,19 @@ def same(results):
             assert (a is None and b is None) or np.array_equal(a.view(np.uint8), b.view(np.uint8)), f"padding of {kind}"
 
 
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("before,lengths,heads,n,counts", [
+    (100, [40, 30, 3, 20], 4, 3, [3, 1, 0, 2]),                    # one workgroup for both
+    (1500, [300, 200, 400, 100], 8, 5, [5, 2, 0, 1]),              # rows in parts
+    (2500, [150] * 10, 16, 75, [75, 75, 20, 1, 0, 75, 3, 40, 75, 75]),    # tiles over the prefix
+    (2000, [1500, 1300], 16, 900, [333, 900])], ids=["close", "rows", "mixed", "tiles"])
+def test_over_a_prefix(sdk, before, lengths, heads, n, counts, dtype):
+    kv = 2 if heads < 16 else 4
+    prefix, own = pair_of(sdk, kv, (128, 128), [before], 1), pair_of(sdk, kv, (128, 128), lengths, 2)
+    q = own.rng.standard_normal((len(lengths), heads, n, 128)).astype(DTYPES[dtype])
+    same([(kind, [attend(prefix, own, x, None, 0.3, True, counts)]) for kind, x in paddings(own.rng, q, counts)])
+
+
 @pytest.mark.parametrize("weighted", [False, True], ids=["", "weights"])
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
 @pytest.mark.parametrize("lengths,heads,n,counts", [
@@ -36,3 +49,31 @@ def test_over_own_tokens(sdk, lengths, heads, n, counts, dtype, weighted):
     q = own.rng.standard_normal((len(lengths), heads, n, 128)).astype(DTYPES[dtype])
     w0 = np.zeros((len(lengths), 4, max(lengths)), np.float32) if weighted else None
     same([(kind, attend_plain(sdk, own.cache, x, 0.3, True, counts, w0, 128)) for kind, x in paddings(own.rng, q, counts)])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_more_sequences_than_one_launch_takes(sdk, dtype):
+    """Padding of other sequences than a launch's own tokens are of; whole sequences,
+    groups and tiles of padding."""
+    rng = np.random.default_rng(4)
+    members = [0, 290, 3, 30, 0, 1]
+    prefix = pair_of(sdk, 1, (32, 32), [5, 700, 64, 130, 9, 0], 5)
+    own = pair_of(sdk, 1, (32, 32), [int(n) for n in rng.integers(0, 70, sum(members))], 6)
+    counts = [int(c) for c in rng.integers(0, 5, sum(members))]
+    counts[20:60] = [0] * 40
+    counts[290:293] = [0] * 3
+    run(prefix, own, dtype, 2, 4, members, causal=False, counts=counts, what="few rows")
+    q = own.rng.standard_normal((sum(members), 2, 4, 32)).astype(DTYPES[dtype])
+    same([(kind, [attend(prefix, own, x, members, 0.3, True, counts)]) for kind, x in paddings(own.rng, q, counts)])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_tiles_of_padding(sdk, dtype):
+    """Packed tiles, and waves of them, without a row that is there, in 300 sequences."""
+    rng = np.random.default_rng(7)
+    prefix, own = pair_of(sdk, 2, (64, 64), [1900], 8), pair_of(sdk, 2, (64, 64), [30 + b % 5 for b in range(300)], 9)
+    counts = [0 if b % 60 < 40 else int(c) for b, c in enumerate(rng.integers(0, 25, 300))]
+    counts[299] = 24
+    run(prefix, own, dtype, 2, 24, counts=counts, what="tiles")
+    q = own.rng.standard_normal((300, 2, 24, 64)).astype(DTYPES[dtype])
+    same([(kind, [attend(prefix, own, x, None, 0.3, True, counts)]) for kind, x in paddings(own.rng, q, counts)])
