@@ -125,8 +125,8 @@ __global__ __launch_bounds__(kBatchPerLaunch) void kv_counts_kernel(uint32_t *co
 struct JoinArgs {
     const float *part_o;
     const f32x2 *part_ml;
-    size_t rows, first_row;    // of all sequences; where the launch's begin
-    uint32_t parts, vdim, all;   // all: rows of the launch
+    size_t rows, first_row;    // of all sequences; of the first of `count`
+    uint32_t parts, vdim, from, all;   // the launch's rows: from first_row + from on, `all` of them
     FastDiv per_row;             // threads of a row, four elements each
     bool padded;                 // some rows are padding, by `count`
     FastDiv n, per_sequence;     // rows of a query head, and of a sequence
@@ -140,8 +140,9 @@ struct JoinArgs {
 template <typename S, uint32_t kHeld> __global__ __launch_bounds__(kThreads) void kv_join_kernel(S *out, JoinArgs a) {
     const uint32_t i = blockIdx.x * kThreads + threadIdx.x, r = fast_div(i, a.per_row), d = 4 * (i - r * a.per_row.divisor);
     if (r >= a.all) return;
-    const size_t row = a.first_row + r;
-    if (a.padded && r - fast_div(r, a.n) * a.n.divisor >= a.count.n[fast_div(r, a.per_sequence)]) return;
+    const uint32_t at = a.from + r;
+    const size_t row = a.first_row + at;
+    if (a.padded && at - fast_div(at, a.n) * a.n.divisor >= a.count.n[fast_div(at, a.per_sequence)]) return;
     const uint32_t last = a.parts - 1;
     auto load = [&](uint32_t s) {
         const float *const src = a.part_o + ((size_t)s * a.rows + row) * a.vdim + d;
@@ -475,14 +476,12 @@ hipError_t run(const View &prefix, const PrefixShape &ps, const View &c, const A
             own.pairs = batch * c.heads;
             status = launch_fold<S>(own, parts, false, 0, true, s);
         } else {
-            // (whole sequences, fewer than 2^32 threads)
-            const uint32_t threads = (c.vdim + 3) / 4, most = (1u << 31) / threads / per_sequence;
-            for (uint32_t b = 0; b < batch && status == hipSuccess;) {
-                const uint32_t now = batch - b < most ? batch - b : most < 1 ? 1 : most;
-                JoinArgs j{own.part_o, own.part_ml, p.rows, (size_t)(first + b) * per_sequence, parts, c.vdim,
-                           now * per_sequence, make_fast_div(threads), sh.counts != nullptr, make_fast_div(sh.n),
-                           make_fast_div(per_sequence), {}};
-                for (uint32_t i = 0; i < now; ++i) j.count.n[i] = own.count.n[b + i];
+            const uint32_t threads = (c.vdim + 3) / 4, most = join_rows(c.vdim), rows = batch * per_sequence;
+            JoinArgs j{own.part_o, own.part_ml, p.rows, (size_t)first * per_sequence, parts, c.vdim, 0, 0,
+                       make_fast_div(threads), sh.counts != nullptr, make_fast_div(sh.n), make_fast_div(per_sequence),
+                       own.count};
+            for (; j.from < rows && status == hipSuccess; j.from += j.all) {
+                j.all = rows - j.from < most ? rows - j.from : most;
                 auto join = [&](auto kernel) {
                     kernel<<<(j.all * threads + kThreads - 1) / kThreads, kThreads, 0, s>>>(static_cast<S *>(output), j);
                 };
@@ -490,7 +489,6 @@ hipError_t run(const View &prefix, const PrefixShape &ps, const View &c, const A
                 else if (parts <= 4) join(kv_join_kernel<S, 4>);
                 else join(kv_join_kernel<S, 8>);
                 status = hipGetLastError();
-                b += now;
             }
         }
         if (status != hipSuccess) return status;

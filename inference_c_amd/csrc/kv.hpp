@@ -103,6 +103,9 @@ struct PrefixShape {
     uint32_t batch, most, longest;
     const uint32_t *members;
 };
+// Rows that a launch of its parts' join takes, a thread for each four of their elements:
+// fewer than 2^32 threads.
+constexpr uint32_t join_rows(uint32_t vdim) { return (1u << 31) / ((vdim + 3) / 4); }
 size_t attention_shared_workspace(bool f32, const View &prefix, const PrefixShape &p, const View &c,
                                   const AttentionShape &a);
 hipError_t attention_shared(bool f32, const View &prefix, const PrefixShape &p, const View &c, const AttentionShape &a,

@@ -113,7 +113,7 @@ int reorder(TensorKvCache *c, Buf parents, char *error, size_t capacity) {
                   "cache reorder: kernel launch", error, capacity) ? 1 : 0;
 }
 
-// Query rows of a call, at most: its launches hold fewer than 2^32 threads.
+// Query rows of a call, at most: a pass's launch holds fewer than 2^32 threads.
 constexpr size_t kMaxSharedRows = size_t{1} << 26;
 
 int attention_shared(TensorDType dtype, const TensorKvCache *prefix, const TensorKvCache *c, Buf query,
