@@ -4,9 +4,7 @@
 // (k_kv_shared.hip).
 #include "kv_handle.hpp"
 
-#include <climits>
 #include <cmath>
-#include <cstdlib>
 #include <memory>
 #include <new>
 
