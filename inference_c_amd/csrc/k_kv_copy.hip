@@ -103,7 +103,10 @@ struct ReorderArgs {
 // workgroup does kColumns of its 16 bytes' columns, kAhead of them at once. Measured (us,
 // 16 x 8 x 850 and 4 groups of 16 x 1000): one column 57 and 56, two one after another 54
 // and 59, four 53 and 49, four by twos 50 and 50, eight by twos 53 and 55; 32 groups of 4 x
-// 100 tokens 10.5 one by one, 8.7 by twos.
+// 100 tokens 10.5 one by one, 8.7 by twos. More than 16 beams run short of scalar registers
+// for their parents, and 64 of vector registers too (a wave per SIMD, and spills): 128
+// sequences of 1000 tokens, of which 114 to 125 move, in groups of 8 78 us, of 16 103, of 32
+// 119 (4.3 TB/s), of 64 266 (1.9 TB/s).
 constexpr uint32_t kColumns = 4, kColumn = kThreads * 16;
 template <uint32_t kBeams>
 __global__ __launch_bounds__(kThreads) void kv_reorder_kernel(ReorderArgs a) {
