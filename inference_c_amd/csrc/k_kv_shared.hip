@@ -63,9 +63,8 @@ __global__ __launch_bounds__(kThreads) void kv_shared_solo_kernel(Both<S>) {
 
 // Both by tiles. Four sequences' 512 rows behind 8000 tokens, 32/8 heads of 128, f16: 285 us
 // (975 TFLOP/s; 330 in the first calls, before the clock settles), bound as kv_tiles_kernel
-// is. A pass over own tokens that goes on over the
-// prefix, without parts, took 344 us against 322 and the join's 16 then: its workgroups end all
-// at once.
+// is. A pass over own tokens that goes on over the prefix, without parts, took 344 us against
+// 322 and the join's 16: its workgroups end all at once.
 template <typename S, uint32_t P>
 __global__ __launch_bounds__(kThreads, tiles_twice(sizeof(S) == 4, P) ? 2 : 1) void kv_shared_tiles_kernel(Both<S>) {
     __shared__ __attribute__((aligned(16))) typename TilesLds<P>::Keys ks;

@@ -1,9 +1,13 @@
 """Padded query rows of attention over the cache and over a shared prefix: what they
 hold has no effect on any bit of the rows that are there, nor on the weights."""
+import ctypes
+
 import numpy as np
 import pytest
 
-from tests.test_gpu_kv_attention import attend as attend_plain
+from tests import beam_model
+from tests.kv_model import u32s
+from tests.test_gpu_kv_attention import attend as attend_plain, compare
 from tests.test_gpu_kv_cache import DTYPES
 from tests.test_gpu_kv_shared import attend, pair_of, run
 
@@ -77,3 +81,44 @@ def test_tiles_of_padding(sdk, dtype):
     run(prefix, own, dtype, 2, 24, counts=counts, what="tiles")
     q = own.rng.standard_normal((300, 2, 24, 64)).astype(DTYPES[dtype])
     same([(kind, [attend(prefix, own, x, None, 0.3, True, counts)]) for kind, x in paddings(own.rng, q, counts)])
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("batch", [40, 300])
+def test_recorded(sdk, batch, dtype):
+    """Two recorded calls with other paddings: each keeps its own, whatever eager calls
+    with others do between the replays."""
+    hip, stream = sdk.lib, ctypes.c_void_p(sdk.stream())
+    rng = np.random.default_rng(10)
+    prefix = pair_of(sdk, 1, (32, 32), [900], 11, capacity=1200)
+    own = pair_of(sdk, 1, (32, 32), [int(n) for n in rng.integers(5, 40, batch)], 12, capacity=200)
+    q = rng.standard_normal((batch, 2, 5, 32)).astype(DTYPES[dtype])
+    given, runs = sdk.from_numpy(q), []
+    for _ in range(2):
+        counts = [int(c) for c in rng.integers(0, 6, batch)]
+        out = sdk.from_numpy(np.full(q.shape, 99, q.dtype))
+        call = (f"tensor_kv_cache_attention_shared_{dtype}", prefix.cache, own.cache, given, None, u32s(counts), 0.2, 0, out)
+        sdk.call(*call)
+        sdk.synchronize()
+        graph, exe = ctypes.c_void_p(), ctypes.c_void_p()
+        assert hip.hipStreamBeginCapture(stream, 2) == 0
+        try:
+            sdk.call(*call)
+        finally:
+            assert hip.hipStreamEndCapture(stream, ctypes.byref(graph)) == 0
+        assert hip.hipGraphInstantiate(ctypes.byref(exe), graph, None, None, ctypes.c_size_t(0)) == 0
+        assert hip.hipGraphDestroy(graph) == 0
+        runs.append((exe, counts, out))
+    for replay in range(3):
+        own.append(20)
+        for _, _, out in runs:
+            out.upload(np.full(q.shape, 99, q.dtype))
+        for exe, _, _ in runs:
+            assert hip.hipGraphLaunch(exe, stream) == 0
+        attend(prefix, own, q, None, 0.2, False, [(b + replay) % 6 for b in range(batch)])
+        model = beam_model.joined(prefix.model, own.model, [batch])
+        for _, counts, out in runs:
+            compare(model, q, 0.2, False, counts, out.download(), what=f"replay {replay}")
+    sdk.synchronize()
+    for exe, _, _ in runs:
+        assert hip.hipGraphExecDestroy(exe) == 0
